@@ -71,6 +71,17 @@ class ModelConfig(ctypes.Structure):
                 ("swiglu_limit", ctypes.c_float)]
 
 
+class RopeArgs(ctypes.Structure):
+    """Mirror of gptoss_rope_args_t."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out", "k_cache", "v_cache", "pos",
+                                               "slots", "inv_freq")] + \
+               [(n, ctypes.c_longlong) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride",
+                                                 "k_cache_stride", "v_cache_stride", "n_slots")] + \
+               [("concentration", ctypes.c_float)] + \
+               [(n, ctypes.c_int) for n in ("n_rows", "n_q_heads", "n_kv_heads", "head_dim",
+                                            "rotary_dim", "interleaved", "angle_f32", "dtype")]
+
+
 _lib = None
 
 
@@ -135,6 +146,8 @@ def load_library() -> ctypes.CDLL:
         "gptoss_decode_set_tensor": (c_int, [vp, c_char_p, c_int, vp, c_int, c_int]),
         "gptoss_decode_set_kv": (c_int, [vp, c_int, c_int, c_int, c_int, c_int, vp, vp]),
         "gptoss_decode_get_kv": (c_int, [vp, c_int, c_int, c_int, c_int, c_int, vp, vp]),
+        "gptoss_decode_rope_table": (c_int, [c_int, ctypes.c_float, ctypes.c_float, c_int, vp, fp]),
+        "gptoss_decode_rope_append": (c_int, [ctypes.POINTER(RopeArgs), vp]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(lib, name)
@@ -172,6 +185,107 @@ def permute_static(slot_expert, slot_weight, n_rows, top_k, n_experts, expert_of
                                        _ptr(sorted_weight), _ptr(row_of), ctypes.c_void_p(stream))
     if rc != GPTOSS_OK:
         raise MoeError(rc, lib.gptoss_moe_last_error(None).decode())
+
+
+# -- the handle-free operators of a prompt pass and of a drawn token
+_DTYPE_CODES = {"torch.bfloat16": 0, "torch.float16": 1, "torch.float32": 2}
+
+
+def _check_op(lib, rc):
+    if rc != GPTOSS_OK:
+        raise MoeError(rc, (lib.gptoss_decode_last_error(None) or b"").decode())
+
+
+def _dtype_code(t, what):
+    code = _DTYPE_CODES.get(str(t.dtype))
+    if code is None:
+        raise TypeError(f"{what}: element type {t.dtype} is not supported")
+    return code
+
+
+def _vector(t, what, dtype, n, device):
+    """Address of a contiguous 1-D tensor of n elements (None stays None)."""
+    if t is None:
+        return None
+    if str(t.dtype) != dtype:
+        raise TypeError(f"{what} must be {dtype}, not {t.dtype}")
+    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous with {n} elements, not {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, expected {device}")
+    return t.data_ptr()
+
+
+def _rows(t, what, dtype, device, heads=None, head_dim=None):
+    """(address, row stride) of a [rows, heads, head_dim] tensor with contiguous heads."""
+    if t is None:
+        return None, 0
+    if t.dtype != dtype:
+        raise TypeError(f"{what} must be {dtype}, not {t.dtype}")
+    if t.dim() != 3 or (heads is not None and tuple(t.shape[1:]) != (heads, head_dim)):
+        raise ValueError(f"{what} must be [rows, {heads}, {head_dim}], not {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, expected {device}")
+    rows, h, d = t.shape
+    s0, s1, s2 = t.stride()
+    if (d > 1 and s2 != 1) or (h > 1 and s1 != d):
+        raise ValueError(f"{what}: the heads of a row must be contiguous (strides {t.stride()})")
+    return t.data_ptr(), (s0 if rows > 1 else h * d)
+
+
+def _on_gpu(t, what):
+    if not t.is_cuda:
+        raise ValueError(f"{what} must be on a GPU, it is on {t.device}")
+    return t.device
+
+
+def rope_table(rotary_dim, theta, scaling_factor=1.0, initial_context_length=4096):
+    """gptoss_decode_rope_table: (inv_freq float32 [rotary_dim / 2], concentration)."""
+    lib = load_library()
+    inv = np.empty(max(rotary_dim // 2, 0), dtype=np.float32)
+    conc = ctypes.c_float()
+    _check_op(lib, lib.gptoss_decode_rope_table(rotary_dim, theta, scaling_factor,
+                                                initial_context_length, _ptr(inv),
+                                                ctypes.byref(conc)))
+    return inv, float(conc.value)
+
+
+def rope_append(q, k, v, pos, inv_freq, q_out=None, k_cache=None, v_cache=None, slots=None,
+                concentration=1.0, interleaved=False, angle_f32=False, stream=0):
+    """gptoss_decode_rope_append: rotary positions on q and k, k and v stored at their cache
+    rows.  q [rows, heads, head_dim], k and v [rows, kv heads, head_dim] (any row stride, heads
+    contiguous; each may be None) in bf16, fp16 or fp32; k_cache / v_cache [slots, kv heads,
+    head_dim]; pos int32 [rows] (< 0: row skipped); slots int64 [rows] or None (row i to cache
+    row i); inv_freq float32 [rotary_dim / 2].  q_out may be q, and without slots k_cache may
+    be k.  All tensors are on one GPU, `stream` is a stream of it (0: its default stream)."""
+    lib = load_library()
+    first = next((t for t in (q, k, v) if t is not None), None)
+    if first is None:
+        raise ValueError("q, k and v are all None")
+    dev, dtype, rows, d = _on_gpu(first, "input"), first.dtype, first.shape[0], first.shape[-1]
+    kv = k if k is not None else v
+    hq, hkv = (0 if q is None else q.shape[1]), (0 if kv is None else kv.shape[1])
+    qp, qs = _rows(q, "q", dtype, dev, hq, d)
+    kp, ks = _rows(k, "k", dtype, dev, hkv, d)
+    vp, vs = _rows(v, "v", dtype, dev, hkv, d)
+    qop, qos = _rows(q_out, "q_out", dtype, dev, hq, d)
+    kcp, kcs = _rows(k_cache, "k_cache", dtype, dev, hkv, d)
+    vcp, vcs = _rows(v_cache, "v_cache", dtype, dev, hkv, d)
+    for name, t in (("k", k), ("v", v)):
+        if t is not None and t.shape[0] != rows:
+            raise ValueError(f"{name} has {t.shape[0]} rows, expected {rows}")
+    if q_out is not None and q_out.shape[0] != rows:
+        raise ValueError(f"q_out has {q_out.shape[0]} rows, expected {rows}")
+    caches = [t.shape[0] for t in (k_cache, v_cache) if t is not None]
+    if len(set(caches)) > 1:
+        raise ValueError("k_cache and v_cache have different numbers of rows")
+    args = RopeArgs(qp, kp, vp, qop, kcp, vcp, _vector(pos, "pos", "torch.int32", rows, dev),
+                    _vector(slots, "slots", "torch.int64", rows, dev),
+                    _vector(inv_freq, "inv_freq", "torch.float32", inv_freq.shape[0], dev),
+                    qs, ks, vs, qos, kcs, vcs, caches[0] if caches else 0, concentration, rows, hq,
+                    hkv, d, 2 * inv_freq.shape[0], interleaved, angle_f32,
+                    _dtype_code(first, "input"))
+    _check_op(lib, lib.gptoss_decode_rope_append(ctypes.byref(args), ctypes.c_void_p(stream)))
 
 
 class MoeEngine:

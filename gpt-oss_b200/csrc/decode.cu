@@ -24,11 +24,13 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <atomic>
 #include <string>
 #include <vector>
 
 #include "../../include/gptoss_decode_b200.h"
 #include "common.cuh"
+#include "decode_ops.h"
 #include "engine.h"
 #include "gemm_epilogue.cuh"
 
@@ -448,6 +450,33 @@ static int dfail(gptoss_decode *h, int code, const char *fmt, ...) {
   return code;
 }
 
+namespace gptoss {
+
+int decode_error(int code, const char *fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  g_decode_create_err = buf;
+  return code;
+}
+
+int sm_count(int device) {
+  static std::atomic<int> known[64];
+  const bool keep = device >= 0 && device < 64;
+  int n = keep ? known[device].load(std::memory_order_relaxed) : 0;
+  if (n > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    return 1;
+  }
+  if (keep) known[device].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+}  // namespace gptoss
+
 #define DCK(h, call)                                                                  \
   do {                                                                                \
     cudaError_t e__ = (call);                                                         \
@@ -463,16 +492,13 @@ static cudaError_t dalloc(T **p, size_t n) {
 // inv_freq and concentration exactly as the reference computes them on the host
 // (compute_concentration_and_inv_freq, run.cpp:423-474; ntk_beta 32, ntk_alpha 1,
 // run.cpp:583-584), in float.
-static void rope_tables(const gptoss_model_config_t &c, std::vector<float> *inv_freq,
-                        float *concentration) {
-  const int d_half = c.head_dim / 2;
-  const float base = c.rope_theta, sf = c.rope_scaling_factor;
-  const float ctx = static_cast<float>(c.initial_context_length);
+static void rope_table(int rotary_dim, float base, float sf, float ctx, float *inv_freq,
+                       float *concentration) {
+  const int d_half = rotary_dim / 2;
   const float ntk_beta = 32.0f, ntk_alpha = 1.0f;
-  inv_freq->resize(d_half);
   std::vector<float> freq(d_half);
   for (int i = 0; i < d_half; i++)
-    freq[i] = powf(base, static_cast<float>(2 * i) / static_cast<float>(c.head_dim));
+    freq[i] = powf(base, static_cast<float>(2 * i) / static_cast<float>(rotary_dim));
   if (sf > 1.0f) {
     *concentration = 0.1f * logf(sf) + 1.0f;
     const float low = d_half * logf(ctx / (ntk_beta * 2.0f * M_PI)) / logf(base);
@@ -483,11 +509,11 @@ static void rope_tables(const gptoss_model_config_t &c, std::vector<float> *inv_
       float ramp = (static_cast<float>(i) - low) / (high - low);
       ramp = ramp < 0 ? 0 : (ramp > 1 ? 1 : ramp);
       const float mask = 1.0f - ramp;
-      (*inv_freq)[i] = interpolation * (1.0f - mask) + extrapolation * mask;
+      inv_freq[i] = interpolation * (1.0f - mask) + extrapolation * mask;
     }
   } else {
     *concentration = 1.0f;
-    for (int i = 0; i < d_half; i++) (*inv_freq)[i] = 1.0f / freq[i];
+    for (int i = 0; i < d_half; i++) inv_freq[i] = 1.0f / freq[i];
   }
 }
 
@@ -498,6 +524,21 @@ const char *gptoss_decode_last_error(const gptoss_decode_t *h) {
 }
 
 gptoss_moe_t *gptoss_decode_moe(gptoss_decode_t *h) { return h ? h->moe : nullptr; }
+
+int gptoss_decode_rope_table(int rotary_dim, float theta, float scaling_factor,
+                             int initial_context_length, float *inv_freq_host,
+                             float *concentration) {
+  if (!inv_freq_host || !concentration || rotary_dim <= 0 || rotary_dim > 1024 || rotary_dim % 2)
+    return decode_error(GPTOSS_E_INVALID,
+                        "rope_table: rotary_dim must be even and in 2..1024, the outputs non-null");
+  if (!(theta > 1.0f) || !isfinite(theta) || !isfinite(scaling_factor) ||
+      (scaling_factor > 1.0f && initial_context_length <= 0))
+    return decode_error(GPTOSS_E_INVALID,
+                        "rope_table: theta must be above 1 and the context length positive");
+  rope_table(rotary_dim, theta, scaling_factor, static_cast<float>(initial_context_length),
+             inv_freq_host, concentration);
+  return GPTOSS_OK;
+}
 
 int gptoss_decode_device_count(void) {
   int n = 0, good = 0;
@@ -608,8 +649,9 @@ int gptoss_decode_create_ep(const gptoss_model_config_t *cfg, int max_batch, int
     e = cudaMemcpy(h->ones, one.data(), B * sizeof(float), cudaMemcpyHostToDevice);
     if (e != cudaSuccess) return bail(GPTOSS_E_CUDA, cudaGetErrorString(e));
   }
-  std::vector<float> inv;
-  rope_tables(c, &inv, &h->concentration);
+  std::vector<float> inv(c.head_dim / 2);
+  rope_table(c.head_dim, c.rope_theta, c.rope_scaling_factor,
+             static_cast<float>(c.initial_context_length), inv.data(), &h->concentration);
   e = cudaMemcpy(h->inv_freq, inv.data(), inv.size() * 4, cudaMemcpyHostToDevice);
   if (e != cudaSuccess) return bail(GPTOSS_E_CUDA, cudaGetErrorString(e));
   *out = h;

@@ -128,6 +128,61 @@ int gptoss_decode_get_logits(gptoss_decode_t *h, int row, float *logits_host);
 /* The MoE engine inside (for its options, taps and stage timers). */
 gptoss_moe_t *gptoss_decode_moe(gptoss_decode_t *h);
 
+/*
+ * The operators of a prompt pass and of a drawn token, without a handle: every pointer is a
+ * device pointer owned by the caller, all on one GPU (which need not be the current one;
+ * `stream` belongs to it, NULL = its default stream).  The calls allocate nothing, keep
+ * nothing between calls, do not synchronise and may be captured into CUDA graphs; calls on
+ * different streams or threads are independent.  They return 0 or a negative GPTOSS_E_*
+ * code with the text in gptoss_decode_last_error(NULL), and launch nothing when they fail.
+ * `status` fields are optional device words in which a kernel leaves a code of
+ * gptoss_moe_device_status (first writer wins; the caller clears it).
+ */
+enum { GPTOSS_DTYPE_BF16 = 0, GPTOSS_DTYPE_FP16 = 1, GPTOSS_DTYPE_FP32 = 2 };
+
+/*
+ * Rotary frequencies: inv_freq [rotary_dim / 2] (host) and the factor on cosine and sine,
+ * as the engine computes them from its config (run.cpp:423-474): theta^(-2i / rotary_dim),
+ * and for scaling_factor > 1 the YaRN interpolation over initial_context_length.
+ */
+int gptoss_decode_rope_table(int rotary_dim, float theta, float scaling_factor,
+                             int initial_context_length, float *inv_freq_host,
+                             float *concentration);
+
+/*
+ * Rotary positions on the rows of a batch and the append to the KV cache: what the decode
+ * step does to one projection output per sequence (run.cpp:575-596), for any number of
+ * rows.  Row i has its position pos[i]; rows with pos[i] < 0 are skipped.  With
+ * a = pos[i] * inv_freq[j] and (c, s) = concentration * (cos a, sin a), the pairs (x1, x2) of
+ * the first rotary_dim elements of every q and k head become (x1 c - x2 s, x2 c + x1 s); the
+ * pair j is elements (j, j + rotary_dim / 2), or (2j, 2j + 1) when `interleaved`; the rest of
+ * a head is copied, and so is v.  The arithmetic is fp32, rounded once to the type.
+ *   q  [n_rows, n_q_heads, head_dim] -> q_out (same shape; may be q itself)
+ *   k  [n_rows, n_kv_heads, head_dim] -> rows of k_cache [n_slots, n_kv_heads, head_dim]
+ *   v  likewise -> v_cache
+ * Heads are contiguous, rows are `*_stride` elements apart (a row of q | k | v as the
+ * projection leaves it: all three strides are its length).  slots[i] is the cache row of row
+ * i; NULL: row i (n_slots >= n_rows then).  A row whose slot is outside [0, n_slots) is not
+ * stored.  Two rows with one slot leave one of them there, element by element undefined.
+ * q (with q_out), k (with k_cache) and v (with v_cache) may each be NULL.  k_cache may be k
+ * itself when slots is NULL; other overlaps of inputs and outputs are not allowed.
+ * angle_f32 = 0: the angle is formed in fp64 (exact for every position); 1: pos * inv_freq
+ * is rounded to fp32 first, as the reference and gptoss_decode_step do.
+ */
+typedef struct {
+  const void *q, *k, *v;
+  void *q_out, *k_cache, *v_cache;
+  const int *pos;             /* [n_rows] */
+  const long long *slots;     /* [n_rows] or NULL */
+  const float *inv_freq;      /* [rotary_dim / 2], device */
+  long long q_stride, k_stride, v_stride, q_out_stride, k_cache_stride, v_cache_stride;
+  long long n_slots;
+  float concentration;
+  int n_rows, n_q_heads, n_kv_heads, head_dim, rotary_dim;
+  int interleaved, angle_f32, dtype;
+} gptoss_rope_args_t;
+int gptoss_decode_rope_append(const gptoss_rope_args_t *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
