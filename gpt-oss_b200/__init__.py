@@ -82,6 +82,17 @@ class RopeArgs(ctypes.Structure):
                                             "rotary_dim", "interleaved", "angle_f32", "dtype")]
 
 
+class AttentionArgs(ctypes.Structure):
+    """Mirror of gptoss_attention_args_t."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "q_start", "kv_start", "kv_len",
+                                               "sinks", "status")] + \
+               [(n, ctypes.c_longlong) for n in ("q_stride", "k_stride", "v_stride", "out_stride",
+                                                 "n_kv_rows")] + \
+               [("scale", ctypes.c_float)] + \
+               [(n, ctypes.c_int) for n in ("n_tokens", "n_seqs", "n_q_heads", "n_kv_heads",
+                                            "head_dim", "window", "max_kv_len", "dtype")]
+
+
 _lib = None
 
 
@@ -148,6 +159,7 @@ def load_library() -> ctypes.CDLL:
         "gptoss_decode_get_kv": (c_int, [vp, c_int, c_int, c_int, c_int, c_int, vp, vp]),
         "gptoss_decode_rope_table": (c_int, [c_int, ctypes.c_float, ctypes.c_float, c_int, vp, fp]),
         "gptoss_decode_rope_append": (c_int, [ctypes.POINTER(RopeArgs), vp]),
+        "gptoss_decode_prompt_attention": (c_int, [ctypes.POINTER(AttentionArgs), vp]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(lib, name)
@@ -286,6 +298,37 @@ def rope_append(q, k, v, pos, inv_freq, q_out=None, k_cache=None, v_cache=None, 
                     hkv, d, 2 * inv_freq.shape[0], interleaved, angle_f32,
                     _dtype_code(first, "input"))
     _check_op(lib, lib.gptoss_decode_rope_append(ctypes.byref(args), ctypes.c_void_p(stream)))
+
+
+def prompt_attention(q, k, v, q_start, kv_start, kv_len, out, sinks=None, scale=None, window=0,
+                     max_kv_len=0, status=None, stream=0):
+    """gptoss_decode_prompt_attention: causal attention of packed query rows over K / V rows.
+    q and out [tokens, heads, head_dim], k and v [kv rows, kv heads, head_dim] (any row stride
+    that is a multiple of 8, heads contiguous) in bf16 or fp16; q_start int32 [seqs + 1],
+    kv_start int64 [seqs], kv_len int32 [seqs]; sinks float32 [heads] or None; scale defaults
+    to 1 / sqrt(head_dim); window 0 = none; max_kv_len: the largest kv_len where the caller
+    knows it; status: int32 [1] tensor or None."""
+    lib = load_library()
+    dev, dtype = _on_gpu(q, "q"), q.dtype
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError("q and k must have three dimensions")
+    tokens, hq, d = q.shape
+    n_kv, hkv, _ = k.shape
+    qp, qs = _rows(q, "q", dtype, dev, hq, d)
+    kp, ks = _rows(k, "k", dtype, dev, hkv, d)
+    vp, vs = _rows(v, "v", dtype, dev, hkv, d)
+    op, os_ = _rows(out, "out", dtype, dev, hq, d)
+    if v.shape[0] != n_kv or out.shape[0] != tokens:
+        raise ValueError("k and v, or q and out, have different numbers of rows")
+    n = kv_len.shape[0]
+    args = AttentionArgs(qp, kp, vp, op, _vector(q_start, "q_start", "torch.int32", n + 1, dev),
+                         _vector(kv_start, "kv_start", "torch.int64", n, dev),
+                         _vector(kv_len, "kv_len", "torch.int32", n, dev),
+                         _vector(sinks, "sinks", "torch.float32", hq, dev),
+                         _vector(status, "status", "torch.int32", 1, dev), qs, ks, vs, os_, n_kv,
+                         d ** -0.5 if scale is None else scale, tokens, n, hq, hkv, d, window,
+                         max_kv_len, _dtype_code(q, "q"))
+    _check_op(lib, lib.gptoss_decode_prompt_attention(ctypes.byref(args), ctypes.c_void_p(stream)))
 
 
 class MoeEngine:

@@ -183,6 +183,45 @@ typedef struct {
 } gptoss_rope_args_t;
 int gptoss_decode_rope_append(const gptoss_rope_args_t *args, void *stream);
 
+/*
+ * Attention of packed query rows over K / V rows that are in place (a cache, or the packed
+ * keys and values of the same prompts): a whole prompt, a piece of one on top of its context,
+ * single tokens, or any mixture, in one launch.  It computes for every row what the decode
+ * step computes for one (run.cpp:601-647): causal, grouped heads (query head h reads KV head
+ * h / (n_q_heads / n_kv_heads)), an optional sink logit per query head that takes probability
+ * mass and has no value, an optional sliding window.
+ *   q, out  [n_tokens, n_q_heads, head_dim]; sequence i owns rows q_start[i] .. q_start[i+1]
+ *   k, v    [n_kv_rows, n_kv_heads, head_dim]; its keys are rows kv_start[i] .. + kv_len[i]
+ * The last query of a sequence stands at its last key: query j of L sees key t when
+ * t <= p and (window == 0 or t > p - window), p = kv_len[i] - L + j.  A query that sees no
+ * key (kv_len[i] < L leaves p < 0) gets zeros.  bf16 or fp16, softmax in fp32; the
+ * probabilities are rounded to the type before they multiply v, the result once at the end.
+ * K and V rows outside every sequence, or that no query of a sequence sees, may hold
+ * anything (NaN included); those that some query sees must be finite.
+ * Heads are contiguous, rows are `*_stride` elements apart; addresses and strides in bytes
+ * are multiples of 16.  head_dim 32, 64 or 128; n_q_heads a multiple of n_kv_heads, at most
+ * 128 times it.  q_start is ascending from 0 to n_tokens; a sequence whose entries
+ * break that, whose keys leave [0, n_kv_rows) or whose kv_len is negative is left unwritten
+ * and reported as status 104.  Rows that belong to no sequence are left unwritten too.
+ * max_kv_len: an upper bound on kv_len that the host knows (0 = not known); it only chooses
+ * how the work is split.
+ */
+typedef struct {
+  const void *q, *k, *v;
+  void *out;
+  const int *q_start;         /* [n_seqs + 1] */
+  const long long *kv_start;  /* [n_seqs] */
+  const int *kv_len;          /* [n_seqs] */
+  const float *sinks;         /* [n_q_heads] or NULL */
+  int *status;                /* or NULL */
+  long long q_stride, k_stride, v_stride, out_stride;
+  long long n_kv_rows;
+  float scale;                /* on q . k, 1 / sqrt(head_dim) as a rule */
+  int n_tokens, n_seqs, n_q_heads, n_kv_heads, head_dim;
+  int window, max_kv_len, dtype;
+} gptoss_attention_args_t;
+int gptoss_decode_prompt_attention(const gptoss_attention_args_t *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
