@@ -93,6 +93,14 @@ class AttentionArgs(ctypes.Structure):
                                             "head_dim", "window", "max_kv_len", "dtype")]
 
 
+class SampleArgs(ctypes.Structure):
+    """Mirror of gptoss_sample_args_t."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "u", "temperature", "top_k", "top_p",
+                                               "min_p", "pos", "next")] + \
+               [("stride", ctypes.c_longlong)] + \
+               [(n, ctypes.c_int) for n in ("n_rows", "vocab", "dtype")]
+
+
 _lib = None
 
 
@@ -160,6 +168,7 @@ def load_library() -> ctypes.CDLL:
         "gptoss_decode_rope_table": (c_int, [c_int, ctypes.c_float, ctypes.c_float, c_int, vp, fp]),
         "gptoss_decode_rope_append": (c_int, [ctypes.POINTER(RopeArgs), vp]),
         "gptoss_decode_prompt_attention": (c_int, [ctypes.POINTER(AttentionArgs), vp]),
+        "gptoss_decode_sample": (c_int, [ctypes.POINTER(SampleArgs), vp]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(lib, name)
@@ -329,6 +338,28 @@ def prompt_attention(q, k, v, q_start, kv_start, kv_len, out, sinks=None, scale=
                          d ** -0.5 if scale is None else scale, tokens, n, hq, hkv, d, window,
                          max_kv_len, _dtype_code(q, "q"))
     _check_op(lib, lib.gptoss_decode_prompt_attention(ctypes.byref(args), ctypes.c_void_p(stream)))
+
+
+def sample_tokens(logits, u, next_tokens, temperature=None, top_k=None, top_p=None, min_p=None,
+                  pos=None, stream=0):
+    """gptoss_decode_sample: next_tokens int32 [rows] drawn from logits [rows, vocab] (bf16, fp16
+    or fp32, any row stride) with the uniform numbers u float32 [rows].  temperature, top_p,
+    min_p float32 [rows], top_k int32 [rows], pos int32 [rows]; None switches one off
+    (temperature None = 1; a temperature <= 0 is the argmax)."""
+    lib = load_library()
+    dev = _on_gpu(logits, "logits")
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be [rows, vocab] with contiguous rows")
+    rows, vocab = logits.shape
+    f32, i32 = "torch.float32", "torch.int32"
+    args = SampleArgs(logits.data_ptr(), _vector(u, "u", f32, rows, dev),
+                      _vector(temperature, "temperature", f32, rows, dev),
+                      _vector(top_k, "top_k", i32, rows, dev), _vector(top_p, "top_p", f32, rows, dev),
+                      _vector(min_p, "min_p", f32, rows, dev), _vector(pos, "pos", i32, rows, dev),
+                      _vector(next_tokens, "next_tokens", i32, rows, dev),
+                      logits.stride(0) if rows > 1 else vocab, rows, vocab,
+                      _dtype_code(logits, "logits"))
+    _check_op(lib, lib.gptoss_decode_sample(ctypes.byref(args), ctypes.c_void_p(stream)))
 
 
 class MoeEngine:

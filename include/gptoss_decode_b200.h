@@ -222,6 +222,43 @@ typedef struct {
 } gptoss_attention_args_t;
 int gptoss_decode_prompt_attention(const gptoss_attention_args_t *args, void *stream);
 
+/*
+ * The next token of every row, drawn from its logits with given uniform numbers (the step's
+ * argmax is the greedy case; the reference samples on the host, run.cpp:780-910).  For a
+ * row with temperature T > 0, weights w_i = exp((logit_i - max) / T); tokens are ordered by
+ * logit, largest first, lowest id first among equals, and the kept set is the longest prefix
+ * of that order that satisfies, in turn,
+ *   top_k:  at most top_k[r] tokens (<= 0 or >= vocab: no limit);
+ *   top_p:  the weight in front of a token, among those that top_k kept, is below top_p[r]
+ *           times their total (>= 1: no limit; the first token always stays);
+ *   min_p:  w_i >= min_p[r] (w of the likeliest token is 1, which stays; <= 0: no limit).
+ * A NaN in one of the last two is no limit either.
+ * next[r] is the lowest kept id whose running sum of kept weights, in the order of the ids,
+ * exceeds u[r] times their total, u in [0, 1) (values outside are clamped, NaN counts as 0).
+ * T <= 0 or NaN: the largest logit, lowest id among equals.  NaN logits count as -infinity,
+ * which is never drawn; a row with nothing else gives 0, as the argmax of the step does.
+ * Where logits are +infinity those alone are kept, with equal weight, as far as top_k and
+ * top_p leave them.  Rows with pos[r] < 0 give -1.
+ * Weights are formed in fp64 and summed as multiples of 2^-44 in 64-bit integers, so sums do
+ * not depend on their order and a draw does not either; a weight below 2^-45 counts as 0.
+ * logits [n_rows, vocab], rows `stride` elements apart, in bf16, fp16 or fp32; vocab up to
+ * 2^18.  temperature, top_k, top_p, min_p, u: device arrays of n_rows (NULL: 1, no limit, no
+ * limit, no limit; u is required).
+ */
+typedef struct {
+  const void *logits;
+  const float *u;
+  const float *temperature;   /* or NULL */
+  const int *top_k;           /* or NULL */
+  const float *top_p;         /* or NULL */
+  const float *min_p;         /* or NULL */
+  const int *pos;             /* or NULL */
+  int *next;                  /* [n_rows] */
+  long long stride;
+  int n_rows, vocab, dtype;
+} gptoss_sample_args_t;
+int gptoss_decode_sample(const gptoss_sample_args_t *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
