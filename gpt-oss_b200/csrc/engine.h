@@ -196,6 +196,11 @@ cudaError_t launch_gate_up(gptoss_moe *h, int layer, cudaStream_t stream, int pa
 cudaError_t launch_down(gptoss_moe *h, int layer, cudaStream_t stream);
 int make_tmap_2d_bf16(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer,
                       uint32_t box_inner, uint32_t box_outer, std::string *err);
+// a [rows, heads, head_dim] tensor of a 16-bit type whose rows are row_stride elements apart,
+// boxes of [box_rows, box_heads, box_dim]; box_dim 64 (128-byte swizzle) or 32 (64-byte swizzle)
+int make_tmap_rows(CUtensorMap *map, const void *base, bool fp16, uint64_t head_dim, uint64_t heads,
+                   uint64_t rows, uint64_t row_stride, uint32_t box_dim, uint32_t box_heads,
+                   uint32_t box_rows, std::string *err);
 int gemm_tile_n(int which);  // N extent of one tile: 0 = gate_up, 1 = down
 // grouped_gemm_pair.cu
 cudaError_t launch_gate_up_pair(gptoss_moe *h, int layer, cudaStream_t stream, int part = 0);

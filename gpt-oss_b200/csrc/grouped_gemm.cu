@@ -365,6 +365,27 @@ int make_tmap_2d_bf16(CUtensorMap *map, const void *base, uint64_t inner, uint64
   return GPTOSS_OK;
 }
 
+int make_tmap_rows(CUtensorMap *map, const void *base, bool fp16, uint64_t head_dim, uint64_t heads,
+                   uint64_t rows, uint64_t row_stride, uint32_t box_dim, uint32_t box_heads,
+                   uint32_t box_rows, std::string *err) {
+  EncodeTiledFn fn = get_encode_fn(err);
+  if (!fn) return GPTOSS_E_CUDA;
+  cuuint64_t dims[3] = {head_dim, heads, rows};
+  cuuint64_t strides[2] = {head_dim * 2, row_stride * 2};
+  cuuint32_t box[3] = {box_dim, box_heads, box_rows};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                  const_cast<void *>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  box_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    if (err) *err = "cuTensorMapEncodeTiled (rows) failed with CUresult " + std::to_string((int)r);
+    return GPTOSS_E_CUDA;
+  }
+  return GPTOSS_OK;
+}
+
 int make_tmap_tiles_bf16(CUtensorMap *map, const void *base, uint64_t n_tiles, std::string *err) {
   EncodeTiledFn fn = get_encode_fn(err);
   if (!fn) return GPTOSS_E_CUDA;

@@ -339,7 +339,7 @@ def test_too_many_rows_and_nothing_to_do(pkg):
 
     lib = pkg.load_library()
     assert lib.gptoss_decode_prompt_attention(None, None) == pkg.GPTOSS_E_INVALID
-    a = _c_args(pkg, n_kv_rows=1 << 31)
+    a = _c_args(pkg, n_kv_rows=(1 << 31) - 256)
     assert lib.gptoss_decode_prompt_attention(ctypes.byref(a), None) == pkg.GPTOSS_E_CAPACITY
     for change in (dict(n_tokens=0, q=None, out=None), dict(n_seqs=0, q_start=None)):
         a = _c_args(pkg, **change)
