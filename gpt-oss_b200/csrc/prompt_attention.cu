@@ -5,11 +5,12 @@
 //
 // A tile is 128 rows of one MMA: kTok = 128 / group query tokens times the `group` query heads
 // that share a KV head, so K and V are read once for the whole group and a sequence of a few
-// tokens still fills rows.  A CTA owns two tiles (A and B, consecutive tokens) of one sequence
-// and KV head and runs them over the same stream of blocks of 128 keys:
+// tokens still fills rows.  A job is two tiles (A and B, consecutive tokens) of one sequence and
+// KV head over the same stream of blocks of 128 keys.  CTAs are persistent, one per SM:
 //   warps 0-3, 4-7  softmax of tile A, of tile B: a thread owns a row (a TMEM lane)
-//   warp 8          TMA: Q of both tiles once, then K and V blocks into two rings
-//   warp 9          TMEM allocation and the MMAs, S = Q K^T and O += P V
+//   warp 8          TMA: Q of both tiles, then K and V blocks into two rings
+//   warps 9, 10     the MMAs of tile A and of tile B, S = Q K^T and O += P V
+//   warp 11         the jobs, a few ahead of the others
 // S comes from TMEM into registers whole (128 per thread), so the row maximum costs no second
 // read; P goes back to TMEM as the MMA's 16-bit row operand, V is read in place as an N-major
 // operand.  The maximum that scales a row is only moved when it grows by more than 8 (a factor
@@ -42,51 +43,109 @@
 
 namespace gptoss {
 
-constexpr int kAttnThreads = 320;
-constexpr int kKeys = 128;            // keys per block
+constexpr int kAttnThreads = 384;
+constexpr int kKeys = 64;             // keys per unit
 constexpr int kAttnTmemCols = 512;
 constexpr int kAttnMaxSplit = 8;      // CTAs of a cluster that share a pair of tiles
+constexpr int kJobs = 4;              // jobs that may be at work in different warps
 
 template <int D>
 struct AttnShape {
   static constexpr int kBox = D < 64 ? D : 64;            // elements of one swizzled row
   static constexpr int kPanels = D / kBox;                // 64-wide panels of a head
-  static constexpr int kPanelBytes = 128 * kBox * 2;      // 128 rows of a panel
-  static constexpr int kTileBytes = kPanels * kPanelBytes;
-  static constexpr int kStages = D == 128 ? 2 : 4;        // K blocks and V blocks in flight
-  static constexpr int kRingBytes = kStages * kTileBytes;
-  // P beside S in TMEM (S 2 x 128 columns, P 2 x 64, O 2 x D), or in S's place
+  static constexpr int kQPanelBytes = 128 * kBox * 2;
+  static constexpr int kPanelBytes = kKeys * kBox * 2;    // a panel of K or V
+  static constexpr int kQBytes = kPanels * kQPanelBytes;
+  static constexpr int kUnitBytes = kPanels * kPanelBytes;
+  static constexpr int kStages = D == 128 ? 4 : 8;        // units of K and of V in flight
+  static constexpr int kRingBytes = kStages * kUnitBytes;
+  // TMEM: S of tile x, buffer j at column 128 x + 64 j.  P beside S (2 x 2 x 32 columns, then
+  // O 2 x D), or in the place of the S that it was made from.
   static constexpr bool kApart = D <= 64;
   static constexpr int kColP = kApart ? 256 : 0;
-  static constexpr int kStrideP = kApart ? 64 : 128;
+  static constexpr int kStrideP = kApart ? 64 : 128, kBufferP = kApart ? 32 : 64;
   static constexpr int kColO = kApart ? 384 : 256;
   static constexpr int kStrideO = kApart ? 64 : 128;
-  static constexpr int kOperandBytes = 2 * kTileBytes + 2 * kRingBytes;
+  static constexpr int kOperandBytes = 2 * kQBytes + 2 * kRingBytes;
   // fp32 partial outputs of both tiles take the operands' place in a split launch
   static constexpr int kSmemBytes = 1024 + (kOperandBytes > 256 * D * 4 ? kOperandBytes : 256 * D * 4);
 };
 
 struct AttnBarriers {
-  uint64_t q_full[2], s_full[2], s_free[2], p_full[2], o_full[2], v_tail;
-  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
+  uint64_t job_full[kJobs], job_empty[kJobs], steal;
+  uint64_t q_full[2], q_empty[2], v_tail;
+  uint64_t s_full[2][2], s_free[2][2], p_full[2][2], o_full[2][2];  // [tile][buffer]
+  uint64_t k_full[8], k_empty[8], v_full[8], v_empty[8];
 };
 
-// Which rows a CTA works on, found once by one warp.
+// The rows and keys of one job.
 struct AttnJob {
-  int seq;                // -1: nothing to do
+  int kvh;                // KV head; -1: there are no more jobs
   int q_row0;             // first query row of the pair of tiles
   int tokens[2];          // valid tokens of the tiles
-  int kv_row0;            // first key of block 0 (row of k)
-  int first_pos;          // position of the first query token, relative to block 0's first key
-  int keys;               // keys from block 0's first to the last that the pair sees
-  int begin[2], end[2];   // blocks of each tile, within this CTA's share
-  int blk0, blk1;         // blocks of this CTA
+  int kv_row0;            // first key of unit 0 (row of k)
+  int first_pos;          // position of the first query token, relative to unit 0's first key
+  int keys;               // keys from unit 0's first to the last that the pair sees
+  int begin[2], end[2];   // units of each tile, within this CTA's share
+  int unit0, unit1;       // units of this CTA
 };
 
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// two fp32 lanes in one instruction
+__device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ float2 f32x2_parts(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t f32x2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t f32x2_add(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// 2^x of two values in [-125, 127] on the FMA pipes: x = n + f with n the nearest integer (the
+// addition of 1.5 * 2^23 rounds to it and leaves it in the low bits), 2^f by the polynomial of
+// least relative error on [-1/2, 1/2] (Remez exchange; degree 3: 7.5e-5, degree 4: 2.6e-6),
+// n added to the exponent.  Smaller x give 2^-125.
+template <int kDegree>
+__device__ __forceinline__ float2 poly_exp2(float2 x) {
+  const uint64_t v = f32x2(fmaxf(x.x, -125.f), fmaxf(x.y, -125.f));
+  const uint64_t magic = f32x2(12582912.f, 12582912.f), minus = f32x2(-1.f, -1.f);
+  const uint64_t t = f32x2_add(v, magic);
+  const uint64_t n = f32x2_add(t, f32x2(-12582912.f, -12582912.f));
+  const uint64_t f = f32x2_fma(n, minus, v);
+  uint64_t p;
+  if (kDegree == 3) {
+    p = f32x2_fma(f, f32x2(0.0551716685f, 0.0551716685f), f32x2(0.2426111251f, 0.2426111251f));
+    p = f32x2_fma(p, f, f32x2(0.6932609677f, 0.6932609677f));
+    p = f32x2_fma(p, f, f32x2(0.9999280572f, 0.9999280572f));
+  } else {
+    p = f32x2_fma(f, f32x2(0.0095701022f, 0.0095701022f), f32x2(0.0559178591f, 0.0559178591f));
+    p = f32x2_fma(p, f, f32x2(0.2402474433f, 0.2402474433f));
+    p = f32x2_fma(p, f, f32x2(0.6931217909f, 0.6931217909f));
+    p = f32x2_fma(p, f, f32x2(0.9999992847f, 0.9999992847f));
+  }
+  const float2 r = f32x2_parts(p), m = f32x2_parts(t);
+  return make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(m.x) << 23)),
+                     __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(m.y) << 23)));
 }
 __device__ __forceinline__ uint32_t pack16(float lo, float hi, bf16 *) { return pack_bf16(lo, hi); }
 __device__ __forceinline__ uint32_t pack16(float lo, float hi, __half *) {
@@ -176,8 +235,9 @@ __device__ __forceinline__ float row_factor(float m, float l, const float *sinks
 // Slots: a pair of tiles covers 2 * tok tokens; sequence i's pairs start at slot
 // q_start[i] / (2 tok) + i, which leaves room for a partial pair per sequence and needs no
 // prefix sum.  One warp finds the slot's sequence by counting the starts at or before it.
-__device__ void attn_find_job(const gptoss_attention_args_t &a, int tok, int slot, int rank, int split,
-                              int lane, AttnJob *job) {
+// Returns (warp-uniform) whether there is anything to do for the slot.
+__device__ bool attn_find_job(const gptoss_attention_args_t &a, int tok, int slot, int kvh, int rank,
+                              int split, int lane, AttnJob *job) {
   const int pair = 2 * tok;
   int below = 0;
   bool broken = false;
@@ -185,55 +245,97 @@ __device__ void attn_find_job(const gptoss_attention_args_t &a, int tok, int slo
     const int i = i0 + lane;
     bool hit = false;
     if (i < a.n_seqs) {
-      const int q0 = a.q_start[i];
-      broken |= q0 < 0 || a.q_start[i + 1] < q0 || a.q_start[i + 1] > a.n_tokens;
+      const int q0 = __ldg(a.q_start + i), q1 = __ldg(a.q_start + i + 1);
+      broken |= q0 < 0 || q1 < q0 || q1 > a.n_tokens;
       hit = q0 / pair + i <= slot;
     }
     below += __popc(__ballot_sync(0xffffffffu, hit));
   }
   if (broken) set_status(a.status, kStatusBadIndex);
-  if (lane != 0) return;
-  job->seq = -1;
-  job->blk0 = job->blk1 = 0;
-  for (int x = 0; x < 2; x++) job->tokens[x] = job->begin[x] = job->end[x] = 0;
   const int seq = below - 1;
-  if (seq < 0) return;
-  const int q0 = a.q_start[seq], q1 = a.q_start[seq + 1];
-  if (q0 < 0 || q1 < q0 || q1 > a.n_tokens) return;
+  if (seq < 0) return false;
+  const int q0 = __ldg(a.q_start + seq), q1 = __ldg(a.q_start + seq + 1);
+  if (q0 < 0 || q1 < q0 || q1 > a.n_tokens) return false;
   const long long t0 = static_cast<long long>(slot - (q0 / pair + seq)) * pair;
   const int len_q = q1 - q0;
-  if (t0 < 0 || t0 >= len_q) return;
-  const long long start = a.kv_start[seq];
-  const int len = a.kv_len[seq];
+  if (t0 < 0 || t0 >= len_q) return false;
+  const long long start = __ldg(a.kv_start + seq);
+  const int len = __ldg(a.kv_len + seq);
   if (len < 0 || start < 0 || start > a.n_kv_rows - len) {
     set_status(a.status, kStatusBadIndex);
-    return;
+    return false;
   }
+  if (lane != 0) return true;
   const int n_tok = static_cast<int>(min(static_cast<long long>(pair), len_q - t0));
   const long long pos = static_cast<long long>(len) - len_q + t0;  // of the pair's first token
   const long long lo = a.window > 0 ? max(0ll, pos - a.window + 1) : 0;
   const long long hi = max(lo, pos + n_tok);  // one past the last key that the pair sees
-  const int blocks = static_cast<int>((hi - lo + kKeys - 1) / kKeys);
-  job->seq = seq;
+  const int units = static_cast<int>((hi - lo + kKeys - 1) / kKeys);
+  job->kvh = kvh;
   job->q_row0 = q0 + static_cast<int>(t0);
   job->kv_row0 = static_cast<int>(start + lo);
   job->first_pos = static_cast<int>(pos - lo);
   job->keys = static_cast<int>(hi - lo);
-  job->blk0 = static_cast<int>(static_cast<long long>(blocks) * rank / split);
-  job->blk1 = static_cast<int>(static_cast<long long>(blocks) * (rank + 1) / split);
+  job->unit0 = static_cast<int>(static_cast<long long>(units) * rank / split);
+  job->unit1 = static_cast<int>(static_cast<long long>(units) * (rank + 1) / split);
   for (int x = 0; x < 2; x++) {
     const int n = min(max(n_tok - x * tok, 0), tok);
     job->tokens[x] = n;
+    job->begin[x] = job->end[x] = job->unit0;
     if (n == 0) continue;
     const long long p = pos + x * tok;  // the tile's first token
     const long long from = a.window > 0 ? max(0ll, p - a.window + 1) - lo : 0;
     const long long to = p + n - lo;    // may be <= 0
     const int b = static_cast<int>(from / kKeys);
     const int e = to > 0 ? static_cast<int>((to + kKeys - 1) / kKeys) : 0;
-    job->begin[x] = max(b, job->blk0);
-    job->end[x] = max(job->begin[x], min(e, job->blk1));
+    job->begin[x] = max(b, job->unit0);
+    job->end[x] = max(job->begin[x], min(e, job->unit1));
   }
+  return true;
 }
+
+// Asks for a CTA of this grid that has not started; the 16-byte answer says which one was
+// taken out of the launch, or that there is none left (nothing may be asked after that).
+__device__ __forceinline__ void steal_pair(void *answer, uint64_t *bar) {
+  mbar_arrive_expect_tx(bar, 16);
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+      :
+      : "r"(smem_u32(answer)), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ bool stolen_pair(const void *answer, uint32_t *pair) {
+  uint32_t got, x;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      ".reg .b128 r;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t"
+      "}"
+      : "=r"(got), "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  if (got) *pair = x;
+  return got != 0;
+}
+
+// Position in a ring of N slots.
+template <int N>
+struct Ring {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == N) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+};
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kAttnThreads, 1)
@@ -245,38 +347,49 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
   constexpr bool kHalf = !std::is_same<T, bf16>::value;
   extern __shared__ unsigned char smem_raw[];
   __shared__ AttnBarriers bar;
-  __shared__ AttnJob job;
+  __shared__ AttnJob jobs[kJobs];
+  __shared__ __align__(16) unsigned char steal_answer[16];
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_word;
   __shared__ float part_m[256], part_l[256];
   unsigned char *smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
-  unsigned char *sm_q = smem, *sm_k = smem + 2 * S::kTileBytes, *sm_v = sm_k + S::kRingBytes;
+  unsigned char *sm_q = smem, *sm_k = smem + 2 * S::kQBytes, *sm_v = sm_k + S::kRingBytes;
   volatile int *abort_flag = &abort_word;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (through a shuffle, so that the compiler knows what the warp shares)
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = split > 1 ? static_cast<int>(cluster_cta_rank()) : 0;
-  // the last slots first: a long prompt's last tiles see the most keys
-  const int unit = blockIdx.x / split;
-  const int slot = n_slots - 1 - unit / a.n_kv_heads, kvh = unit % a.n_kv_heads;
 
   if (warp == 9) {
     tmem_alloc(&tmem_holder, kAttnTmemCols);
     tmem_relinquish();
   } else if (warp == 8) {
-    attn_find_job(a, tok, slot, rank, split, lane, &job);
+    if (elect_one()) {
+      tma_prefetch_desc(&map_q);
+      tma_prefetch_desc(&map_k);
+      tma_prefetch_desc(&map_v);
+    }
   } else if (threadIdx.x == 0) {
+    for (int j = 0; j < kJobs; j++) {
+      mbar_init(&bar.job_full[j], 1);
+      mbar_init(&bar.job_empty[j], 10);  // 8 softmax warps, 2 issuing warps
+    }
+    mbar_init(&bar.steal, 1);
+    mbar_init(&bar.v_tail, 1);
     for (int x = 0; x < 2; x++) {
       mbar_init(&bar.q_full[x], 1);
-      mbar_init(&bar.s_full[x], 1);
-      mbar_init(&bar.s_free[x], 4);
-      mbar_init(&bar.p_full[x], 4);
-      mbar_init(&bar.o_full[x], 1);
+      mbar_init(&bar.q_empty[x], 1);
+      for (int j = 0; j < 2; j++) {
+        mbar_init(&bar.s_full[x][j], 1);
+        mbar_init(&bar.s_free[x][j], 4);
+        mbar_init(&bar.p_full[x][j], 4);
+        mbar_init(&bar.o_full[x][j], 1);
+      }
     }
-    mbar_init(&bar.v_tail, 1);
     for (int s = 0; s < S::kStages; s++) {
       mbar_init(&bar.k_full[s], 1);
-      mbar_init(&bar.k_empty[s], 1);
+      mbar_init(&bar.k_empty[s], 2);
       mbar_init(&bar.v_full[s], 1);
-      mbar_init(&bar.v_empty[s], 1);
+      mbar_init(&bar.v_empty[s], 2);
     }
     abort_word = 0;
     mbar_fence_init();
@@ -284,258 +397,439 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_holder;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_holder, 0);
 
   float m = -INFINITY, l = 0.f;  // a softmax thread's row
-  if (job.seq >= 0 && warp == 8) {
-    // ---------------------------------------------------------------- loads
-    const int n = job.blk1 - job.blk0;
-    if (n > 0 && elect_one()) {
-      for (int x = 0; x < 2; x++) {
-        if (job.begin[x] >= job.end[x]) continue;
-        mbar_arrive_expect_tx(&bar.q_full[x], static_cast<uint32_t>(S::kPanels) * tok * group * S::kBox * 2);
-        for (int p = 0; p < S::kPanels; p++)
-          tma_load_3d(sm_q + x * S::kTileBytes + p * S::kPanelBytes, &map_q, &bar.q_full[x],
-                      p * S::kBox, kvh * group, job.q_row0 + x * tok);
-      }
-    }
-    bool ok = true;
-    for (int i = 0; i < n && ok; i++) {
-      const int st = i % S::kStages;
-      const uint32_t free_parity = (static_cast<uint32_t>(i / S::kStages) & 1u) ^ 1u;
-      const int rel = (job.blk0 + i) * kKeys;
-      const bool tail = rel + kKeys > job.keys;
-      ok = warp_wait(&bar.k_empty[st], free_parity, abort_flag);
-      if (ok && elect_one()) {
-        mbar_arrive_expect_tx(&bar.k_full[st], S::kTileBytes);
-        for (int p = 0; p < S::kPanels; p++)
-          tma_load_3d(sm_k + st * S::kTileBytes + p * S::kPanelBytes, &map_k, &bar.k_full[st],
-                      p * S::kBox, kvh, job.kv_row0 + rel);
-      }
-      ok = ok && warp_wait(&bar.v_empty[st], free_parity, abort_flag);
-      // The last block may reach past the last key: what lies there may be anything, and 0
-      // times NaN is NaN, so those rows of V are cleared before the block is handed on.
-      uint64_t *landed = tail ? &bar.v_tail : &bar.v_full[st];
-      unsigned char *v = sm_v + st * S::kTileBytes;
-      if (ok && elect_one()) {
-        mbar_arrive_expect_tx(landed, S::kTileBytes);
-        for (int p = 0; p < S::kPanels; p++)
-          tma_load_3d(v + p * S::kPanelBytes, &map_v, landed, p * S::kBox, kvh, job.kv_row0 + rel);
-      }
-      if (ok && tail) {
-        ok = warp_wait(landed, 0, abort_flag);
-        constexpr int kRowChunks = S::kBox * 2 / 16;
-        for (int p = 0; ok && p < S::kPanels; p++)
-          for (int c = (job.keys - rel) * kRowChunks + lane; c < kKeys * kRowChunks; c += 32)
-            *reinterpret_cast<uint4 *>(v + p * S::kPanelBytes + c * 16) = make_uint4(0, 0, 0, 0);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  int part_rows = 0;             // split launch: rows of this thread's tile, whether it had keys
+  bool part_any = false;
+  bool ok = true;
+  int code = kStatusOk;
+  Ring<kJobs> jr;
+  // whether there is a job in jobs[jr.slot] (false too when a wait ran out: ok is false then)
+  auto have_job = [&]() {
+    ok = ok && warp_wait(&bar.job_full[jr.slot], jr.phase, abort_flag);
+    return ok && jobs[jr.slot].kvh >= 0;
+  };
+  auto done_job = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bar.job_empty[jr.slot]);
+    jr.next();
+  };
+
+  // Registers: 384 threads were launched with 168 each (64512); the four warps that hold no
+  // tiles keep 72 and the eight that do take 216 (128 * 72 + 256 * 216 = 64512).
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 8) {
+      // -------------------------------------------------------------- jobs and loads
+      // The grid has a CTA (with a split: a cluster) per pair of tiles; this CTA does its own
+      // and then, one at a time, those of CTAs that have not started, in their order.  It asks
+      // for the next one only when the last loads of this one are due, so that a long job does
+      // not keep another waiting.
+      code = kStatusWaitTimeoutProducer;
+      uint32_t pair = blockIdx.x / split, steal_phase = 0, q_phase[2] = {1u, 1u}, tail_phase = 0;
+      Ring<S::kStages> ring;
+      bool have = true, asked = false;
+      auto ask = [&]() {
+        if (asked || split > 1) return;
+        asked = true;
+        if (elect_one()) steal_pair(steal_answer, &bar.steal);
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.v_full[st]);
+      };
+      auto answer = [&]() {
+        have = false;
+        if (!asked) return;
+        asked = false;
+        ok = ok && warp_wait(&bar.steal, steal_phase, abort_flag);
+        steal_phase ^= 1u;
+        have = ok && stolen_pair(steal_answer, &pair);
+        __syncwarp();
+      };
+      while (ok) {
+        ok = warp_wait(&bar.job_empty[jr.slot], jr.phase ^ 1u, abort_flag);
+        AttnJob &job = jobs[jr.slot];
+        bool found = false;
+        while (ok && have && !found) {
+          // the last slots first: a long prompt's last tiles see the most keys
+          const uint32_t up = pair / a.n_kv_heads;
+          found = attn_find_job(a, tok, n_slots - 1 - static_cast<int>(up),
+                                static_cast<int>(pair - up * a.n_kv_heads), rank, split, lane, &job);
+          if (!found) {
+            ask();
+            answer();
+          }
+        }
+        if (!ok) break;
+        if (!found && lane == 0) job.kvh = -1;  // the end
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.job_full[jr.slot]);
+        if (!found) break;
+        jr.next();
+        auto load_q = [&](int x) {
+          if (job.begin[x] >= job.end[x]) return;
+          ok = ok && warp_wait(&bar.q_empty[x], q_phase[x], abort_flag);
+          q_phase[x] ^= 1u;
+          if (ok && elect_one()) {
+            mbar_arrive_expect_tx(&bar.q_full[x], static_cast<uint32_t>(S::kPanels) * tok * group * S::kBox * 2);
+            for (int p = 0; p < S::kPanels; p++)
+              tma_load_3d(sm_q + x * S::kQBytes + p * S::kQPanelBytes, &map_q, &bar.q_full[x],
+                          p * S::kBox, job.kvh * group, job.q_row0 + x * tok);
+          }
+          __syncwarp();
+        };
+        load_q(0);
+        const int unit0 = job.unit0, unit1 = job.unit1;
+        for (int u = unit0; ok && u < unit1; u++) {
+          const int rel = u * kKeys;
+          const bool tail = rel + kKeys > job.keys;
+          unsigned char *k = sm_k + ring.slot * S::kUnitBytes, *v = sm_v + ring.slot * S::kUnitBytes;
+          ok = warp_wait(&bar.k_empty[ring.slot], ring.phase ^ 1u, abort_flag);
+          if (ok && elect_one()) {
+            mbar_arrive_expect_tx(&bar.k_full[ring.slot], S::kUnitBytes);
+            for (int p = 0; p < S::kPanels; p++)
+              tma_load_3d(k + p * S::kPanelBytes, &map_k, &bar.k_full[ring.slot], p * S::kBox,
+                          job.kvh, job.kv_row0 + rel);
+          }
+          __syncwarp();
+          if (u == unit0) load_q(1);
+          if (u + S::kStages >= unit1) ask();
+          ok = ok && warp_wait(&bar.v_empty[ring.slot], ring.phase ^ 1u, abort_flag);
+          // The last unit may reach past the last key: what lies there may be anything, and 0
+          // times NaN is NaN, so those rows of V are cleared before the unit is handed on.
+          uint64_t *landed = tail ? &bar.v_tail : &bar.v_full[ring.slot];
+          if (ok && elect_one()) {
+            mbar_arrive_expect_tx(landed, S::kUnitBytes);
+            for (int p = 0; p < S::kPanels; p++)
+              tma_load_3d(v + p * S::kPanelBytes, &map_v, landed, p * S::kBox, job.kvh, job.kv_row0 + rel);
+          }
+          __syncwarp();
+          if (ok && tail) {
+            ok = warp_wait(landed, tail_phase, abort_flag);
+            tail_phase ^= 1u;
+            constexpr int kRowChunks = S::kBox * 2 / 16;
+            for (int p = 0; ok && p < S::kPanels; p++)
+              for (int c = (job.keys - rel) * kRowChunks + lane; c < kKeys * kRowChunks; c += 32)
+                *reinterpret_cast<uint4 *>(v + p * S::kPanelBytes + c * 16) = make_uint4(0, 0, 0, 0);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.v_full[ring.slot]);
+          }
+          ring.next();
+        }
+        ask();
+        answer();
       }
-      if (!ok) {
-        set_status(a.status, kStatusWaitTimeoutProducer);
-        *abort_flag = 1;
-      }
-    }
-  } else if (job.seq >= 0 && warp == 9) {
-    // ---------------------------------------------------------------- MMAs
-    constexpr uint32_t idesc_s = attn_idesc(kHalf, kKeys, false);
-    constexpr uint32_t idesc_o = attn_idesc(kHalf, D, true);
-    const uint64_t desc_q = attn_desc<D>(smem_u32(sm_q));
-    const uint64_t desc_k = attn_desc<D>(smem_u32(sm_k));
-    const uint64_t desc_v = attn_desc<D>(smem_u32(sm_v));
-    const int b0 = job.blk0, n = job.blk1 - job.blk0;
-    int s_done[2] = {0, 0}, o_done[2] = {0, 0};  // products issued per tile
-    bool ok = true;
-    auto active = [&](int x, int i) { return b0 + i >= job.begin[x] && b0 + i < job.end[x]; };
-    auto scores = [&](int x, int i) {  // S_x = Q_x K_i^T
-      const int st = i % S::kStages;
-      if (s_done[x] == 0) ok = ok && warp_wait(&bar.q_full[x], 0, abort_flag);
-      // S is free again once its readers have it in registers; where P takes its place, the
-      // product that read that P was issued before (products run in the order of issue)
-      if (S::kApart && s_done[x] > 0)
-        ok = ok && warp_wait(&bar.s_free[x], (s_done[x] - 1) & 1, abort_flag);
-      if (!ok) return;
-      tc_fence_after();
-      if (elect_one()) {
+    } else if (warp < 11) {
+      // -------------------------------------------------------------- MMAs
+      code = kStatusWaitTimeoutMma;
+      constexpr uint32_t idesc_s = attn_idesc(kHalf, kKeys, false);
+      constexpr uint32_t idesc_o = attn_idesc(kHalf, D, true);
+      const int x = warp - 9;
+      const uint64_t desc_q = attn_desc<D>(smem_u32(sm_q + x * S::kQBytes));
+      const uint64_t desc_k = attn_desc<D>(smem_u32(sm_k));
+      const uint64_t desc_v = attn_desc<D>(smem_u32(sm_v));
+      const uint32_t tm_s = tmem + x * 128, tm_p = tmem + S::kColP + x * S::kStrideP;
+      const uint32_t tm_o = tmem + S::kColO + x * S::kStrideO;
+      Ring<S::kStages> kr, vr;
+      Ring<2> sr, pr;  // buffers of S being written, of P being read
+      uint32_t q_phase = 0;
+      for (; have_job(); done_job()) {
+        const AttnJob &job = jobs[jr.slot];
+        const int begin = job.begin[x], end = job.end[x], unit0 = job.unit0, unit1 = job.unit1;
+        auto scores = [&](int u) {  // S = Q K_u^T
+          ok = ok && warp_wait(&bar.k_full[kr.slot], kr.phase, abort_flag);
+          const bool active = u >= begin && u < end;
+          if (active) {
+            if (u == begin) {
+              ok = ok && warp_wait(&bar.q_full[x], q_phase, abort_flag);
+              q_phase ^= 1u;
+            }
+            // S is free again once its readers have it in registers; where P takes its place,
+            // the product that read that P was issued before (one warp's products run in order)
+            if (S::kApart) ok = ok && warp_wait(&bar.s_free[x][sr.slot], sr.phase ^ 1u, abort_flag);
+            tc_fence_after();
+            if (ok && elect_one()) {
+              const uint64_t dk = desc_k + (kr.slot * S::kUnitBytes >> 4);
 #pragma unroll
-        for (int k = 0; k < D / 16; k++) {
-          constexpr int kPerPanel = S::kBox / 16;
-          const uint32_t off = ((k / kPerPanel) * S::kPanelBytes + (k % kPerPanel) * 32) >> 4;
-          umma_bf16(tmem + x * 128, desc_q + (x * S::kTileBytes >> 4) + off,
-                    desc_k + (st * S::kTileBytes >> 4) + off, idesc_s, k != 0);
-        }
-        umma_commit(&bar.s_full[x]);
-      }
-      s_done[x]++;
-    };
-    auto values = [&](int x, int i) {  // O_x += P_x V_i
-      const int st = i % S::kStages;
-      ok = ok && warp_wait(&bar.p_full[x], o_done[x] & 1, abort_flag);
-      if (!ok) return;
-      tc_fence_after();
-      if (elect_one()) {
+              for (int k = 0; k < D / 16; k++) {
+                constexpr int kPerPanel = S::kBox / 16;
+                umma_bf16(tm_s + sr.slot * 64,
+                          desc_q + (((k / kPerPanel) * S::kQPanelBytes + (k % kPerPanel) * 32) >> 4),
+                          dk + (((k / kPerPanel) * S::kPanelBytes + (k % kPerPanel) * 32) >> 4),
+                          idesc_s, k != 0);
+              }
+              umma_commit(&bar.s_full[x][sr.slot]);
+              umma_commit(&bar.k_empty[kr.slot]);
+              if (u == end - 1) umma_commit(&bar.q_empty[x]);
+            }
+            sr.next();
+          } else if (ok && lane == 0) {
+            mbar_arrive(&bar.k_empty[kr.slot]);
+          }
+          __syncwarp();
+          kr.next();
+        };
+        auto values = [&](int u) {  // O += P V_u
+          ok = ok && warp_wait(&bar.v_full[vr.slot], vr.phase, abort_flag);
+          if (u >= begin && u < end) {
+            ok = ok && warp_wait(&bar.p_full[x][pr.slot], pr.phase, abort_flag);
+            tc_fence_after();
+            if (ok && elect_one()) {
+              const uint64_t dv = desc_v + (vr.slot * S::kUnitBytes >> 4);
 #pragma unroll
-        for (int k = 0; k < kKeys / 16; k++)
-          umma_ta(tmem + S::kColO + x * S::kStrideO, tmem + S::kColP + x * S::kStrideP + k * 8,
-                  desc_v + ((st * S::kTileBytes + k * 16 * S::kBox * 2) >> 4), idesc_o,
-                  o_done[x] > 0 || k != 0);
-        umma_commit(&bar.o_full[x]);
-      }
-      o_done[x]++;
-    };
-    auto wait_ring = [&](uint64_t *full, int i) {
-      ok = ok && warp_wait(&full[i % S::kStages], (i / S::kStages) & 1, abort_flag);
-    };
-    // (nobody waits for the last ones)
-    auto release = [&](uint64_t *empty, int i) {
-      if (ok && i + S::kStages < n && elect_one()) umma_commit(&empty[i % S::kStages]);
-    };
-    if (n > 0) {
-      wait_ring(bar.k_full, 0);
-      for (int x = 0; x < 2; x++)
-        if (active(x, 0)) scores(x, 0);
-      release(bar.k_empty, 0);
-    }
-    for (int i = 0; i < n && ok; i++) {
-      const bool more = i + 1 < n;
-      if (S::kApart) {
-        if (more) {
-          wait_ring(bar.k_full, i + 1);
-          for (int x = 0; x < 2; x++)
-            if (active(x, i + 1)) scores(x, i + 1);
-          release(bar.k_empty, i + 1);
+              for (int k = 0; k < kKeys / 16; k++)
+                umma_ta(tm_o, tm_p + pr.slot * S::kBufferP + k * 8, dv + ((k * 16 * S::kBox * 2) >> 4),
+                        idesc_o, k != 0 ? 1u : (u > begin ? 1u : 0u));
+              umma_commit(&bar.v_empty[vr.slot]);
+              // last: who has waited for it has waited for everything before it
+              umma_commit(&bar.o_full[x][pr.slot]);
+            }
+            pr.next();
+          } else if (ok && lane == 0) {
+            mbar_arrive(&bar.v_empty[vr.slot]);
+          }
+          __syncwarp();
+          vr.next();
+        };
+        // The scores are two units ahead of the values, one per buffer of S.  Where P takes the
+        // place of S they can only follow the values that free it.
+        for (int u = unit0; u < unit1 && u < unit0 + 2; u++) scores(u);
+        for (int u = unit0; ok && u < unit1; u++) {
+          if (S::kApart && u + 2 < unit1) scores(u + 2);
+          values(u);
+          if (!S::kApart && u + 2 < unit1) scores(u + 2);
         }
-        wait_ring(bar.v_full, i);
-        for (int x = 0; x < 2; x++)
-          if (active(x, i)) values(x, i);
-        release(bar.v_empty, i);
-      } else {
-        wait_ring(bar.v_full, i);
-        if (more) wait_ring(bar.k_full, i + 1);
-        for (int x = 0; x < 2; x++) {
-          if (active(x, i)) values(x, i);
-          if (more && active(x, i + 1)) scores(x, i + 1);
-        }
-        release(bar.v_empty, i);
-        if (more) release(bar.k_empty, i + 1);
       }
     }
-    if (!ok) {
-      set_status(a.status, kStatusWaitTimeoutMma);
-      *abort_flag = 1;
-    }
-  } else if (job.seq >= 0) {
+  } else {
     // ---------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    code = kStatusWaitTimeoutEpilogue;
     const int x = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;
-    const int rows = job.tokens[x] * group;
-    const bool warp_live = quarter * 32 < rows;
+    const int row_tok = row / group, row_head = row - row_tok * group;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t col_s = tmem + lanes + x * 128;
     const uint32_t col_p = tmem + lanes + S::kColP + x * S::kStrideP;
     const uint32_t col_o = tmem + lanes + S::kColO + x * S::kStrideO;
     const float c = a.scale * 1.4426950408889634f;
-    // keys [first, last] relative to block 0, of this row and of the warp's rows together
-    auto last_of = [&](int r) { return job.first_pos + x * tok + r / group; };
-    const int last = last_of(row);
-    const long long first_ll = a.window > 0 ? static_cast<long long>(last) - a.window + 1 : 0;
-    const int first = static_cast<int>(max(first_ll, -1ll));
-    const int last_min = __shfl_sync(0xffffffffu, last, 0);
-    const int first_max = __shfl_sync(0xffffffffu, first, 31);
-    bool ok = true;
-    const int count = job.end[x] - job.begin[x];
-    for (int i = 0; i < count; i++) {
-      const int key0 = (job.begin[x] + i) * kKeys;
-      uint32_t s[4][32];
-      ok = warp_wait(&bar.s_full[x], i & 1, abort_flag);
-      if (!ok) break;
-      tc_fence_after();
-      float base = 0.f;
-      if (warp_live) {
-#pragma unroll
-        for (int q = 0; q < 4; q++) tmem_ld32(col_s + 32 * q, s[q]);
-#pragma unroll
-        for (int q = 0; q < 4; q++) tmem_ld_wait32(s[q]);
-      }
-      if (S::kApart) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.s_free[x]);
-      }
-      float scale_o = 1.f;
-      if (warp_live) {
-        if (key0 + kKeys - 1 > last_min || key0 < first_max) {
-#pragma unroll
-          for (int q = 0; q < 4; q++)
-#pragma unroll
-            for (int e = 0; e < 32; e++) {
-              const int t = key0 + 32 * q + e;
-              if (t > last || t < first) s[q][e] = 0xff800000u;
-            }
+    Ring<2> sr, pr, orr;       // buffers of S being read, of P being written, of P read by MMAs
+    for (; have_job(); done_job()) {
+      const AttnJob &job = jobs[jr.slot];
+      const int rows = job.tokens[x] * group;
+      const bool warp_live = quarter * 32 < rows;
+      const int begin = job.begin[x], n = job.end[x] - begin;
+      // keys [first, last] relative to unit 0, of this row and of the warp's rows together
+      const int last = job.first_pos + x * tok + row_tok;
+      const long long first_ll = a.window > 0 ? static_cast<long long>(last) - a.window + 1 : 0;
+      const int first = static_cast<int>(max(first_ll, -1ll));
+      const int last_min = __shfl_sync(0xffffffffu, last, 0);
+      const int first_max = __shfl_sync(0xffffffffu, first, 31);
+      int o_done = 0;  // products with V waited for
+      auto wait_products = [&](int upto) {
+        for (; ok && o_done < upto; o_done++) {
+          ok = warp_wait(&bar.o_full[x][orr.slot], orr.phase, abort_flag);
+          orr.next();
         }
-        float mx[4];
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-          mx[q] = __uint_as_float(s[q][0]);
-#pragma unroll
-          for (int e = 1; e < 32; e++) mx[q] = fmaxf(mx[q], __uint_as_float(s[q][e]));
-        }
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
-        if (top > m + 8.f) {
-          scale_o = fast_exp2(m - top);
-          l *= scale_o;
-          m = top;
-        }
-        base = m == -INFINITY ? 0.f : m;
-      }
-      // the product of the block before has read P and written O
-      if (i > 0) {
-        ok = warp_wait(&bar.o_full[x], (i - 1) & 1, abort_flag);
-        if (!ok) break;
         tc_fence_after();
-      }
-      if (warp_live) {
-        if (i > 0 && __any_sync(0xffffffffu, scale_o != 1.f)) {
-#pragma unroll
-          for (int d = 0; d < D; d += 16) {
-            uint32_t o[16];
-            tmem_ld16(col_o + d, o);
-            tmem_ld_wait16(o);
-#pragma unroll
-            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * scale_o);
-            tmem_st16(col_o + d, o);
-          }
+      };
+      m = -INFINITY;
+      l = 0.f;
+      if (!warp_live) {  // no rows here: only keep step
+        for (int i = 0; ok && i < n; i++) {
+          ok = warp_wait(&bar.s_full[x][sr.slot], sr.phase, abort_flag);
+          if (S::kApart && lane == 0) mbar_arrive(&bar.s_free[x][sr.slot]);
+          sr.next();
+          if (ok) wait_products(i - 1);
+          __syncwarp();
+          if (ok && lane == 0) mbar_arrive(&bar.p_full[x][pr.slot]);
+          pr.next();
         }
-        float sum[2] = {0.f, 0.f};
+      } else if (n > 0) {
+        float scale_o = 1.f, base = 0.f;
+        uint32_t sa[2][32], sb[2][32];
+        // S of the next unit on its way to registers
+        auto fetch = [&](uint32_t (&s)[2][32]) {
+          ok = ok && warp_wait(&bar.s_full[x][sr.slot], sr.phase, abort_flag);
+          tc_fence_after();
+          tmem_ld32(col_s + sr.slot * 64, s[0]);
+          tmem_ld32(col_s + sr.slot * 64 + 32, s[1]);
+        };
+        // there, its buffer released, keys that the row does not see masked
+        auto arrived = [&](uint32_t (&s)[2][32], int i) {
+          tmem_ld_wait32(s[0]);
+          tmem_ld_wait32(s[1]);
+          if (S::kApart) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.s_free[x][sr.slot]);
+          }
+          sr.next();
+          const int key0 = (begin + i) * kKeys;
+          if (key0 + kKeys - 1 > last_min || key0 < first_max) {
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-          uint32_t p[16];
+            for (int q = 0; q < 2; q++)
+#pragma unroll
+              for (int e = 0; e < 32; e++) {
+                const int t = key0 + 32 * q + e;
+                if (t > last || t < first) s[q][e] = 0xff800000u;
+              }
+          }
+          __syncwarp();
+        };
+        auto maximum = [&](const uint32_t (&s)[2][32]) {
+          float mx[4];
+#pragma unroll
+          for (int q = 0; q < 4; q++) {
+            const uint32_t *v = &s[q >> 1][(q & 1) * 16];
+            mx[q] = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
+#pragma unroll
+            for (int e = 2; e < 16; e += 2)
+              mx[q] = max3(mx[q], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+          }
+          return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+        };
+        auto move_maximum = [&](float top) {
+          scale_o = 1.f;
+          if (top > m + 8.f) {
+            scale_o = fast_exp2(m - top);
+            l *= scale_o;
+            m = top;
+          }
+          base = m == -INFINITY ? 0.f : m;
+        };
+        uint64_t sum = 0;
+        auto exps = [&](const uint32_t (&s)[32], uint32_t (&p)[16]) {
+          const uint64_t c2 = f32x2(c, c), base2 = f32x2(-base, -base);
 #pragma unroll
           for (int e = 0; e < 16; e++) {
-            const float p0 = fast_exp2(fmaf(__uint_as_float(s[q][2 * e]), c, -base));
-            const float p1 = fast_exp2(fmaf(__uint_as_float(s[q][2 * e + 1]), c, -base));
-            sum[0] += p0;
-            sum[1] += p1;
-            p[e] = pack16(p0, p1, static_cast<T *>(nullptr));
+            float2 y = f32x2_parts(f32x2_fma(
+                f32x2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), c2, base2));
+            // a quarter of the exponentials on the FMA pipes (see poly_exp2)
+            if (e % 4 == 1)
+              y = poly_exp2<kHalf ? 4 : 3>(y);
+            else
+              y = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+            sum = f32x2_add(sum, f32x2(y.x, y.y));
+            p[e] = pack16(y.x, y.y, static_cast<T *>(nullptr));
           }
-          tmem_st16(col_p + 16 * q, p);
+        };
+        auto publish = [&]() {  // P of the unit before is in TMEM
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar.p_full[x][pr.slot]);
+          pr.next();
+        };
+        // O and P's buffer are the thread's again, O follows a moved maximum, P goes to TMEM
+        auto store = [&](const uint32_t (&p)[2][16], int i) {
+          // P's buffer was read by the product of two units ago; O is written by the last one
+          const bool moved = i > 0 && __any_sync(0xffffffffu, scale_o != 1.f);
+          wait_products(moved ? i : i - 1);
+          if (!ok) return;
+          if (moved) {
+#pragma unroll
+            for (int d = 0; d < D; d += 16) {
+              uint32_t o[16];
+              tmem_ld16(col_o + d, o);
+              tmem_ld_wait16(o);
+#pragma unroll
+              for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * scale_o);
+              tmem_st16(col_o + d, o);
+            }
+          }
+          tmem_st16(col_p + pr.slot * S::kBufferP, p[0]);
+          tmem_st16(col_p + pr.slot * S::kBufferP + 16, p[1]);
+          const float2 sums = f32x2_parts(sum);
+          l += sums.x + sums.y;
+          sum = 0;
+        };
+        // One unit.  With P apart, the next S is loaded and its maximum found, and the last P
+        // handed over, in the shadow of this unit's exponentials; with P in the place of S the
+        // MMAs wait for every P, which goes out at once.
+        auto unit = [&](const uint32_t (&cur)[2][32], uint32_t (&nxt)[2][32], int i) {
+          const bool more = i + 1 < n;
+          uint32_t p[2][16];
+          float top = -INFINITY;
+          if (S::kApart) {
+            if (more) fetch(nxt);
+            exps(cur[0], p[0]);
+            if (i > 0) publish();
+            if (more) {
+              arrived(nxt, i + 1);
+              exps(cur[1], p[1]);
+              top = maximum(nxt);
+            } else {
+              exps(cur[1], p[1]);
+            }
+            store(p, i);
+            if (!more && ok) publish();
+          } else {
+            exps(cur[0], p[0]);
+            exps(cur[1], p[1]);
+            store(p, i);
+            if (ok) publish();
+            if (more) {
+              fetch(nxt);
+              arrived(nxt, i + 1);
+              top = maximum(nxt);
+            }
+          }
+          if (more) move_maximum(top);
+        };
+        fetch(sa);
+        if (ok) {
+          arrived(sa, 0);
+          move_maximum(maximum(sa));
+          for (int i = 0; ok && i < n; i += 2) {
+            unit(sa, sb, i);
+            if (ok && i + 1 < n) unit(sb, sa, i + 1);
+          }
         }
-        l += sum[0] + sum[1];
-        tmem_st_wait();
+      }
+      const bool any = n > 0;
+      if (ok && any) wait_products(n);
+      if (split > 1) {
+        part_rows = rows;
+        part_any = any;
+        continue;  // a split launch has one job per CTA; its parts are joined below
+      }
+      if (!ok || !warp_live) continue;
+      const int head = job.kvh * group + row_head;
+      const float f = row_factor(m, l, a.sinks, head);
+      T *out = static_cast<T *>(a.out) +
+               static_cast<long long>(job.q_row0 + x * tok + row_tok) * a.out_stride +
+               static_cast<long long>(head) * D;
+#pragma unroll
+      for (int d = 0; d < D; d += 16) {
+        uint32_t o[16];
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[e] = 0u;
+        if (any) {
+          tmem_ld16(col_o + d, o);
+          tmem_ld_wait16(o);
+        }
+        if (row < rows) {
+          uint32_t w[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+            w[e] = f == 0.f ? 0u
+                            : pack16(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f,
+                                     static_cast<T *>(nullptr));
+          *reinterpret_cast<uint4 *>(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4 *>(out + d + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+        __syncwarp();
       }
       tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.p_full[x]);
     }
-    if (ok && count > 0) ok = warp_wait(&bar.o_full[x], (count - 1) & 1, abort_flag);
-    if (!ok) {
-      set_status(a.status, kStatusWaitTimeoutEpilogue);
-      *abort_flag = 1;
-    }
-    tc_fence_after();
+  }
+  if (!ok) {
+    set_status(a.status, code);
+    *abort_flag = 1;
   }
   // every copy and product of the CTA has been waited for above (unless a wait ran out)
+  tc_fence_before();
   __syncthreads();
   if (*abort_flag) {
     const uint64_t t0 = global_timer_ns();  // let what is in flight land
@@ -544,69 +838,51 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
     __syncthreads();
   }
   tc_fence_after();
-  const int x = warp >> 2, quarter = warp & 3;
-  const int row = quarter * 32 + lane;
-  const int rows = warp < 8 && job.seq >= 0 ? job.tokens[x] * group : 0;
-  if (quarter * 32 < rows && (split > 1 || !*abort_flag)) {
-    const int head = kvh * group + row % group;
-    const bool any = job.end[x] > job.begin[x];
-    float f = 1.f;
-    if (split == 1) f = row_factor(m, l, a.sinks, head);
-    T *out = static_cast<T *>(a.out) +
-             static_cast<long long>(job.q_row0 + x * tok + row / group) * a.out_stride +
-             static_cast<long long>(head) * D;
-    const uint32_t col_o = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + S::kColO + x * S::kStrideO;
-    part_m[x * 128 + row] = m;
-    part_l[x * 128 + row] = l;
-#pragma unroll
-    for (int d = 0; d < D; d += 16) {
-      uint32_t o[16];
-#pragma unroll
-      for (int e = 0; e < 16; e++) o[e] = 0u;
-      if (any) {
-        tmem_ld16(col_o + d, o);
-        tmem_ld_wait16(o);
-      }
-      if (split > 1) {
-        // 16-byte pieces of a row are permuted by the row, so that a warp's rows spread over
-        // the banks
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          *reinterpret_cast<uint4 *>(smem + part_offset<D>(x * 128 + row, d / 4 + e)) =
-              make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-      } else if (row < rows) {
-        uint32_t w[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-          w[e] = f == 0.f ? 0u
-                          : pack16(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f,
-                                   static_cast<T *>(nullptr));
-        *reinterpret_cast<uint4 *>(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
-        *reinterpret_cast<uint4 *>(out + d + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-      }
-      __syncwarp();
-    }
-  }
   if (split > 1) {
+    const int x = warp >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    if (quarter * 32 < part_rows) {
+      const uint32_t col_o = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + S::kColO + x * S::kStrideO;
+      part_m[x * 128 + row] = m;
+      part_l[x * 128 + row] = l;
+      if (part_any) {
+#pragma unroll
+        for (int d = 0; d < D; d += 16) {
+          uint32_t o[16];
+          tmem_ld16(col_o + d, o);
+          tmem_ld_wait16(o);
+          // 16-byte pieces of a row are permuted by the row, so that a warp's rows spread
+          // over the banks
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            *reinterpret_cast<uint4 *>(smem + part_offset<D>(x * 128 + row, d / 4 + e)) =
+                make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        }
+      }
+    }
     tc_fence_before();
     cluster_barrier_all();
-    // the CTAs of the cluster share the rows out among their threads, 8 elements a time
-    const int pieces = job.seq >= 0 ? (job.tokens[0] + job.tokens[1]) * group * (D / 8) : 0;
+    // the CTAs of the cluster share the rows out among their threads, 8 elements a time (the
+    // job's rows are the same in all of them)
+    const AttnJob &job = jobs[0];
+    const int pieces = job.kvh >= 0 ? (job.tokens[0] + job.tokens[1]) * group * (D / 8) : 0;
     for (int i = rank * kAttnThreads + threadIdx.x; i < pieces; i += split * kAttnThreads) {
       const int r = i / (D / 8), piece = i % (D / 8);
       const int rows_a = job.tokens[0] * group;
       const int tile = r >= rows_a, rt = r - tile * rows_a;
       const int pr = tile * 128 + rt;
-      const int head = kvh * group + rt % group;
+      const int head = job.kvh * group + rt % group;
       float mr[kAttnMaxSplit], all = -INFINITY;
-      for (int k = 0; k < split; k++) {
-        mr[k] = ld_cluster_f32(smem_u32(&part_m[pr]), k);
+#pragma unroll
+      for (int k = 0; k < kAttnMaxSplit; k++) {
+        mr[k] = k < split ? ld_cluster_f32(smem_u32(&part_m[pr]), k) : -INFINITY;
         all = fmaxf(all, mr[k]);
       }
       float sum = 0.f, acc[8];
 #pragma unroll
       for (int e = 0; e < 8; e++) acc[e] = 0.f;
-      for (int k = 0; k < split; k++) {
+#pragma unroll
+      for (int k = 0; k < kAttnMaxSplit; k++) {
         if (mr[k] == -INFINITY) continue;  // that CTA saw no key of this row
         const float w = fast_exp2(mr[k] - all);
         sum += ld_cluster_f32(smem_u32(&part_l[pr]), k) * w;
@@ -641,6 +917,7 @@ static int attention_launch(const gptoss_attention_args_t &a, int sms, cudaStrea
   typedef AttnShape<D> S;
   const int group = a.n_q_heads / a.n_kv_heads, tok = 128 / group;
   const long long slots = a.n_tokens / (2 * tok) + static_cast<long long>(a.n_seqs);
+  if (slots > INT32_MAX) return decode_error(GPTOSS_E_CAPACITY, "prompt_attention: too many rows and sequences");
   CUtensorMap map_q, map_k, map_v;
   std::string err;
   const bool fp16 = !std::is_same<T, bf16>::value;
@@ -659,10 +936,17 @@ static int attention_launch(const gptoss_attention_args_t &a, int sms, cudaStrea
   const long long blocks = (most + kKeys - 1) / kKeys;
   int split = 1;
   while (split < kAttnMaxSplit && slots * a.n_kv_heads * split * 2 <= sms && blocks >= 4 * split) split *= 2;
-  const long long grid = slots * a.n_kv_heads * split;
+  const long long units = slots * a.n_kv_heads;
+  const long long grid = units * split;
   if (grid > INT32_MAX) return decode_error(GPTOSS_E_CAPACITY, "prompt_attention: too many rows for one launch");
   auto kernel = prompt_attention_kernel<T, D>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes);
+  // the kernel's warps share out the registers of a launch with 168 each: with fewer they would
+  // wait for more for ever
+  cudaFuncAttributes fa = {};
+  cudaError_t e = cudaFuncGetAttributes(&fa, kernel);
+  if (e == cudaSuccess && fa.numRegs != 168)
+    return decode_error(GPTOSS_E_STATE, "prompt_attention: built with %d registers, not 168", fa.numRegs);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes);
   if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
