@@ -43,8 +43,9 @@
 
 namespace gptoss {
 
-constexpr int kAttnThreads = 384;
-constexpr int kKeys = 64;             // keys per unit
+constexpr int kAttnThreads = 640;
+constexpr int kAttnSoftmaxWarps = 16;
+constexpr int kKeys = 128;            // keys per unit
 constexpr int kAttnTmemCols = 512;
 constexpr int kAttnMaxSplit = 8;      // CTAs of a cluster that share a pair of tiles
 constexpr int kJobs = 4;              // jobs that may be at work in different warps
@@ -57,13 +58,14 @@ struct AttnShape {
   static constexpr int kPanelBytes = kKeys * kBox * 2;    // a panel of K or V
   static constexpr int kQBytes = kPanels * kQPanelBytes;
   static constexpr int kUnitBytes = kPanels * kPanelBytes;
-  static constexpr int kStages = D == 128 ? 4 : 8;        // units of K and of V in flight
+  static constexpr int kStages = D == 128 ? 2 : 4;        // units of K and of V in flight
   static constexpr int kRingBytes = kStages * kUnitBytes;
-  // TMEM: S of tile x, buffer j at column 128 x + 64 j.  P beside S (2 x 2 x 32 columns, then
-  // O 2 x D), or in the place of the S that it was made from.
+  // TMEM: S of tile x at column 128 x.  P beside S (2 x 64 columns, then O 2 x D), or in the
+  // place of the S that it was made from.
   static constexpr bool kApart = D <= 64;
+  static constexpr int kIssuers = kApart ? 2 : 1;         // warps that issue MMAs
   static constexpr int kColP = kApart ? 256 : 0;
-  static constexpr int kStrideP = kApart ? 64 : 128, kBufferP = kApart ? 32 : 64;
+  static constexpr int kStrideP = kApart ? 64 : 128;
   static constexpr int kColO = kApart ? 384 : 256;
   static constexpr int kStrideO = kApart ? 64 : 128;
   static constexpr int kOperandBytes = 2 * kQBytes + 2 * kRingBytes;
@@ -73,9 +75,8 @@ struct AttnShape {
 
 struct AttnBarriers {
   uint64_t job_full[kJobs], job_empty[kJobs], steal;
-  uint64_t q_full[2], q_empty[2], v_tail;
-  uint64_t s_full[2][2], s_free[2][2], p_full[2][2], o_full[2][2];  // [tile][buffer]
-  uint64_t k_full[8], k_empty[8], v_full[8], v_empty[8];
+  uint64_t q_full[2], q_empty[2], s_full[2], s_free[2], p_full[2], o_full[2], v_tail;
+  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
 };
 
 // The rows and keys of one job.
@@ -351,6 +352,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
   __shared__ __align__(16) unsigned char steal_answer[16];
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_word;
+  __shared__ float exchange[2][2][2][128];  // [parity][tile][half of the columns][row]
   __shared__ float part_m[256], part_l[256];
   unsigned char *smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
   unsigned char *sm_q = smem, *sm_k = smem + 2 * S::kQBytes, *sm_v = sm_k + S::kRingBytes;
@@ -359,10 +361,10 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = split > 1 ? static_cast<int>(cluster_cta_rank()) : 0;
 
-  if (warp == 9) {
+  if (warp == 17) {
     tmem_alloc(&tmem_holder, kAttnTmemCols);
     tmem_relinquish();
-  } else if (warp == 8) {
+  } else if (warp == 16) {
     if (elect_one()) {
       tma_prefetch_desc(&map_q);
       tma_prefetch_desc(&map_k);
@@ -371,25 +373,23 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
   } else if (threadIdx.x == 0) {
     for (int j = 0; j < kJobs; j++) {
       mbar_init(&bar.job_full[j], 1);
-      mbar_init(&bar.job_empty[j], 10);  // 8 softmax warps, 2 issuing warps
+      mbar_init(&bar.job_empty[j], kAttnSoftmaxWarps + S::kIssuers);
     }
     mbar_init(&bar.steal, 1);
     mbar_init(&bar.v_tail, 1);
     for (int x = 0; x < 2; x++) {
       mbar_init(&bar.q_full[x], 1);
       mbar_init(&bar.q_empty[x], 1);
-      for (int j = 0; j < 2; j++) {
-        mbar_init(&bar.s_full[x][j], 1);
-        mbar_init(&bar.s_free[x][j], 4);
-        mbar_init(&bar.p_full[x][j], 4);
-        mbar_init(&bar.o_full[x][j], 1);
-      }
+      mbar_init(&bar.s_full[x], 1);
+      mbar_init(&bar.s_free[x], kAttnSoftmaxWarps / 2);
+      mbar_init(&bar.p_full[x], kAttnSoftmaxWarps / 2);
+      mbar_init(&bar.o_full[x], 1);
     }
     for (int s = 0; s < S::kStages; s++) {
       mbar_init(&bar.k_full[s], 1);
-      mbar_init(&bar.k_empty[s], 2);
+      mbar_init(&bar.k_empty[s], S::kIssuers);
       mbar_init(&bar.v_full[s], 1);
-      mbar_init(&bar.v_empty[s], 2);
+      mbar_init(&bar.v_empty[s], S::kIssuers);
     }
     abort_word = 0;
     mbar_fence_init();
@@ -416,11 +416,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
     jr.next();
   };
 
-  // Registers: 384 threads were launched with 168 each (64512); the four warps that hold no
-  // tiles keep 72 and the eight that do take 216 (128 * 72 + 256 * 216 = 64512).
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 8) {
+  // Registers: 640 threads were launched with 96 each (61440); the four warps that hold no
+  // tiles keep 64 and the sixteen that do take 104 (128 * 64 + 512 * 104 = 61440).
+  if (warp >= kAttnSoftmaxWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == 16) {
       // -------------------------------------------------------------- jobs and loads
       // The grid has a CTA (with a split: a cluster) per pair of tiles; this CTA does its own
       // and then, one at a time, those of CTAs that have not started, in their order.  It asks
@@ -519,101 +519,144 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
         ask();
         answer();
       }
-    } else if (warp < 11) {
+    } else if (warp < 17 + S::kIssuers) {
       // -------------------------------------------------------------- MMAs
+      // With P beside S a warp per tile issues; the tiles then never wait for each other.  With
+      // P in S's place a tile's next scores follow its values, the MMAs are on the tile's
+      // critical path, and one warp keeps the two tiles' batches apart (interleaved they would
+      // both take twice as long and the exponentials would wait for both).
       code = kStatusWaitTimeoutMma;
       constexpr uint32_t idesc_s = attn_idesc(kHalf, kKeys, false);
       constexpr uint32_t idesc_o = attn_idesc(kHalf, D, true);
-      const int x = warp - 9;
-      const uint64_t desc_q = attn_desc<D>(smem_u32(sm_q + x * S::kQBytes));
+      const uint64_t desc_q = attn_desc<D>(smem_u32(sm_q));
       const uint64_t desc_k = attn_desc<D>(smem_u32(sm_k));
       const uint64_t desc_v = attn_desc<D>(smem_u32(sm_v));
-      const uint32_t tm_s = tmem + x * 128, tm_p = tmem + S::kColP + x * S::kStrideP;
-      const uint32_t tm_o = tmem + S::kColO + x * S::kStrideO;
       Ring<S::kStages> kr, vr;
-      Ring<2> sr, pr;  // buffers of S being written, of P being read
-      uint32_t q_phase = 0;
+      struct Tile {
+        int x, begin, end;
+        uint32_t q_phase, free_phase, p_phase;
+      };
+      auto scores = [&](Tile &t, int u, bool last_reader) {  // S = Q K_u^T
+        ok = ok && warp_wait(&bar.k_full[kr.slot], kr.phase, abort_flag);
+        const bool active = u >= t.begin && u < t.end;
+        if (active) {
+          if (u == t.begin) {
+            ok = ok && warp_wait(&bar.q_full[t.x], t.q_phase, abort_flag);
+            t.q_phase ^= 1u;
+          }
+          // S is free again once its readers have it in registers; where P takes its place, the
+          // product that read that P was issued before (one warp's products run in order)
+          if (S::kApart) {
+            ok = ok && warp_wait(&bar.s_free[t.x], t.free_phase, abort_flag);
+            t.free_phase ^= 1u;
+          }
+          tc_fence_after();
+        }
+        if (ok && elect_one()) {
+          if (active) {
+            const uint64_t dq = desc_q + (t.x * S::kQBytes >> 4);
+            const uint64_t dk = desc_k + (kr.slot * S::kUnitBytes >> 4);
+#pragma unroll
+            for (int k = 0; k < D / 16; k++) {
+              constexpr int kPerPanel = S::kBox / 16;
+              umma_bf16(tmem + t.x * 128,
+                        dq + (((k / kPerPanel) * S::kQPanelBytes + (k % kPerPanel) * 32) >> 4),
+                        dk + (((k / kPerPanel) * S::kPanelBytes + (k % kPerPanel) * 32) >> 4),
+                        idesc_s, k != 0);
+            }
+            umma_commit(&bar.s_full[t.x]);
+            if (u == t.end - 1) umma_commit(&bar.q_empty[t.x]);
+          }
+          if (last_reader) umma_commit(&bar.k_empty[kr.slot]);
+        }
+        __syncwarp();
+      };
+      auto values = [&](Tile &t, int u, bool last_reader) {  // O += P V_u
+        ok = ok && warp_wait(&bar.v_full[vr.slot], vr.phase, abort_flag);
+        const bool active = u >= t.begin && u < t.end;
+        if (active) {
+          ok = ok && warp_wait(&bar.p_full[t.x], t.p_phase, abort_flag);
+          t.p_phase ^= 1u;
+          tc_fence_after();
+        }
+        if (ok && elect_one()) {
+          if (active) {
+            const uint64_t dv = desc_v + (vr.slot * S::kUnitBytes >> 4);
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; k++)
+              umma_ta(tmem + S::kColO + t.x * S::kStrideO, tmem + S::kColP + t.x * S::kStrideP + k * 8,
+                      dv + ((k * 16 * S::kBox * 2) >> 4), idesc_o, k != 0 ? 1u : (u > t.begin ? 1u : 0u));
+          }
+          if (last_reader) umma_commit(&bar.v_empty[vr.slot]);
+          // last: who has waited for it has waited for everything before it
+          if (active) umma_commit(&bar.o_full[t.x]);
+        }
+        __syncwarp();
+      };
+      Tile t0 = {S::kApart ? warp - 17 : 0, 0, 0, 0u, 1u, 0u}, t1 = {1, 0, 0, 0u, 1u, 0u};
       for (; have_job(); done_job()) {
         const AttnJob &job = jobs[jr.slot];
-        const int begin = job.begin[x], end = job.end[x], unit0 = job.unit0, unit1 = job.unit1;
-        auto scores = [&](int u) {  // S = Q K_u^T
-          ok = ok && warp_wait(&bar.k_full[kr.slot], kr.phase, abort_flag);
-          const bool active = u >= begin && u < end;
-          if (active) {
-            if (u == begin) {
-              ok = ok && warp_wait(&bar.q_full[x], q_phase, abort_flag);
-              q_phase ^= 1u;
+        const int unit0 = job.unit0, unit1 = job.unit1;
+        t0.begin = job.begin[t0.x];
+        t0.end = job.end[t0.x];
+        t1.begin = job.begin[1];
+        t1.end = job.end[1];
+        if (S::kApart) {
+          for (int u = unit0; ok && u <= unit1; u++) {
+            if (u < unit1) {
+              scores(t0, u, true);
+              kr.next();
             }
-            // S is free again once its readers have it in registers; where P takes its place,
-            // the product that read that P was issued before (one warp's products run in order)
-            if (S::kApart) ok = ok && warp_wait(&bar.s_free[x][sr.slot], sr.phase ^ 1u, abort_flag);
-            tc_fence_after();
-            if (ok && elect_one()) {
-              const uint64_t dk = desc_k + (kr.slot * S::kUnitBytes >> 4);
-#pragma unroll
-              for (int k = 0; k < D / 16; k++) {
-                constexpr int kPerPanel = S::kBox / 16;
-                umma_bf16(tm_s + sr.slot * 64,
-                          desc_q + (((k / kPerPanel) * S::kQPanelBytes + (k % kPerPanel) * 32) >> 4),
-                          dk + (((k / kPerPanel) * S::kPanelBytes + (k % kPerPanel) * 32) >> 4),
-                          idesc_s, k != 0);
-              }
-              umma_commit(&bar.s_full[x][sr.slot]);
-              umma_commit(&bar.k_empty[kr.slot]);
-              if (u == end - 1) umma_commit(&bar.q_empty[x]);
+            if (u > unit0) {
+              values(t0, u - 1, true);
+              vr.next();
             }
-            sr.next();
-          } else if (ok && lane == 0) {
-            mbar_arrive(&bar.k_empty[kr.slot]);
           }
-          __syncwarp();
-          kr.next();
-        };
-        auto values = [&](int u) {  // O += P V_u
-          ok = ok && warp_wait(&bar.v_full[vr.slot], vr.phase, abort_flag);
-          if (u >= begin && u < end) {
-            ok = ok && warp_wait(&bar.p_full[x][pr.slot], pr.phase, abort_flag);
-            tc_fence_after();
-            if (ok && elect_one()) {
-              const uint64_t dv = desc_v + (vr.slot * S::kUnitBytes >> 4);
-#pragma unroll
-              for (int k = 0; k < kKeys / 16; k++)
-                umma_ta(tm_o, tm_p + pr.slot * S::kBufferP + k * 8, dv + ((k * 16 * S::kBox * 2) >> 4),
-                        idesc_o, k != 0 ? 1u : (u > begin ? 1u : 0u));
-              umma_commit(&bar.v_empty[vr.slot]);
-              // last: who has waited for it has waited for everything before it
-              umma_commit(&bar.o_full[x][pr.slot]);
-            }
-            pr.next();
-          } else if (ok && lane == 0) {
-            mbar_arrive(&bar.v_empty[vr.slot]);
+        } else {
+          if (unit0 < unit1) {
+            scores(t0, unit0, false);
+            scores(t1, unit0, true);
+            kr.next();
           }
-          __syncwarp();
-          vr.next();
-        };
-        // The scores are two units ahead of the values, one per buffer of S.  Where P takes the
-        // place of S they can only follow the values that free it.
-        for (int u = unit0; u < unit1 && u < unit0 + 2; u++) scores(u);
-        for (int u = unit0; ok && u < unit1; u++) {
-          if (S::kApart && u + 2 < unit1) scores(u + 2);
-          values(u);
-          if (!S::kApart && u + 2 < unit1) scores(u + 2);
+          for (int u = unit0; ok && u < unit1; u++) {
+            const bool more = u + 1 < unit1;
+            values(t0, u, false);
+            if (more) scores(t0, u + 1, false);
+            values(t1, u, true);
+            if (more) {
+              scores(t1, u + 1, true);
+              kr.next();
+            }
+            vr.next();
+          }
         }
       }
     }
   } else {
     // ---------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     code = kStatusWaitTimeoutEpilogue;
-    const int x = warp >> 2, quarter = warp & 3;
+    // two warps per 32 rows: a thread has a row and 64 of a unit's 128 keys
+    const int x = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
     const int row = quarter * 32 + lane;
-    const int row_tok = row / group, row_head = row - row_tok * group;
+    const int row_tok = row / group;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t col_s = tmem + lanes + x * 128;
-    const uint32_t col_p = tmem + lanes + S::kColP + x * S::kStrideP;
-    const uint32_t col_o = tmem + lanes + S::kColO + x * S::kStrideO;
+    const uint32_t col_s = tmem + lanes + x * 128 + half * 64;
+    const uint32_t col_p = tmem + lanes + S::kColP + x * S::kStrideP + half * 32;
+    const uint32_t col_o = tmem + lanes + S::kColO + x * S::kStrideO + half * (D / 2);
     const float c = a.scale * 1.4426950408889634f;
-    Ring<2> sr, pr, orr;       // buffers of S being read, of P being written, of P read by MMAs
+    uint32_t s_phase = 0, o_phase = 0, parity = 0;
+    // Hands over a value of the thread's row and returns that of the thread with the row's other
+    // keys.  The barrier has no limit of its own: a warp that gives up raises the abort flag,
+    // which is looked at before every call, and arrives once in its partner's place.
+    const int pair_barrier = 1 + x * 4 + quarter;
+    auto both = [&](float mine) {
+      exchange[parity][x][half][row] = mine;
+      named_barrier_sync(pair_barrier, 64);
+      const float other = exchange[parity][x][half ^ 1][row];
+      parity ^= 1u;
+      return other;
+    };
     for (; have_job(); done_job()) {
       const AttnJob &job = jobs[jr.slot];
       const int rows = job.tokens[x] * group;
@@ -625,48 +668,24 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
       const int first = static_cast<int>(max(first_ll, -1ll));
       const int last_min = __shfl_sync(0xffffffffu, last, 0);
       const int first_max = __shfl_sync(0xffffffffu, first, 31);
-      int o_done = 0;  // products with V waited for
-      auto wait_products = [&](int upto) {
-        for (; ok && o_done < upto; o_done++) {
-          ok = warp_wait(&bar.o_full[x][orr.slot], orr.phase, abort_flag);
-          orr.next();
-        }
-        tc_fence_after();
-      };
       m = -INFINITY;
       l = 0.f;
-      if (!warp_live) {  // no rows here: only keep step
-        for (int i = 0; ok && i < n; i++) {
-          ok = warp_wait(&bar.s_full[x][sr.slot], sr.phase, abort_flag);
-          if (S::kApart && lane == 0) mbar_arrive(&bar.s_free[x][sr.slot]);
-          sr.next();
-          if (ok) wait_products(i - 1);
-          __syncwarp();
-          if (ok && lane == 0) mbar_arrive(&bar.p_full[x][pr.slot]);
-          pr.next();
-        }
-      } else if (n > 0) {
-        float scale_o = 1.f, base = 0.f;
-        uint32_t sa[2][32], sb[2][32];
-        // S of the next unit on its way to registers
-        auto fetch = [&](uint32_t (&s)[2][32]) {
-          ok = ok && warp_wait(&bar.s_full[x][sr.slot], sr.phase, abort_flag);
-          tc_fence_after();
-          tmem_ld32(col_s + sr.slot * 64, s[0]);
-          tmem_ld32(col_s + sr.slot * 64 + 32, s[1]);
-        };
-        // there, its buffer released, keys that the row does not see masked
-        auto arrived = [&](uint32_t (&s)[2][32], int i) {
+      for (int i = 0; i < n; i++) {
+        ok = warp_wait(&bar.s_full[x], s_phase, abort_flag) && !*abort_flag;
+        s_phase ^= 1u;
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s[2][32], p[2][16];
+        if (warp_live) {
+          tmem_ld32(col_s, s[0]);
+          tmem_ld32(col_s + 32, s[1]);
           tmem_ld_wait32(s[0]);
           tmem_ld_wait32(s[1]);
-          if (S::kApart) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bar.s_free[x][sr.slot]);
-          }
-          sr.next();
-          const int key0 = (begin + i) * kKeys;
-          if (key0 + kKeys - 1 > last_min || key0 < first_max) {
+        }
+        float scale_o = 1.f;
+        if (warp_live) {
+          const int key0 = (begin + i) * kKeys + half * 64;
+          if (key0 + 63 > last_min || key0 < first_max) {
 #pragma unroll
             for (int q = 0; q < 2; q++)
 #pragma unroll
@@ -675,9 +694,6 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
                 if (t > last || t < first) s[q][e] = 0xff800000u;
               }
           }
-          __syncwarp();
-        };
-        auto maximum = [&](const uint32_t (&s)[2][32]) {
           float mx[4];
 #pragma unroll
           for (int q = 0; q < 4; q++) {
@@ -687,49 +703,48 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
             for (int e = 2; e < 16; e += 2)
               mx[q] = max3(mx[q], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
           }
-          return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
-        };
-        auto move_maximum = [&](float top) {
-          scale_o = 1.f;
+          float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+          top = fmaxf(top, both(top));
+          if (S::kApart) {  // (the barrier in `both` has seen every lane's S in registers)
+            tc_fence_before();
+            if (lane == 0) mbar_arrive(&bar.s_free[x]);
+          }
           if (top > m + 8.f) {
             scale_o = fast_exp2(m - top);
             l *= scale_o;
             m = top;
           }
-          base = m == -INFINITY ? 0.f : m;
-        };
-        uint64_t sum = 0;
-        auto exps = [&](const uint32_t (&s)[32], uint32_t (&p)[16]) {
+          const float base = m == -INFINITY ? 0.f : m;
           const uint64_t c2 = f32x2(c, c), base2 = f32x2(-base, -base);
+          uint64_t sum = 0;
 #pragma unroll
-          for (int e = 0; e < 16; e++) {
-            float2 y = f32x2_parts(f32x2_fma(
-                f32x2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), c2, base2));
-            // a quarter of the exponentials on the FMA pipes (see poly_exp2)
-            if (e % 4 == 1)
-              y = poly_exp2<kHalf ? 4 : 3>(y);
-            else
-              y = make_float2(fast_exp2(y.x), fast_exp2(y.y));
-            sum = f32x2_add(sum, f32x2(y.x, y.y));
-            p[e] = pack16(y.x, y.y, static_cast<T *>(nullptr));
-          }
-        };
-        auto publish = [&]() {  // P of the unit before is in TMEM
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bar.p_full[x][pr.slot]);
-          pr.next();
-        };
-        // O and P's buffer are the thread's again, O follows a moved maximum, P goes to TMEM
-        auto store = [&](const uint32_t (&p)[2][16], int i) {
-          // P's buffer was read by the product of two units ago; O is written by the last one
-          const bool moved = i > 0 && __any_sync(0xffffffffu, scale_o != 1.f);
-          wait_products(moved ? i : i - 1);
-          if (!ok) return;
-          if (moved) {
+          for (int q = 0; q < 2; q++)
 #pragma unroll
-            for (int d = 0; d < D; d += 16) {
+            for (int e = 0; e < 16; e++) {
+              float2 y = f32x2_parts(f32x2_fma(
+                  f32x2(__uint_as_float(s[q][2 * e]), __uint_as_float(s[q][2 * e + 1])), c2, base2));
+              // a quarter of the exponentials on the FMA pipes (see poly_exp2)
+              if (e % 4 == 1)
+                y = poly_exp2<kHalf ? 4 : 3>(y);
+              else
+                y = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+              sum = f32x2_add(sum, f32x2(y.x, y.y));
+              p[q][e] = pack16(y.x, y.y, static_cast<T *>(nullptr));
+            }
+          const float2 sums = f32x2_parts(sum);
+          l += sums.x + sums.y;
+        }
+        if (S::kApart && !warp_live && lane == 0) mbar_arrive(&bar.s_free[x]);
+        if (i > 0) {  // the product of the unit before has read P and written O
+          ok = warp_wait(&bar.o_full[x], o_phase, abort_flag);
+          o_phase ^= 1u;
+          if (!ok) break;
+          tc_fence_after();
+        }
+        if (warp_live) {
+          if (i > 0 && __any_sync(0xffffffffu, scale_o != 1.f)) {
+#pragma unroll
+            for (int d = 0; d < D / 2; d += 16) {
               uint32_t o[16];
               tmem_ld16(col_o + d, o);
               tmem_ld_wait16(o);
@@ -738,70 +753,43 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
               tmem_st16(col_o + d, o);
             }
           }
-          tmem_st16(col_p + pr.slot * S::kBufferP, p[0]);
-          tmem_st16(col_p + pr.slot * S::kBufferP + 16, p[1]);
-          const float2 sums = f32x2_parts(sum);
-          l += sums.x + sums.y;
-          sum = 0;
-        };
-        // One unit.  With P apart, the next S is loaded and its maximum found, and the last P
-        // handed over, in the shadow of this unit's exponentials; with P in the place of S the
-        // MMAs wait for every P, which goes out at once.
-        auto unit = [&](const uint32_t (&cur)[2][32], uint32_t (&nxt)[2][32], int i) {
-          const bool more = i + 1 < n;
-          uint32_t p[2][16];
-          float top = -INFINITY;
-          if (S::kApart) {
-            if (more) fetch(nxt);
-            exps(cur[0], p[0]);
-            if (i > 0) publish();
-            if (more) {
-              arrived(nxt, i + 1);
-              exps(cur[1], p[1]);
-              top = maximum(nxt);
-            } else {
-              exps(cur[1], p[1]);
-            }
-            store(p, i);
-            if (!more && ok) publish();
-          } else {
-            exps(cur[0], p[0]);
-            exps(cur[1], p[1]);
-            store(p, i);
-            if (ok) publish();
-            if (more) {
-              fetch(nxt);
-              arrived(nxt, i + 1);
-              top = maximum(nxt);
-            }
-          }
-          if (more) move_maximum(top);
-        };
-        fetch(sa);
-        if (ok) {
-          arrived(sa, 0);
-          move_maximum(maximum(sa));
-          for (int i = 0; ok && i < n; i += 2) {
-            unit(sa, sb, i);
-            if (ok && i + 1 < n) unit(sb, sa, i + 1);
-          }
+          tmem_st16(col_p, p[0]);
+          tmem_st16(col_p + 16, p[1]);
+          tmem_st_wait();
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.p_full[x]);
       }
       const bool any = n > 0;
-      if (ok && any) wait_products(n);
+      if (ok && any) {
+        ok = warp_wait(&bar.o_full[x], o_phase, abort_flag);
+        o_phase ^= 1u;
+        tc_fence_after();
+      }
+      if (warp_live) {
+        ok = ok && !*abort_flag;
+        if (ok) {
+          l += both(l);
+        } else {
+          *abort_flag = 1;
+          __threadfence_block();
+          asm volatile("bar.arrive %0, 64;" ::"r"(pair_barrier) : "memory");
+        }
+      }
       if (split > 1) {
         part_rows = rows;
         part_any = any;
         continue;  // a split launch has one job per CTA; its parts are joined below
       }
       if (!ok || !warp_live) continue;
-      const int head = job.kvh * group + row_head;
+      const int head = job.kvh * group + row - row_tok * group;
       const float f = row_factor(m, l, a.sinks, head);
       T *out = static_cast<T *>(a.out) +
                static_cast<long long>(job.q_row0 + x * tok + row_tok) * a.out_stride +
-               static_cast<long long>(head) * D;
+               static_cast<long long>(head) * D + half * (D / 2);
 #pragma unroll
-      for (int d = 0; d < D; d += 16) {
+      for (int d = 0; d < D / 2; d += 16) {
         uint32_t o[16];
 #pragma unroll
         for (int e = 0; e < 16; e++) o[e] = 0u;
@@ -839,15 +827,18 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
   }
   tc_fence_after();
   if (split > 1) {
-    const int x = warp >> 2, quarter = warp & 3;
+    const int x = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     if (quarter * 32 < part_rows) {
-      const uint32_t col_o = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + S::kColO + x * S::kStrideO;
-      part_m[x * 128 + row] = m;
-      part_l[x * 128 + row] = l;
+      const uint32_t col_o = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + S::kColO +
+                             x * S::kStrideO + half * (D / 2);
+      if (half == 0) {
+        part_m[x * 128 + row] = m;
+        part_l[x * 128 + row] = l;
+      }
       if (part_any) {
 #pragma unroll
-        for (int d = 0; d < D; d += 16) {
+        for (int d = 0; d < D / 2; d += 16) {
           uint32_t o[16];
           tmem_ld16(col_o + d, o);
           tmem_ld_wait16(o);
@@ -855,7 +846,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
           // over the banks
 #pragma unroll
           for (int e = 0; e < 4; e++)
-            *reinterpret_cast<uint4 *>(smem + part_offset<D>(x * 128 + row, d / 4 + e)) =
+            *reinterpret_cast<uint4 *>(smem + part_offset<D>(x * 128 + row, (half * (D / 2) + d) / 4 + e)) =
                 make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
         }
       }
@@ -906,7 +897,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 17) {
     tc_fence_after();
     tmem_dealloc(tmem, kAttnTmemCols);
   }
@@ -940,12 +931,12 @@ static int attention_launch(const gptoss_attention_args_t &a, int sms, cudaStrea
   const long long grid = units * split;
   if (grid > INT32_MAX) return decode_error(GPTOSS_E_CAPACITY, "prompt_attention: too many rows for one launch");
   auto kernel = prompt_attention_kernel<T, D>;
-  // the kernel's warps share out the registers of a launch with 168 each: with fewer they would
+  // the kernel's warps share out the registers of a launch with 96 each: with fewer they would
   // wait for more for ever
   cudaFuncAttributes fa = {};
   cudaError_t e = cudaFuncGetAttributes(&fa, kernel);
-  if (e == cudaSuccess && fa.numRegs != 168)
-    return decode_error(GPTOSS_E_STATE, "prompt_attention: built with %d registers, not 168", fa.numRegs);
+  if (e == cudaSuccess && fa.numRegs != 96)
+    return decode_error(GPTOSS_E_STATE, "prompt_attention: built with %d registers, not 96", fa.numRegs);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes);
   if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg = {};
