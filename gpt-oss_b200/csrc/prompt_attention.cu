@@ -686,13 +686,17 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
         if (warp_live) {
           const int key0 = (begin + i) * kKeys + half * 64;
           if (key0 + 63 > last_min || key0 < first_max) {
+            // one bit per key, so that a key costs a bit test and a select
 #pragma unroll
-            for (int q = 0; q < 2; q++)
+            for (int q = 0; q < 2; q++) {
+              const int lo = first - key0 - 32 * q, hi = last - key0 - 32 * q;
+              const uint32_t from = lo <= 0 ? 0xffffffffu : (lo > 31 ? 0u : 0xffffffffu << lo);
+              const uint32_t upto = hi >= 31 ? 0xffffffffu : (hi < 0 ? 0u : (2u << hi) - 1u);
+              const uint32_t seen = from & upto;
 #pragma unroll
-              for (int e = 0; e < 32; e++) {
-                const int t = key0 + 32 * q + e;
-                if (t > last || t < first) s[q][e] = 0xff800000u;
-              }
+              for (int e = 0; e < 32; e++)
+                if (!(seen & (1u << e))) s[q][e] = 0xff800000u;
+            }
           }
           float mx[4];
 #pragma unroll
@@ -723,8 +727,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
             for (int e = 0; e < 16; e++) {
               float2 y = f32x2_parts(f32x2_fma(
                   f32x2(__uint_as_float(s[q][2 * e]), __uint_as_float(s[q][2 * e + 1])), c2, base2));
-              // a quarter of the exponentials on the FMA pipes (see poly_exp2)
-              if (e % 4 == 1)
+              // an eighth of the exponentials on the FMA pipes (see poly_exp2)
+              if (e % 8 == 1)
                 y = poly_exp2<kHalf ? 4 : 3>(y);
               else
                 y = make_float2(fast_exp2(y.x), fast_exp2(y.y));
