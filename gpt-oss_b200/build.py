@@ -16,8 +16,8 @@ LIB = PKG_DIR / "libgptoss_moe_b200.so"
 
 CU_SOURCES = ["moe_api.cu", "router.cu", "permute.cu", "grouped_gemm.cu", "grouped_gemm_pair.cu",
               "weights.cu", "mxfp4.cu", "ep.cu", "decode.cu", "rope.cu",
-              "prompt_attention.cu", "sample.cu"]
-HEADERS = ["common.cuh", "decode_ops.h", "engine.h", "ep.h", "gemm_epilogue.cuh", "umma_2sm.cuh"]
+              "prompt_attention.cu", "token_attention.cu", "sample.cu"]
+HEADERS = ["attention_rows.cuh", "common.cuh", "decode_ops.h", "engine.h", "ep.h", "gemm_epilogue.cuh", "umma_2sm.cuh"]
 
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "--threads", "0",

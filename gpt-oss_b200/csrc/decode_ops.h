@@ -64,6 +64,9 @@ inline int launch_result(const char *what, cudaError_t e = cudaSuccess) {
 // Multiprocessors of the device (looked up once per device).
 int sm_count(int device);
 
+// token_attention.cu: prompt attention of sequences with a few query rows each
+int launch_token_attention(const gptoss_attention_args_t &a, int sms, cudaStream_t st);
+
 inline bool aligned(const void *p, size_t bytes) {
   return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
 }

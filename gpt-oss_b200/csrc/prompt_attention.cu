@@ -29,17 +29,12 @@
 // Probabilities are rounded to the 16-bit type for the second product (tensor cores take both
 // operands in one type); their sum is taken in fp32 before that rounding.
 #include <cuda.h>
-#include <cuda_fp16.h>
-#include <math.h>
 
 #include <algorithm>
 #include <string>
 #include <type_traits>
 
-#include "common.cuh"
-#include "decode_ops.h"
-#include "engine.h"
-#include "umma_2sm.cuh"
+#include "attention_rows.cuh"
 
 namespace gptoss {
 
@@ -91,11 +86,6 @@ struct AttnJob {
   int unit0, unit1;       // units of this CTA
 };
 
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
@@ -148,11 +138,6 @@ __device__ __forceinline__ float2 poly_exp2(float2 x) {
   return make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(m.x) << 23)),
                      __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(m.y) << 23)));
 }
-__device__ __forceinline__ uint32_t pack16(float lo, float hi, bf16 *) { return pack_bf16(lo, hi); }
-__device__ __forceinline__ uint32_t pack16(float lo, float hi, __half *) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
 // one CTA, M operand in tensor memory
 __device__ __forceinline__ void umma_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b,
                                         uint32_t idesc, uint32_t accumulate) {
@@ -175,13 +160,6 @@ __device__ __forceinline__ void tma_load_3d(void *smem_dst, const void *tmap, ui
       : "r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)),
         "r"(c0), "r"(c1), "r"(c2)
       : "memory");
-}
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t cta) {
-  uint32_t remote;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(cta));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
-  return v;
 }
 
 // A wait whose outcome the whole warp shares (what follows is issued by the converged warp).
@@ -210,83 +188,34 @@ __host__ __device__ constexpr uint32_t attn_idesc(bool fp16, int n, bool b_n_maj
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
 }
 
-__device__ __forceinline__ void ld_cluster_f32x4(uint32_t addr, uint32_t cta, float *v) {
-  uint32_t remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(cta));
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
-               : "r"(remote)
-               : "memory");
-}
 // Byte offset of 16-byte piece `piece` of fp32 row `row` among the partial outputs.
 template <int D>
 __device__ __forceinline__ uint32_t part_offset(int row, int piece) {
   return static_cast<uint32_t>((row * (D / 4) + (piece ^ (row & 7))) * 16);
 }
-// What a row's sum of p v is multiplied with: 1 / (l + 2^(sink' - m)); 0 where no key was seen.
-__device__ __forceinline__ float row_factor(float m, float l, const float *sinks, int head) {
-  if (m == -INFINITY) return 0.f;
-  if (!sinks) return 1.f / l;
-  const float sink = sinks[head] * 1.4426950408889634f;
-  const float all = fmaxf(m, sink);
-  const float f = fast_exp2(m - all);
-  return f / (l * f + fast_exp2(sink - all));
-}
-
-// Slots: a pair of tiles covers 2 * tok tokens; sequence i's pairs start at slot
-// q_start[i] / (2 tok) + i, which leaves room for a partial pair per sequence and needs no
-// prefix sum.  One warp finds the slot's sequence by counting the starts at or before it.
-// Returns (warp-uniform) whether there is anything to do for the slot.
+// The job of a slot (a pair of tiles) and KV head, for this CTA's share of the keys.
 __device__ bool attn_find_job(const gptoss_attention_args_t &a, int tok, int slot, int kvh, int rank,
                               int split, int lane, AttnJob *job) {
-  const int pair = 2 * tok;
-  int below = 0;
-  bool broken = false;
-  for (int i0 = 0; i0 < a.n_seqs; i0 += 32) {
-    const int i = i0 + lane;
-    bool hit = false;
-    if (i < a.n_seqs) {
-      const int q0 = __ldg(a.q_start + i), q1 = __ldg(a.q_start + i + 1);
-      broken |= q0 < 0 || q1 < q0 || q1 > a.n_tokens;
-      hit = q0 / pair + i <= slot;
-    }
-    below += __popc(__ballot_sync(0xffffffffu, hit));
-  }
-  if (broken) set_status(a.status, kStatusBadIndex);
-  const int seq = below - 1;
-  if (seq < 0) return false;
-  const int q0 = __ldg(a.q_start + seq), q1 = __ldg(a.q_start + seq + 1);
-  if (q0 < 0 || q1 < q0 || q1 > a.n_tokens) return false;
-  const long long t0 = static_cast<long long>(slot - (q0 / pair + seq)) * pair;
-  const int len_q = q1 - q0;
-  if (t0 < 0 || t0 >= len_q) return false;
-  const long long start = __ldg(a.kv_start + seq);
-  const int len = __ldg(a.kv_len + seq);
-  if (len < 0 || start < 0 || start > a.n_kv_rows - len) {
-    set_status(a.status, kStatusBadIndex);
-    return false;
-  }
+  AttnRows r;
+  if (!attn_find_rows(a, 2 * tok, slot, lane, &r)) return false;
   if (lane != 0) return true;
-  const int n_tok = static_cast<int>(min(static_cast<long long>(pair), len_q - t0));
-  const long long pos = static_cast<long long>(len) - len_q + t0;  // of the pair's first token
-  const long long lo = a.window > 0 ? max(0ll, pos - a.window + 1) : 0;
-  const long long hi = max(lo, pos + n_tok);  // one past the last key that the pair sees
-  const int units = static_cast<int>((hi - lo + kKeys - 1) / kKeys);
+  const int units = (r.keys + kKeys - 1) / kKeys;
   job->kvh = kvh;
-  job->q_row0 = q0 + static_cast<int>(t0);
-  job->kv_row0 = static_cast<int>(start + lo);
-  job->first_pos = static_cast<int>(pos - lo);
-  job->keys = static_cast<int>(hi - lo);
+  job->q_row0 = r.q_row0;
+  job->kv_row0 = static_cast<int>(r.kv_row0);
+  job->first_pos = r.first_pos;
+  job->keys = r.keys;
   job->unit0 = static_cast<int>(static_cast<long long>(units) * rank / split);
   job->unit1 = static_cast<int>(static_cast<long long>(units) * (rank + 1) / split);
   for (int x = 0; x < 2; x++) {
-    const int n = min(max(n_tok - x * tok, 0), tok);
+    const int n = min(max(r.tokens - x * tok, 0), tok);
     job->tokens[x] = n;
     job->begin[x] = job->end[x] = job->unit0;
     if (n == 0) continue;
-    const long long p = pos + x * tok;  // the tile's first token
-    const long long from = a.window > 0 ? max(0ll, p - a.window + 1) - lo : 0;
-    const long long to = p + n - lo;    // may be <= 0
+    // relative to unit 0's first key: the tile's first token, the first key it sees
+    const long long p = static_cast<long long>(r.first_pos) + x * tok;
+    const long long from = a.window > 0 ? max(0ll, p - a.window + 1) : 0;
+    const long long to = p + n;  // may be <= 0
     const int b = static_cast<int>(from / kKeys);
     const int e = to > 0 ? static_cast<int>((to + kKeys - 1) / kKeys) : 0;
     job->begin[x] = max(b, job->unit0);
@@ -644,7 +573,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
     const uint32_t col_s = tmem + lanes + x * 128 + half * 64;
     const uint32_t col_p = tmem + lanes + S::kColP + x * S::kStrideP + half * 32;
     const uint32_t col_o = tmem + lanes + S::kColO + x * S::kStrideO + half * (D / 2);
-    const float c = a.scale * 1.4426950408889634f;
+    const float c = a.scale * kLog2e;
     uint32_t s_phase = 0, o_phase = 0, parity = 0;
     // Hands over a value of the thread's row and returns that of the thread with the row's other
     // keys.  The barrier has no limit of its own: a warp that gives up raises the abort flag,
@@ -959,6 +888,13 @@ static int attention_launch(const gptoss_attention_args_t &a, int sms, cudaStrea
   return launch_result("prompt_attention", e);
 }
 
+// Few query rows per sequence go to the kernel of token_attention.cu: when a sequence has on
+// average at most the tokens that fill 16 rows.
+static bool rows_are_few(const gptoss_attention_args_t &a) {
+  const int group = a.n_q_heads / a.n_kv_heads;
+  return group <= 16 && a.n_tokens <= static_cast<long long>(a.n_seqs) * (16 / group);
+}
+
 template <typename T>
 static int attention_for(const gptoss_attention_args_t &a, int sms, cudaStream_t st) {
   if (a.head_dim == 32) return attention_launch<T, 32>(a, sms, st);
@@ -1005,6 +941,7 @@ extern "C" int gptoss_decode_prompt_attention(const gptoss_attention_args_t *arg
   if (dev.code) return dev.code;
   const int sms = sm_count(dev.device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rows_are_few(a)) return launch_token_attention(a, sms, st);
   return a.dtype == GPTOSS_DTYPE_BF16 ? attention_for<bf16>(a, sms, st)
                                       : attention_for<__half>(a, sms, st);
 }
