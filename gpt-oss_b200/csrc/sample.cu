@@ -2,47 +2,125 @@
 // gptoss_decode_sample in include/gptoss_decode_b200.h.
 //
 // The kept set is a prefix of the order (logit descending, id ascending), so it is one
-// threshold: all logits above a value and the first few ids among those equal to it.  The
-// thresholds of top-k (a count) and top-p (a weight) are found digit by digit on the logits'
-// ordered bit patterns; nothing is sorted.  Weights are integers (multiples of 2^-44), so
-// every sum is exact whatever its order, and a draw is the same for any split of the row.
+// threshold: all logits above a value and the first few ids among those equal to it.  Nothing
+// is sorted.  Weights are integers (multiples of 2^-44), so every sum is exact whatever its
+// order, and a draw is the same for any split of the row.
 //
-// One CTA per row.
+// A cluster of up to 8 CTAs holds a row in its shared memory: the logits are read from HBM
+// once, and what follows runs on chip:
+//   1. load, maximum (joined over the cluster)
+//   2. where top-k or top-p is set: counts and weights of kBins bins of equal width below the
+//      maximum, summed over the cluster; the bin in which top-k ends, then (with the weight of
+//      what top-k kept) the bin in which top-p ends.  The few logits of such a bin go to a list
+//      that every CTA ranks for itself; a bin with more than kList logits (many equal ones, or
+//      a temperature that is high for their spread) is searched by the digits of their bits
+//   3. running sums in the order of the ids: threads own consecutive ids, block and cluster
+//      prefix; the thread in whose run the drawn value falls walks its run again
+// What bounds it: for large batches the read from HBM (two CTAs per SM, so that one loads while
+// the other computes) and the weights' fp64 arithmetic, about ten operations each; for a few
+// rows the cluster barriers between the steps.
+//
+// A weight has to be good to about 2^-44 relative, not to fp32's 2^-24: with 200000 kept tokens
+// a draw lies within 2^-24 of some running sum every few rows, and would then pick the wrong one.
 #include <cuda_fp16.h>
 #include <math.h>
+
+#include <algorithm>
 
 #include "common.cuh"
 #include "decode_ops.h"
 #include "engine.h"
+#include "umma_2sm.cuh"
 
 namespace gptoss {
 
 typedef unsigned long long u64;
 
-constexpr int kSampleThreads = 1024;
-constexpr uint32_t kKeyNegInf = 0x007fffffu;  // sample_key(-infinity)
-constexpr uint32_t kKeyPosInf = 0xff800000u;  // sample_key(+infinity)
+constexpr int kSampleThreads = 512;
+constexpr int kSampleWarps = kSampleThreads / 32;
+constexpr int kSampleMaxSplit = 8;     // CTAs of a row
+constexpr int kSampleMaxVocab = 1 << 18;
+constexpr int kBins = 512;
+constexpr int kList = 1024;
+constexpr unsigned kAll = 0xffffffffu;        // no limit among equal logits
+constexpr u64 kOne = 1ull << 44;              // weight of the likeliest token
 
-// Order-preserving bits of a logit: NaN as -infinity, -0 as +0.
+// Order-preserving bits of a logit (never NaN or -0 here).
 __device__ __forceinline__ uint32_t sample_key(float x) {
-  if (!(x == x)) return kKeyNegInf;
-  const uint32_t b = __float_as_uint(x + 0.0f);
+  const uint32_t b = __float_as_uint(x);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
+// NaN counts as -infinity, -0 as +0
+__device__ __forceinline__ float clean(float x) { return x == x ? x + 0.0f : -INFINITY; }
 __device__ __forceinline__ float logit_at(const float *p) { return *p; }
 __device__ __forceinline__ float logit_at(const bf16 *p) { return __bfloat162float(*p); }
 __device__ __forceinline__ float logit_at(const __half *p) { return __half2float(*p); }
 
-// exp((x - max) / T) in units of 2^-44.
-__device__ __forceinline__ u64 weight_of(uint32_t key, uint32_t max_key, double inv_t) {
-  if (key == max_key) return 1ull << 44;
-  if (max_key == kKeyPosInf || key == kKeyNegInf) return 0;
-  const double d = static_cast<double>(key_value(key)) - static_cast<double>(key_value(max_key));
-  return static_cast<u64>(exp(d * inv_t) * 17592186044416.0 + 0.5);
+struct SampleShared {
+  double table[128];               // 2^(-j / 128)
+  union {
+    u64 mass[kBins];               // weight of a bin in this CTA's part of the row
+    uint32_t list[kList];          // logits of one bin: the CTA's own, then the row's
+  };
+  unsigned count[kBins];
+  u64 warp_sum[kSampleWarps];
+  u64 best;                        // cluster reads: key and ~id of the CTA's largest logit
+  u64 sum;                         // cluster reads: the CTA's weight
+  unsigned listed;                 // cluster reads: length of the CTA's list
+  unsigned equal;                  // cluster reads: logits equal to the edge in the CTA
+  // results of a search, the same in all CTAs
+  uint32_t edge;
+  unsigned need, take, size, before;
+  u64 above;
+  int bin;
+};
+
+__device__ __forceinline__ uint32_t peer_addr(const void *p, int cta) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(p)), "r"(cta));
+  return remote;
 }
+__device__ __forceinline__ u64 peer_u64(const u64 *p, int cta) {
+  u64 v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(peer_addr(p, cta)) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned peer_u32(const unsigned *p, int cta) {
+  unsigned v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer_addr(p, cta)) : "memory");
+  return v;
+}
+
+// Weights: 2^(44 - y), y = (max - x) / (T ln 2), rounded to an integer.  y = k / 128 + r with
+// an integer k: 2^(-k/128) from a table and an exponent, 2^-r by its Taylor polynomial of
+// degree 4 (|r| <= 1/256: below 4e-14 relative).  All in fp64; the two additions of a power of
+// two round to integers and leave them in the low bits, which spares the slow conversions.
+struct Weigher {
+  double max, scale;      // scale = 128 / (T ln 2)
+  float top, cut;         // logits of at most `cut` weigh nothing
+  bool flat;              // the maximum is +infinity: those logits weigh 1, others nothing
+  const double *table;
+  __device__ __forceinline__ u64 operator()(float x) const {
+    if (x == top) return kOne;
+    if (flat || !(x > cut)) return 0;
+    const double y = (max - static_cast<double>(x)) * scale;
+    const double shifted = y + 6755399441055744.0;  // 1.5 * 2^52
+    const int k = __double2loint(shifted);
+    const double r = (y - (shifted - 6755399441055744.0)) * (-0.69314718055994530942 / 128);
+    double p = fma(r, 1.0 / 24, 1.0 / 6);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    p *= table[k & 127];
+    // 2^(44 - k / 128) by the exponent (k / 128 <= 46), then rounding to an integer
+    p = __hiloint2double(__double2hiint(p) + ((44 - (k >> 7)) << 20), __double2loint(p));
+    const double q = p + 4503599627370496.0;  // 2^52
+    return static_cast<u64>(__double_as_longlong(q)) & 0xfffffffffffffull;
+  }
+};
 
 // Sum over the block of v; every thread gets the exclusive prefix in *before.
 __device__ u64 block_scan(u64 v, u64 *before, u64 *scratch) {
@@ -56,7 +134,8 @@ __device__ u64 block_scan(u64 v, u64 *before, u64 *scratch) {
   if (lane == 31) scratch[warp] = inc;
   __syncthreads();
   u64 base = 0, total = 0;
-  for (int w = 0; w < kSampleThreads / 32; w++) {
+#pragma unroll
+  for (int w = 0; w < kSampleWarps; w++) {
     if (w == warp) base = total;
     total += scratch[w];
   }
@@ -65,148 +144,413 @@ __device__ u64 block_scan(u64 v, u64 *before, u64 *scratch) {
   return total;
 }
 
-struct SampleShared {
-  u64 mass[256];
-  unsigned count[256];
-  u64 scratch[kSampleThreads / 32];
-  u64 best;
-  uint32_t prefix;
-  u64 acc;
-  unsigned need;
-  int pick;
-};
-
 template <typename T>
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(const gptoss_sample_args_t a) {
+__global__ void __launch_bounds__(kSampleThreads)
+sample_kernel(const gptoss_sample_args_t a, int per, int split) {
+  extern __shared__ __align__(16) float slice_mem[];
   __shared__ SampleShared s;
-  const int row = blockIdx.x, tid = threadIdx.x;
-  if (a.pos && a.pos[row] < 0) {
-    if (tid == 0) a.next[row] = -1;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int rank = split > 1 ? static_cast<int>(cluster_cta_rank()) : 0;
+  const int row = blockIdx.x / split;
+  auto sync = [&]() {
+    if (split > 1)
+      cluster_barrier_all();
+    else
+      __syncthreads();
+  };
+  if (a.pos && a.pos[row] < 0) {  // the whole cluster alike
+    if (rank == 0 && tid == 0) a.next[row] = -1;
     return;
   }
-  const T *x = static_cast<const T *>(a.logits) + row * a.stride;
-  const int V = a.vocab;
-  // largest logit, lowest id among equals
-  if (tid == 0) s.best = 0;
-  __syncthreads();
-  u64 best = 0;
-  for (int i = tid; i < V; i += kSampleThreads) {
-    const u64 k = static_cast<u64>(sample_key(logit_at(x + i))) << 32 | (0xffffffffu - i);
-    best = max(best, k);
+  const int id0 = min(a.vocab, rank * per), n = min(a.vocab, id0 + per) - id0;
+  const T *x = static_cast<const T *>(a.logits) + row * a.stride + id0;
+  // ------------------------------------------------------------------ 1. load, maximum
+  // 16-byte loads from the first 16-byte boundary on; the slice starts so far into its buffer
+  // that those end up on 16-byte boundaries there too
+  constexpr int kVec = 16 / sizeof(T);
+  const int head = min(n, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / static_cast<int>(sizeof(T)));
+  float *slice = slice_mem + ((kVec - head) & 3);
+  float best = -INFINITY;
+  int best_id = 0x7fffffff;
+  auto keep = [&](int i, float v) {
+    slice[i] = v;
+    if (v > best) {  // a thread's ids ascend
+      best = v;
+      best_id = id0 + i;
+    }
+  };
+  if (tid < head) keep(tid, clean(logit_at(x + tid)));
+  const int vecs = (n - head) / kVec;
+  const uint4 *xv = reinterpret_cast<const uint4 *>(x + head);
+#pragma unroll 4
+  for (int v = tid; v < vecs; v += kSampleThreads) {
+    const uint4 raw = __ldcs(xv + v);
+    const T *e = reinterpret_cast<const T *>(&raw);
+    float f[kVec];
+#pragma unroll
+    for (int j = 0; j < kVec; j++) f[j] = clean(logit_at(e + j));
+    const int i = head + v * kVec;
+#pragma unroll
+    for (int j = 0; j < kVec; j += 4)
+      *reinterpret_cast<float4 *>(slice + i + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+#pragma unroll
+    for (int j = 0; j < kVec; j++)
+      if (f[j] > best) {
+        best = f[j];
+        best_id = id0 + i + j;
+      }
   }
-  atomicMax(&s.best, best);
-  __syncthreads();
-  const uint32_t max_key = static_cast<uint32_t>(s.best >> 32);
-  const int max_id = static_cast<int>(0xffffffffu - static_cast<uint32_t>(s.best));
+  for (int i = head + vecs * kVec + tid; i < n; i += kSampleThreads) keep(i, clean(logit_at(x + i)));
+  {
+    u64 key = best_id == 0x7fffffff ? 0 : static_cast<u64>(sample_key(best)) << 32 | (0xffffffffu - best_id);
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, i));
+    if (lane == 0) s.warp_sum[tid >> 5] = key;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < kSampleWarps; w++) key = max(key, s.warp_sum[w]);
+      s.best = key;
+    }
+  }
+  for (int i = tid; i < 128; i += kSampleThreads) s.table[i] = exp2(-i / 128.0);
+  for (int i = tid; i < kBins; i += kSampleThreads) s.mass[i] = s.count[i] = 0;
+  sync();
+  u64 key = 0;
+  for (int c = 0; c < split; c++) key = max(key, split > 1 ? peer_u64(&s.best, c) : s.best);
   const float temp = a.temperature ? a.temperature[row] : 1.0f;
-  if (!(temp > 0.0f) || max_key == kKeyNegInf) {
-    if (tid == 0) a.next[row] = max_key == kKeyNegInf ? 0 : max_id;
+  const bool greedy = !(temp > 0.0f);
+  if (greedy || key == 0) {
+    if (rank == 0 && tid == 0) a.next[row] = key == 0 ? 0 : static_cast<int>(0xffffffffu - static_cast<uint32_t>(key));
+    if (split > 1) cluster_barrier_all();  // the others may still read s.best
     return;
   }
-  const double inv_t = 1.0 / static_cast<double>(temp);
+  const float top = key_value(static_cast<uint32_t>(key >> 32));
+  Weigher weigh;
+  weigh.top = top;
+  weigh.flat = top == INFINITY;
+  weigh.max = static_cast<double>(top);
+  weigh.scale = 128 * 1.44269504088896340736 / static_cast<double>(temp);
+  // logits more than 46 T ln 2 below the maximum weigh less than 2^-45 (rounded down: some
+  // that weigh 0 are computed, none that weighs more is left out)
+  weigh.cut = static_cast<float>(fmax(weigh.max - 46 * 0.69314718055994530942 * static_cast<double>(temp), -3.5e38));
+  weigh.cut = weigh.cut > -3.3e38f ? nextafterf(weigh.cut, -INFINITY) : -INFINITY;
+  weigh.table = s.table;
   const int top_k = a.top_k ? a.top_k[row] : 0;
   const float top_p = a.top_p ? a.top_p[row] : 1.0f;
   const float min_p = a.min_p ? a.min_p[row] : 0.0f;
+  const bool by_count = top_k > 0 && top_k < a.vocab, by_mass = top_p < 1.0f;
   // kept: keys above `edge`, and the first `need` ids of those equal to it
   uint32_t edge = 0;
-  unsigned need = 0xffffffffu;
-  for (int mode = 0; mode < 2; mode++) {  // 0: top-k by count, 1: top-p by weight
-    if (mode == 0 && (top_k <= 0 || top_k >= V)) continue;
-    if (mode == 1 && !(top_p < 1.0f)) continue;
-    double limit = 0.0;
-    if (mode == 1) {
-      u64 mine = 0, eq = 0, before;
-      for (int i = tid; i < V; i += kSampleThreads) {
-        const uint32_t k = sample_key(logit_at(x + i));
-        if (k > edge) mine += weight_of(k, max_key, inv_t);
-        if (k == edge) eq++;
+  unsigned need = kAll;
+
+  if (by_count || by_mass) {
+    // ---------------------------------------------------------------- 2. thresholds
+    // bins of T / 16 below the maximum (of 1 / 16 above temperature 1, where the logits' own
+    // spread is what matters), the last one open; float arithmetic is monotonic, so bins
+    // respect the order.  -infinity takes no part.
+    const float to_bin = 16.0f * fmaxf(1.0f, static_cast<float>(1.0 / static_cast<double>(temp)));
+    auto bin_of = [&](float v) {
+      return v == top ? 0 : static_cast<int>(fminf((top - v) * to_bin, static_cast<float>(kBins - 1)));
+    };
+    for (int i = tid; i < n; i += kSampleThreads) {
+      const float v = slice[i];
+      if (v == -INFINITY) continue;
+      const int b = bin_of(v);
+      atomicAdd(&s.count[b], 1u);
+      if (by_mass) {
+        const u64 w = weigh(v);
+        if (w) atomicAdd(&s.mass[b], w);
       }
-      u64 total = block_scan(mine, &before, s.scratch);
-      eq = block_scan(eq, &before, s.scratch);
-      total += min(eq, static_cast<u64>(need)) * weight_of(edge, max_key, inv_t);
-      limit = fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(total);
     }
-    if (tid == 0) {
-      s.prefix = 0;
-      s.acc = 0;
-      s.need = top_k;
-    }
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kSampleThreads) s.mass[i] = s.count[i] = 0;
-      __syncthreads();
-      const uint32_t prefix = s.prefix;
-      for (int i = tid; i < V; i += kSampleThreads) {
-        const uint32_t k = sample_key(logit_at(x + i));
-        if (k < edge || (shift < 24 && (k >> (shift + 8)) != (prefix >> (shift + 8)))) continue;
-        atomicAdd(&s.count[(k >> shift) & 255], 1u);
-        if (mode == 1) atomicAdd(&s.mass[(k >> shift) & 255], weight_of(k, max_key, inv_t));
+    sync();
+    // the row's count and weight of digit or bin b
+    auto gather = [&](int b, unsigned *c, u64 *w) {
+      *c = 0;
+      *w = 0;
+      for (int k = 0; k < split; k++) {
+        *c += split > 1 ? peer_u32(&s.count[b], k) : s.count[b];
+        if (by_mass) *w += split > 1 ? peer_u64(&s.mass[b], k) : s.mass[b];
       }
-      __syncthreads();
+    };
+    static_assert(kBins == kSampleThreads, "a thread per bin in the scans");
+    unsigned my_count;
+    u64 my_mass, count_before, mass_before;
+    gather(tid, &my_count, &my_mass);
+    const u64 all_count = block_scan(my_count, &count_before, s.warp_sum);
+    u64 kept_mass = block_scan(my_mass, &mass_before, s.warp_sum);  // of what top-k keeps
+
+    // How many of the `equal` logits of weight w have less than `limit` in front of them, with
+    // `front` in front of the first.
+    auto take_of = [&](u64 front, u64 w, unsigned equal, double limit) {
+      if (w == 0) return equal;
+      const double q = (limit - static_cast<double>(front)) / static_cast<double>(w);
+      unsigned take = q < 1.0 ? 1u : static_cast<unsigned>(fmin(q, 262144.0));
+      while (static_cast<double>(front + take * w) < limit && take < equal) take++;
+      while (take > 1 && static_cast<double>(front + (take - 1) * w) >= limit) take--;
+      return min(take, equal);
+    };
+    // The edge within bin s.bin (of s.size logits): the `want`-th largest of the bin, or with
+    // limit >= 0 the last one that has less than `limit` in front of it, `acc` being the weight
+    // of the bins before.  Sets s.edge, s.take (how many equal to it stay), s.need (the same,
+    // kAll if all do) and s.above (weight of the bin's logits above the edge, where weights
+    // matter at all).
+    auto search = [&](unsigned want, u64 acc, double limit) {
+      const int bin = s.bin;
+      const unsigned size = s.size;
+      if (tid == 0) s.listed = 0;
+      sync();  // (the counts and weights of the bins have been read by everyone)
+      if (size <= kList) {
+        for (int i = tid; i < n; i += kSampleThreads) {
+          const float v = slice[i];
+          if (v != -INFINITY && bin_of(v) == bin) s.list[atomicAdd(&s.listed, 1u)] = sample_key(v);
+        }
+        sync();
+        constexpr int kPer = kList / kSampleThreads;
+        uint32_t got[kPer];
+        unsigned at = 0;
+        for (int j = 0; j < kPer; j++) got[j] = 0;
+        for (int k = 0; k < split; k++) {
+          const unsigned len = split > 1 ? peer_u32(&s.listed, k) : s.listed;
+          for (int j = 0; j < kPer; j++) {
+            const unsigned i = tid + j * kSampleThreads - at;
+            if (i < len) got[j] = split > 1 ? peer_u32(&s.list[i], k) : s.list[i];
+          }
+          at += len;
+        }
+        sync();
+        // bitonic sort, largest first (zeros, no logit's key, behind)
+        unsigned m = 32;
+        while (m < size) m <<= 1;
+        for (int j = 0; j < kPer; j++)
+          if (tid + j * kSampleThreads < m) s.list[tid + j * kSampleThreads] = got[j];
+        __syncthreads();
+        for (unsigned len = 2; len <= m; len <<= 1)
+          for (unsigned gap = len >> 1; gap > 0; gap >>= 1) {
+            for (unsigned i = tid; i < m / 2; i += kSampleThreads) {
+              const unsigned lo = 2 * i - (i & (gap - 1)), hi = lo + gap;
+              const uint32_t x0 = s.list[lo], x1 = s.list[hi];
+              if ((x0 < x1) == ((lo & len) == 0)) {
+                s.list[lo] = x1;
+                s.list[hi] = x0;
+              }
+            }
+            __syncthreads();
+          }
+        // weights in that order: a thread has kPer neighbours
+        u64 w[kPer], sum = 0, front;
+        for (int j = 0; j < kPer; j++) {
+          const unsigned i = tid * kPer + j;
+          w[j] = by_mass && i < size ? weigh(key_value(s.list[i])) : 0;
+          sum += w[j];
+        }
+        block_scan(sum, &front, s.warp_sum);
+        unsigned stay = want;  // length of the prefix that stays
+        if (limit >= 0.0) {
+          stay = 0;
+          u64 f = acc + front;
+          for (int j = 0; j < kPer; j++) {
+            stay += __syncthreads_count(tid * kPer + j < size && static_cast<double>(f) < limit);
+            f += w[j];
+          }
+        }
+        const uint32_t key = s.list[stay - 1];
+        unsigned above = 0, equal = 0;
+        for (int j = 0; j < kPer; j++) {
+          const unsigned i = tid * kPer + j;
+          above += __syncthreads_count(i < size && s.list[i] > key);
+          equal += __syncthreads_count(i < size && s.list[i] == key);
+        }
+        for (int j = 0; j < kPer; j++) {
+          if (tid * kPer + j == above) s.above = front;
+          front += w[j];
+        }
+        if (tid == 0) {
+          s.edge = key;
+          s.take = stay - above;
+          s.need = s.take < equal ? s.take : kAll;
+        }
+        __syncthreads();
+        return;
+      }
+      // many logits in the bin: by the digits of their bits
+      uint32_t prefix = 0;
+      u64 heavy = 0;
+      for (int shift = 24; shift >= 0; shift -= 8) {
+        sync();  // everyone has read the digits of the round before
+        if (tid < 256) s.mass[tid] = s.count[tid] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += kSampleThreads) {
+          const float v = slice[i];
+          if (v == -INFINITY || bin_of(v) != bin) continue;
+          const uint32_t k = sample_key(v);
+          if (shift < 24 && (k >> (shift + 8)) != (prefix >> (shift + 8))) continue;
+          atomicAdd(&s.count[(k >> shift) & 255], 1u);
+          if (by_mass) {
+            const u64 w = weigh(v);
+            if (w) atomicAdd(&s.mass[(k >> shift) & 255], w);
+          }
+        }
+        sync();
+        unsigned c = 0;
+        u64 w = 0, c_before, w_before;
+        const int digit = 255 - tid;  // largest digit first
+        if (tid < 256) gather(digit, &c, &w);
+        const u64 c_all = block_scan(c, &c_before, s.warp_sum);
+        block_scan(w, &w_before, s.warp_sum);
+        bool here = c > 0;
+        if (limit < 0.0) {
+          here = here && c_before < want && want <= c_before + c;
+        } else {
+          const double front = static_cast<double>(acc + heavy + w_before);
+          here = here && front < limit &&
+                 (static_cast<double>(acc + heavy + w_before + w) >= limit || c_before + c == c_all);
+        }
+        if (here) {
+          s.edge = prefix | static_cast<uint32_t>(digit) << shift;
+          s.before = static_cast<unsigned>(c_before);
+          s.above = w_before;
+          s.need = c;
+        }
+        __syncthreads();
+        prefix = s.edge;
+        want -= s.before;
+        heavy += s.above;
+        __syncthreads();
+      }
       if (tid == 0) {
-        int last = 0;
-        for (int b = 255; b >= 0; b--) {
-          if (!s.count[b]) continue;
-          last = b;
-          if (mode == 0) {
-            if (s.need <= s.count[b]) break;
-            s.need -= s.count[b];
-          } else {
-            if (static_cast<double>(s.acc + s.mass[b]) >= limit) break;
-            s.acc += s.mass[b];
-          }
-        }
-        s.prefix |= static_cast<uint32_t>(last) << shift;
-        if (mode == 1 && shift == 0) {
-          const u64 w = weight_of(s.prefix, max_key, inv_t);
-          unsigned n = 1;
-          if (w > 0) {
-            const double q = (limit - static_cast<double>(s.acc)) / static_cast<double>(w);
-            n = q < 1.0 ? 1u : static_cast<unsigned>(fmin(q, 262144.0));
-            while (static_cast<double>(s.acc + n * w) < limit) n++;
-            while (n > 1 && static_cast<double>(s.acc + (n - 1) * w) >= limit) n--;
-          }
-          s.need = min(n, s.prefix == edge ? need : s.count[last]);
-        }
+        const unsigned equal = s.need;
+        const unsigned take = limit < 0.0 ? want : take_of(acc + heavy, weigh(key_value(prefix)), equal, limit);
+        s.take = take;
+        s.need = take < equal ? take : kAll;
+        s.above = heavy;
       }
       __syncthreads();
+    };
+
+    if (by_count && static_cast<u64>(top_k) < all_count) {
+      const u64 want = top_k;
+      if (count_before < want && want <= count_before + my_count) {
+        s.bin = tid;
+        s.size = my_count;
+        s.before = static_cast<unsigned>(count_before);
+        s.sum = mass_before;
+      }
+      __syncthreads();
+      const u64 acc = s.sum;
+      search(static_cast<unsigned>(want - s.before), 0, -1.0);
+      edge = s.edge;
+      need = s.need;
+      kept_mass = acc + s.above + s.take * weigh(key_value(edge));
     }
-    edge = s.prefix;
-    need = s.need;
-    __syncthreads();
-  }
-  // running sums in the order of the ids: a thread owns a run of consecutive ids
-  const int per = (V + kSampleThreads - 1) / kSampleThreads;
-  const int i0 = min(V, tid * per), i1 = min(V, i0 + per);
-  const double least = min_p > 0.0f ? fmin(static_cast<double>(min_p), 1.0) * 17592186044416.0 : 0.0;
-  u64 eq = 0, eq_before, mass = 0, before;
-  for (int i = i0; i < i1; i++) eq += sample_key(logit_at(x + i)) == edge;
-  block_scan(eq, &eq_before, s.scratch);
-  for (int pass = 0; pass < 2; pass++) {
-    u64 total = 0, target = 0;
-    if (pass == 1) {
-      total = block_scan(mass, &before, s.scratch);
-      const float u0 = a.u[row];
-      const float u = u0 > 0.0f ? fminf(u0, 0.99999994f) : 0.0f;
-      target = static_cast<u64>(static_cast<double>(u) * static_cast<double>(total));
-      if (!(before <= target && target < before + mass)) return;
-    }
-    u64 run = before, rank = eq_before;
-    for (int i = i0; i < i1; i++) {
-      const uint32_t k = sample_key(logit_at(x + i));
-      if (k < edge || (k == edge && rank++ >= need)) continue;
-      const u64 w = weight_of(k, max_key, inv_t);
-      if (static_cast<double>(w) < least) continue;
-      if (pass == 0) {
-        mass += w;
-      } else {
-        run += w;
-        if (run > target) {
-          a.next[row] = i;
-          return;
+    if (by_mass) {
+      const double limit = fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(kept_mass);
+      if (limit > 0.0) {
+        // the bin in which the weight reaches the limit
+        if (static_cast<double>(mass_before) < limit && static_cast<double>(mass_before + my_mass) >= limit) {
+          s.bin = tid;
+          s.size = my_count;
+          s.sum = mass_before;
         }
+        __syncthreads();
+        const u64 acc = s.sum;
+        search(0, acc, limit);
+        if (s.edge > edge) {
+          edge = s.edge;
+          need = s.need;
+        } else if (s.edge == edge) {
+          need = min(need, s.need);
+        }
+      } else {  // the first token only
+        edge = static_cast<uint32_t>(key >> 32);
+        need = 1;
       }
     }
   }
+  // -------------------------------------------------------------------- 3. the draw
+  const u64 least = min_p > 0.0f ? static_cast<u64>(ceil(fmin(static_cast<double>(min_p), 1.0) *
+                                                         static_cast<double>(kOne)))
+                                 : 0;
+  const float edge_value = edge == 0 ? -INFINITY : key_value(edge);
+  const int run = ((n + kSampleThreads - 1) / kSampleThreads) | 1;  // odd: no bank conflicts
+  const int i0 = min(n, tid * run), i1 = min(n, i0 + run);
+  u64 eq_before = 0;
+  if (need != kAll) {  // ids equal to the edge in front of the thread's
+    u64 eq = 0;
+    for (int i = i0; i < i1; i++) eq += slice[i] == edge_value;
+    const u64 all = block_scan(eq, &eq_before, s.warp_sum);
+    if (split > 1) {
+      if (tid == 0) s.equal = static_cast<unsigned>(all);
+      sync();
+      for (int c = 0; c < rank; c++) eq_before += peer_u32(&s.equal, c);
+    }
+  }
+  auto weight_at = [&](int i, u64 *rank_of) -> u64 {
+    const float v = slice[i];
+    if (v < edge_value) return 0;
+    if (need != kAll && v == edge_value && (*rank_of)++ >= need) return 0;
+    const u64 w = weigh(v);
+    return w < least ? 0 : w;
+  };
+  u64 mass = 0, before, r = eq_before;
+  for (int i = i0; i < i1; i++) mass += weight_at(i, &r);
+  const u64 own = block_scan(mass, &before, s.warp_sum);
+  u64 total = own;
+  if (split > 1) {
+    if (tid == 0) s.sum = own;
+    sync();
+    total = 0;
+    for (int c = 0; c < split; c++) {
+      const u64 v = peer_u64(&s.sum, c);
+      if (c < rank) before += v;
+      total += v;
+    }
+  }
+  const float u0 = a.u[row];
+  const float u = u0 > 0.0f ? fminf(u0, 0.99999994f) : 0.0f;
+  const u64 target = static_cast<u64>(static_cast<double>(u) * static_cast<double>(total));
+  if (before <= target && target < before + mass) {
+    u64 sum = before;
+    r = eq_before;
+    for (int i = i0; i < i1; i++) {
+      sum += weight_at(i, &r);
+      if (sum > target) {
+        a.next[row] = id0 + i;
+        break;
+      }
+    }
+  }
+  if (split > 1) cluster_barrier_all();  // nobody leaves while its shared memory is read
+}
+
+template <typename T>
+static int sample_launch(const gptoss_sample_args_t &a, int sms, cudaStream_t st) {
+  // CTAs per row: as few as let two CTAs share an SM, more while that leaves SMs without work
+  int split = 1;
+  auto per_cta = [&](int c) { return ((a.vocab + c - 1) / c + 7) & ~7; };
+  while (split < kSampleMaxSplit && per_cta(split) > 25600) split *= 2;
+  while (split < kSampleMaxSplit && static_cast<long long>(a.n_rows) * split * 2 <= sms && per_cta(split) > 4096)
+    split *= 2;
+  const int per = per_cta(split);
+  const size_t smem = (static_cast<size_t>(per) + 4) * sizeof(float);
+  const long long grid = static_cast<long long>(a.n_rows) * split;
+  if (grid > INT32_MAX) return decode_error(GPTOSS_E_CAPACITY, "sample: too many rows for one launch");
+  auto kernel = sample_kernel<T>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e == cudaSuccess) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(kSampleThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = split;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = split > 1 ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, kernel, a, per, split);
+  }
+  return launch_result("sample", e);
 }
 
 }  // namespace gptoss
@@ -219,7 +563,7 @@ extern "C" int gptoss_decode_sample(const gptoss_sample_args_t *args, void *stre
   if (a.n_rows < 0 || a.vocab <= 0) return decode_error(GPTOSS_E_INVALID, "sample: negative number of rows or no vocabulary");
   if (a.dtype < GPTOSS_DTYPE_BF16 || a.dtype > GPTOSS_DTYPE_FP32)
     return decode_error(GPTOSS_E_INVALID, "sample: unknown dtype %d", a.dtype);
-  if (a.vocab > (1 << 18))
+  if (a.vocab > kSampleMaxVocab)
     return decode_error(GPTOSS_E_CAPACITY, "sample: vocabulary %d is above 262144", a.vocab);
   if (a.stride < a.vocab) return decode_error(GPTOSS_E_INVALID, "sample: the row stride is shorter than the vocabulary");
   if (a.n_rows == 0) return GPTOSS_OK;
@@ -228,12 +572,9 @@ extern "C" int gptoss_decode_sample(const gptoss_sample_args_t *args, void *stre
     return decode_error(GPTOSS_E_INVALID, "sample: logits are not a multiple of their element size");
   OnDeviceOf dev(a.next, "sample: next");
   if (dev.code) return dev.code;
+  const int sms = sm_count(dev.device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a.dtype == GPTOSS_DTYPE_FP32)
-    sample_kernel<float><<<a.n_rows, kSampleThreads, 0, st>>>(a);
-  else if (a.dtype == GPTOSS_DTYPE_BF16)
-    sample_kernel<bf16><<<a.n_rows, kSampleThreads, 0, st>>>(a);
-  else
-    sample_kernel<__half><<<a.n_rows, kSampleThreads, 0, st>>>(a);
-  return launch_result("sample");
+  if (a.dtype == GPTOSS_DTYPE_FP32) return sample_launch<float>(a, sms, st);
+  if (a.dtype == GPTOSS_DTYPE_BF16) return sample_launch<bf16>(a, sms, st);
+  return sample_launch<__half>(a, sms, st);
 }
