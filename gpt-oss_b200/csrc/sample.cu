@@ -23,6 +23,7 @@
 // A weight has to be good to about 2^-44 relative, not to fp32's 2^-24: with 200000 kept tokens
 // a draw lies within 2^-24 of some running sum every few rows, and would then pick the wrong one.
 #include <cuda_fp16.h>
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -73,7 +74,7 @@ struct SampleShared {
   unsigned equal;                  // cluster reads: logits equal to the edge in the CTA
   // results of a search, the same in all CTAs
   uint32_t edge;
-  unsigned need, take, size, before;
+  unsigned need, take, equals, size, before;
   u64 above;
   int bin;
 };
@@ -101,24 +102,43 @@ __device__ __forceinline__ unsigned peer_u32(const unsigned *p, int cta) {
 struct Weigher {
   double max, scale;      // scale = 128 / (T ln 2)
   float top, cut;         // logits of at most `cut` weigh nothing
+  float floor;            // what those are taken for, so that the arithmetic stays in range
   bool flat;              // the maximum is +infinity: those logits weigh 1, others nothing
   const double *table;
+  // N at a time: a weight is a chain of ten dependent fp64 operations
+  template <int N>
+  __device__ __forceinline__ void weigh(const float (&x)[N], u64 (&w)[N]) const {
+    double y[N], p[N], r[N];
+    int k[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      y[i] = (max - static_cast<double>(fmaxf(x[i], floor))) * scale;
+      const double shifted = y[i] + 6755399441055744.0;  // 1.5 * 2^52
+      k[i] = __double2loint(shifted);
+      r[i] = (y[i] - (shifted - 6755399441055744.0)) * (-0.69314718055994530942 / 128);
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) p[i] = fma(r[i], 1.0 / 24, 1.0 / 6);
+#pragma unroll
+    for (int i = 0; i < N; i++) p[i] = fma(p[i], r[i], 0.5);
+#pragma unroll
+    for (int i = 0; i < N; i++) p[i] = fma(p[i], r[i], 1.0);
+#pragma unroll
+    for (int i = 0; i < N; i++) p[i] = fma(p[i], r[i], 1.0) * table[k[i] & 127];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      // 2^(44 - k / 128) by the exponent (k / 128 <= 46), then rounding to an integer
+      const double q = __hiloint2double(__double2hiint(p[i]) + ((44 - (k[i] >> 7)) << 20), __double2loint(p[i])) +
+                       4503599627370496.0;  // 2^52
+      const u64 bits = static_cast<u64>(__double_as_longlong(q)) & 0xfffffffffffffull;
+      w[i] = x[i] == top ? kOne : (!flat && x[i] > cut ? bits : 0);
+    }
+  }
   __device__ __forceinline__ u64 operator()(float x) const {
-    if (x == top) return kOne;
-    if (flat || !(x > cut)) return 0;
-    const double y = (max - static_cast<double>(x)) * scale;
-    const double shifted = y + 6755399441055744.0;  // 1.5 * 2^52
-    const int k = __double2loint(shifted);
-    const double r = (y - (shifted - 6755399441055744.0)) * (-0.69314718055994530942 / 128);
-    double p = fma(r, 1.0 / 24, 1.0 / 6);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    p *= table[k & 127];
-    // 2^(44 - k / 128) by the exponent (k / 128 <= 46), then rounding to an integer
-    p = __hiloint2double(__double2hiint(p) + ((44 - (k >> 7)) << 20), __double2loint(p));
-    const double q = p + 4503599627370496.0;  // 2^52
-    return static_cast<u64>(__double_as_longlong(q)) & 0xfffffffffffffull;
+    const float in[1] = {x};
+    u64 w[1];
+    weigh(in, w);
+    return w[0];
   }
 };
 
@@ -144,9 +164,10 @@ __device__ u64 block_scan(u64 v, u64 *before, u64 *scratch) {
   return total;
 }
 
-template <typename T>
+// split: CTAs of a row
+template <typename T, int split>
 __global__ void __launch_bounds__(kSampleThreads)
-sample_kernel(const gptoss_sample_args_t a, int per, int split) {
+sample_kernel(const gptoss_sample_args_t a, int per) {
   extern __shared__ __align__(16) float slice_mem[];
   __shared__ SampleShared s;
   const int tid = threadIdx.x, lane = tid & 31;
@@ -216,6 +237,7 @@ sample_kernel(const gptoss_sample_args_t a, int per, int split) {
   for (int i = tid; i < kBins; i += kSampleThreads) s.mass[i] = s.count[i] = 0;
   sync();
   u64 key = 0;
+#pragma unroll
   for (int c = 0; c < split; c++) key = max(key, split > 1 ? peer_u64(&s.best, c) : s.best);
   const float temp = a.temperature ? a.temperature[row] : 1.0f;
   const bool greedy = !(temp > 0.0f);
@@ -225,16 +247,17 @@ sample_kernel(const gptoss_sample_args_t a, int per, int split) {
     return;
   }
   const float top = key_value(static_cast<uint32_t>(key >> 32));
-  Weigher weigh;
-  weigh.top = top;
-  weigh.flat = top == INFINITY;
-  weigh.max = static_cast<double>(top);
-  weigh.scale = 128 * 1.44269504088896340736 / static_cast<double>(temp);
+  Weigher weigher;
+  weigher.top = top;
+  weigher.flat = top == INFINITY;
+  weigher.max = static_cast<double>(top);
+  weigher.scale = 128 * 1.44269504088896340736 / static_cast<double>(temp);
   // logits more than 46 T ln 2 below the maximum weigh less than 2^-45 (rounded down: some
   // that weigh 0 are computed, none that weighs more is left out)
-  weigh.cut = static_cast<float>(fmax(weigh.max - 46 * 0.69314718055994530942 * static_cast<double>(temp), -3.5e38));
-  weigh.cut = weigh.cut > -3.3e38f ? nextafterf(weigh.cut, -INFINITY) : -INFINITY;
-  weigh.table = s.table;
+  weigher.cut = static_cast<float>(fmax(weigher.max - 46 * 0.69314718055994530942 * static_cast<double>(temp), -3.5e38));
+  weigher.cut = weigher.cut > -3.3e38f ? nextafterf(weigher.cut, -INFINITY) : -INFINITY;
+  weigher.floor = weigher.cut > -INFINITY ? weigher.cut : -FLT_MAX;
+  weigher.table = s.table;
   const int top_k = a.top_k ? a.top_k[row] : 0;
   const float top_p = a.top_p ? a.top_p[row] : 1.0f;
   const float min_p = a.min_p ? a.min_p[row] : 0.0f;
@@ -252,32 +275,56 @@ sample_kernel(const gptoss_sample_args_t a, int per, int split) {
     auto bin_of = [&](float v) {
       return v == top ? 0 : static_cast<int>(fminf((top - v) * to_bin, static_cast<float>(kBins - 1)));
     };
-    for (int i = tid; i < n; i += kSampleThreads) {
-      const float v = slice[i];
-      if (v == -INFINITY) continue;
-      const int b = bin_of(v);
-      atomicAdd(&s.count[b], 1u);
-      if (by_mass) {
-        const u64 w = weigh(v);
-        if (w) atomicAdd(&s.mass[b], w);
-      }
-    }
-    sync();
     // the row's count and weight of digit or bin b
-    auto gather = [&](int b, unsigned *c, u64 *w) {
+    auto gather = [&](int b, bool weights, unsigned *c, u64 *w) {
+      unsigned cs[split];
+      u64 ws[split];
+#pragma unroll
+      for (int k = 0; k < split; k++) {
+        cs[k] = split > 1 ? peer_u32(&s.count[b], k) : s.count[b];
+        ws[k] = 0;
+        if (weights) ws[k] = split > 1 ? peer_u64(&s.mass[b], k) : s.mass[b];
+      }
       *c = 0;
       *w = 0;
+#pragma unroll
       for (int k = 0; k < split; k++) {
-        *c += split > 1 ? peer_u32(&s.count[b], k) : s.count[b];
-        if (by_mass) *w += split > 1 ? peer_u64(&s.mass[b], k) : s.mass[b];
+        *c += cs[k];
+        *w += ws[k];
       }
     };
     static_assert(kBins == kSampleThreads, "a thread per bin in the scans");
     unsigned my_count;
-    u64 my_mass, count_before, mass_before;
-    gather(tid, &my_count, &my_mass);
-    const u64 all_count = block_scan(my_count, &count_before, s.warp_sum);
-    u64 kept_mass = block_scan(my_mass, &mass_before, s.warp_sum);  // of what top-k keeps
+    u64 my_mass, count_before, mass_before, all_count, all_mass;
+    // Counts (and weights) of the bins, of the logits from `least` on.
+    auto histogram = [&](bool weights, float least) {
+      for (int i0 = tid; i0 < n; i0 += 4 * kSampleThreads) {
+        float v[4];
+        bool in[4];
+        u64 w[4] = {0, 0, 0, 0};
+        bool some = false;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int i = i0 + j * kSampleThreads;
+          v[j] = i < n ? slice[i] : -INFINITY;
+          in[j] = v[j] > -INFINITY && v[j] >= least;
+          some |= in[j];
+        }
+        if (!some) continue;
+        if (weights) weigher.weigh(v, w);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (in[j]) {
+            const int b = bin_of(v[j]);
+            atomicAdd(&s.count[b], 1u);
+            if (w[j]) atomicAdd(&s.mass[b], w[j]);
+          }
+      }
+      sync();
+      gather(tid, weights, &my_count, &my_mass);
+      all_count = block_scan(my_count, &count_before, s.warp_sum);
+      all_mass = block_scan(my_mass, &mass_before, s.warp_sum);
+    };
 
     // How many of the `equal` logits of weight w have less than `limit` in front of them, with
     // `front` in front of the first.
@@ -291,31 +338,35 @@ sample_kernel(const gptoss_sample_args_t a, int per, int split) {
     };
     // The edge within bin s.bin (of s.size logits): the `want`-th largest of the bin, or with
     // limit >= 0 the last one that has less than `limit` in front of it, `acc` being the weight
-    // of the bins before.  Sets s.edge, s.take (how many equal to it stay), s.need (the same,
-    // kAll if all do) and s.above (weight of the bin's logits above the edge, where weights
-    // matter at all).
-    auto search = [&](unsigned want, u64 acc, double limit) {
+    // of the bins before.  Sets s.edge, s.equals (logits equal to it), s.take (how many of them
+    // stay) and s.need (the same, kAll if all do).
+    auto search = [&](bool weights, unsigned want, u64 acc, double limit) {
       const int bin = s.bin;
       const unsigned size = s.size;
+      const float floor_value = edge ? key_value(edge) : -INFINITY;
       if (tid == 0) s.listed = 0;
       sync();  // (the counts and weights of the bins have been read by everyone)
       if (size <= kList) {
         for (int i = tid; i < n; i += kSampleThreads) {
           const float v = slice[i];
-          if (v != -INFINITY && bin_of(v) == bin) s.list[atomicAdd(&s.listed, 1u)] = sample_key(v);
+          if (v > -INFINITY && v >= floor_value && bin_of(v) == bin) s.list[atomicAdd(&s.listed, 1u)] = sample_key(v);
         }
         sync();
         constexpr int kPer = kList / kSampleThreads;
         uint32_t got[kPer];
-        unsigned at = 0;
+        unsigned lens[split], at = 0;
+#pragma unroll
         for (int j = 0; j < kPer; j++) got[j] = 0;
+#pragma unroll
+        for (int k = 0; k < split; k++) lens[k] = split > 1 ? peer_u32(&s.listed, k) : s.listed;
+#pragma unroll
         for (int k = 0; k < split; k++) {
-          const unsigned len = split > 1 ? peer_u32(&s.listed, k) : s.listed;
+#pragma unroll
           for (int j = 0; j < kPer; j++) {
             const unsigned i = tid + j * kSampleThreads - at;
-            if (i < len) got[j] = split > 1 ? peer_u32(&s.list[i], k) : s.list[i];
+            if (i < lens[k]) got[j] = split > 1 ? peer_u32(&s.list[i], k) : s.list[i];
           }
-          at += len;
+          at += lens[k];
         }
         sync();
         // bitonic sort, largest first (zeros, no logit's key, behind)
@@ -340,7 +391,7 @@ sample_kernel(const gptoss_sample_args_t a, int per, int split) {
         u64 w[kPer], sum = 0, front;
         for (int j = 0; j < kPer; j++) {
           const unsigned i = tid * kPer + j;
-          w[j] = by_mass && i < size ? weigh(key_value(s.list[i])) : 0;
+          w[j] = weights && i < size ? weigher(key_value(s.list[i])) : 0;
           sum += w[j];
         }
         block_scan(sum, &front, s.warp_sum);
@@ -360,13 +411,10 @@ sample_kernel(const gptoss_sample_args_t a, int per, int split) {
           above += __syncthreads_count(i < size && s.list[i] > key);
           equal += __syncthreads_count(i < size && s.list[i] == key);
         }
-        for (int j = 0; j < kPer; j++) {
-          if (tid * kPer + j == above) s.above = front;
-          front += w[j];
-        }
         if (tid == 0) {
           s.edge = key;
           s.take = stay - above;
+          s.equals = equal;
           s.need = s.take < equal ? s.take : kAll;
         }
         __syncthreads();
@@ -381,12 +429,12 @@ sample_kernel(const gptoss_sample_args_t a, int per, int split) {
         __syncthreads();
         for (int i = tid; i < n; i += kSampleThreads) {
           const float v = slice[i];
-          if (v == -INFINITY || bin_of(v) != bin) continue;
+          if (v == -INFINITY || v < floor_value || bin_of(v) != bin) continue;
           const uint32_t k = sample_key(v);
           if (shift < 24 && (k >> (shift + 8)) != (prefix >> (shift + 8))) continue;
           atomicAdd(&s.count[(k >> shift) & 255], 1u);
-          if (by_mass) {
-            const u64 w = weigh(v);
+          if (weights) {
+            const u64 w = weigher(v);
             if (w) atomicAdd(&s.mass[(k >> shift) & 255], w);
           }
         }
@@ -394,7 +442,7 @@ sample_kernel(const gptoss_sample_args_t a, int per, int split) {
         unsigned c = 0;
         u64 w = 0, c_before, w_before;
         const int digit = 255 - tid;  // largest digit first
-        if (tid < 256) gather(digit, &c, &w);
+        if (tid < 256) gather(digit, weights, &c, &w);
         const u64 c_all = block_scan(c, &c_before, s.warp_sum);
         block_scan(w, &w_before, s.warp_sum);
         bool here = c > 0;
@@ -419,31 +467,39 @@ sample_kernel(const gptoss_sample_args_t a, int per, int split) {
       }
       if (tid == 0) {
         const unsigned equal = s.need;
-        const unsigned take = limit < 0.0 ? want : take_of(acc + heavy, weigh(key_value(prefix)), equal, limit);
+        const unsigned take = limit < 0.0 ? want : take_of(acc + heavy, weigher(key_value(prefix)), equal, limit);
         s.take = take;
+        s.equals = equal;
         s.need = take < equal ? take : kAll;
-        s.above = heavy;
       }
       __syncthreads();
     };
 
-    if (by_count && static_cast<u64>(top_k) < all_count) {
+    u64 dropped = 0;  // weight of the logits equal to the edge that top-k leaves out
+    if (by_count) {
+      histogram(false, -INFINITY);
       const u64 want = top_k;
-      if (count_before < want && want <= count_before + my_count) {
-        s.bin = tid;
-        s.size = my_count;
-        s.before = static_cast<unsigned>(count_before);
-        s.sum = mass_before;
+      if (want < all_count) {
+        if (count_before < want && want <= count_before + my_count) {
+          s.bin = tid;
+          s.size = my_count;
+          s.before = static_cast<unsigned>(count_before);
+        }
+        __syncthreads();
+        search(false, static_cast<unsigned>(want - s.before), 0, -1.0);
+        edge = s.edge;
+        need = s.need;
+        dropped = (s.equals - s.take) * weigher(key_value(edge));
       }
-      __syncthreads();
-      const u64 acc = s.sum;
-      search(static_cast<unsigned>(want - s.before), 0, -1.0);
-      edge = s.edge;
-      need = s.need;
-      kept_mass = acc + s.above + s.take * weigh(key_value(edge));
     }
     if (by_mass) {
-      const double limit = fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(kept_mass);
+      if (by_count) {  // what top-k left; the arrays are free once everyone has read them
+        sync();
+        s.mass[tid] = s.count[tid] = 0;
+        __syncthreads();
+      }
+      histogram(true, edge ? key_value(edge) : -INFINITY);
+      const double limit = fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(all_mass - dropped);
       if (limit > 0.0) {
         // the bin in which the weight reaches the limit
         if (static_cast<double>(mass_before) < limit && static_cast<double>(mass_before + my_mass) >= limit) {
@@ -453,7 +509,7 @@ sample_kernel(const gptoss_sample_args_t a, int per, int split) {
         }
         __syncthreads();
         const u64 acc = s.sum;
-        search(0, acc, limit);
+        search(true, 0, acc, limit);
         if (s.edge > edge) {
           edge = s.edge;
           need = s.need;
@@ -481,28 +537,51 @@ sample_kernel(const gptoss_sample_args_t a, int per, int split) {
     if (split > 1) {
       if (tid == 0) s.equal = static_cast<unsigned>(all);
       sync();
-      for (int c = 0; c < rank; c++) eq_before += peer_u32(&s.equal, c);
+#pragma unroll
+      for (int c = 0; c < split; c++) {
+        const unsigned v = peer_u32(&s.equal, c);
+        if (c < rank) eq_before += v;
+      }
     }
   }
-  auto weight_at = [&](int i, u64 *rank_of) -> u64 {
-    const float v = slice[i];
-    if (v < edge_value) return 0;
-    if (need != kAll && v == edge_value && (*rank_of)++ >= need) return 0;
-    const u64 w = weigh(v);
-    return w < least ? 0 : w;
+  // weights of four ids from i on, those beyond the thread's run 0; *rank_of counts the ids
+  // equal to the edge
+  auto weights_at = [&](int i, u64 (&w)[4], u64 *rank_of) {
+    float v[4];
+    bool some = false;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      v[j] = i + j < i1 ? slice[i + j] : -INFINITY;
+      if (v[j] < edge_value) v[j] = -INFINITY;
+      if (need != kAll && v[j] == edge_value && (*rank_of)++ >= need) v[j] = -INFINITY;
+      some |= v[j] > -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) w[j] = 0;
+    if (!some) return;
+    weigher.weigh(v, w);
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (w[j] < least) w[j] = 0;
   };
-  u64 mass = 0, before, r = eq_before;
-  for (int i = i0; i < i1; i++) mass += weight_at(i, &r);
+  u64 mass = 0, before, r = eq_before, w4[4];
+  for (int i = i0; i < i1; i += 4) {
+    weights_at(i, w4, &r);
+    mass += (w4[0] + w4[1]) + (w4[2] + w4[3]);
+  }
   const u64 own = block_scan(mass, &before, s.warp_sum);
   u64 total = own;
   if (split > 1) {
     if (tid == 0) s.sum = own;
     sync();
+    u64 sums[split];
+#pragma unroll
+    for (int c = 0; c < split; c++) sums[c] = peer_u64(&s.sum, c);
     total = 0;
+#pragma unroll
     for (int c = 0; c < split; c++) {
-      const u64 v = peer_u64(&s.sum, c);
-      if (c < rank) before += v;
-      total += v;
+      if (c < rank) before += sums[c];
+      total += sums[c];
     }
   }
   const float u0 = a.u[row];
@@ -510,14 +589,17 @@ sample_kernel(const gptoss_sample_args_t a, int per, int split) {
   const u64 target = static_cast<u64>(static_cast<double>(u) * static_cast<double>(total));
   if (before <= target && target < before + mass) {
     u64 sum = before;
+    int pick = -1;
     r = eq_before;
-    for (int i = i0; i < i1; i++) {
-      sum += weight_at(i, &r);
-      if (sum > target) {
-        a.next[row] = id0 + i;
-        break;
+    for (int i = i0; i < i1 && pick < 0; i += 4) {
+      weights_at(i, w4, &r);
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        sum += w4[j];
+        if (pick < 0 && sum > target) pick = i + j;
       }
     }
+    a.next[row] = id0 + pick;
   }
   if (split > 1) cluster_barrier_all();  // nobody leaves while its shared memory is read
 }
@@ -534,7 +616,9 @@ static int sample_launch(const gptoss_sample_args_t &a, int sms, cudaStream_t st
   const size_t smem = (static_cast<size_t>(per) + 4) * sizeof(float);
   const long long grid = static_cast<long long>(a.n_rows) * split;
   if (grid > INT32_MAX) return decode_error(GPTOSS_E_CAPACITY, "sample: too many rows for one launch");
-  auto kernel = sample_kernel<T>;
+  void (*kernel)(const gptoss_sample_args_t, int) =
+      split == 1 ? sample_kernel<T, 1>
+                 : (split == 2 ? sample_kernel<T, 2> : (split == 4 ? sample_kernel<T, 4> : sample_kernel<T, 8>));
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg = {};
@@ -548,7 +632,7 @@ static int sample_launch(const gptoss_sample_args_t &a, int sms, cudaStream_t st
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = split > 1 ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, kernel, a, per, split);
+    e = cudaLaunchKernelEx(&cfg, kernel, a, per);
   }
   return launch_result("sample", e);
 }
