@@ -61,16 +61,17 @@ __device__ __forceinline__ float logit_at(const bf16 *p) { return __bfloat162flo
 __device__ __forceinline__ float logit_at(const __half *p) { return __half2float(*p); }
 
 struct SampleShared {
-  double table[128];               // 2^(-j / 128)
+  double table[16];                // 2^(-j / 16)
   union {
-    u64 mass[kBins];               // weight of a bin in this CTA's part of the row
-    uint32_t list[kList];          // logits of one bin: the CTA's own, then the row's
+    u64 mass[kBins];               // cluster reads: weight of a bin in this CTA's part of the row
+    uint32_t merged[kList];        // the cluster's lists together, largest first
   };
-  unsigned count[kBins];
+  unsigned count[kBins];           // cluster reads: logits of a bin
+  uint32_t list[kList];            // cluster reads: keys that the CTA contributes to a list
   u64 warp_sum[kSampleWarps];
   u64 best;                        // cluster reads: key and ~id of the CTA's largest logit
   u64 sum;                         // cluster reads: the CTA's weight
-  unsigned listed;                 // cluster reads: length of the CTA's list
+  unsigned listed[3];              // cluster reads: lengths of the CTA's lists
   unsigned equal;                  // cluster reads: logits equal to the edge in the CTA
   // results of a search, the same in all CTAs
   uint32_t edge;
@@ -95,12 +96,14 @@ __device__ __forceinline__ unsigned peer_u32(const unsigned *p, int cta) {
   return v;
 }
 
-// Weights: 2^(44 - y), y = (max - x) / (T ln 2), rounded to an integer.  y = k / 128 + r with
-// an integer k: 2^(-k/128) from a table and an exponent, 2^-r by its Taylor polynomial of
-// degree 4 (|r| <= 1/256: below 4e-14 relative).  All in fp64; the two additions of a power of
+// Weights: 2^(44 - y), y = (max - x) / (T ln 2), rounded to an integer.  y = k / 16 + r with
+// an integer k: 2^(-k/16) from a table and an exponent, 2^-r by its Taylor polynomial of
+// degree 6 (|r| <= 1/32: below 1e-15 relative).  All in fp64; the two additions of a power of
 // two round to integers and leave them in the low bits, which spares the slow conversions.
+// (Per SM and cycle: 64 fp64 operations, 16 conversions of fp32 to fp64, and 15.6 lookups in a
+// table of 16 doubles, which lie in different banks; of 128 only 6.9.)
 struct Weigher {
-  double max, scale;      // scale = 128 / (T ln 2)
+  double max, scale;      // scale = 16 / (T ln 2)
   float top, cut;         // logits of at most `cut` weigh nothing
   float floor;            // what those are taken for, so that the arithmetic stays in range
   bool flat;              // the maximum is +infinity: those logits weigh 1, others nothing
@@ -115,20 +118,24 @@ struct Weigher {
       y[i] = (max - static_cast<double>(fmaxf(x[i], floor))) * scale;
       const double shifted = y[i] + 6755399441055744.0;  // 1.5 * 2^52
       k[i] = __double2loint(shifted);
-      r[i] = (y[i] - (shifted - 6755399441055744.0)) * (-0.69314718055994530942 / 128);
+      r[i] = (y[i] - (shifted - 6755399441055744.0)) * (-0.69314718055994530942 / 16);
     }
 #pragma unroll
-    for (int i = 0; i < N; i++) p[i] = fma(r[i], 1.0 / 24, 1.0 / 6);
+    for (int i = 0; i < N; i++) p[i] = fma(r[i], 1.0 / 720, 1.0 / 120);
+#pragma unroll
+    for (int i = 0; i < N; i++) p[i] = fma(p[i], r[i], 1.0 / 24);
+#pragma unroll
+    for (int i = 0; i < N; i++) p[i] = fma(p[i], r[i], 1.0 / 6);
 #pragma unroll
     for (int i = 0; i < N; i++) p[i] = fma(p[i], r[i], 0.5);
 #pragma unroll
     for (int i = 0; i < N; i++) p[i] = fma(p[i], r[i], 1.0);
 #pragma unroll
-    for (int i = 0; i < N; i++) p[i] = fma(p[i], r[i], 1.0) * table[k[i] & 127];
+    for (int i = 0; i < N; i++) p[i] = fma(p[i], r[i], 1.0) * table[k[i] & 15];
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      // 2^(44 - k / 128) by the exponent (k / 128 <= 46), then rounding to an integer
-      const double q = __hiloint2double(__double2hiint(p[i]) + ((44 - (k[i] >> 7)) << 20), __double2loint(p[i])) +
+      // 2^(44 - k / 16) by the exponent (k / 16 <= 46), then rounding to an integer
+      const double q = __hiloint2double(__double2hiint(p[i]) + ((44 - (k[i] >> 4)) << 20), __double2loint(p[i])) +
                        4503599627370496.0;  // 2^52
       const u64 bits = static_cast<u64>(__double_as_longlong(q)) & 0xfffffffffffffull;
       w[i] = x[i] == top ? kOne : (!flat && x[i] > cut ? bits : 0);
@@ -233,7 +240,8 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
       s.best = key;
     }
   }
-  for (int i = tid; i < 128; i += kSampleThreads) s.table[i] = exp2(-i / 128.0);
+  if (tid < 16) s.table[tid] = exp2(-tid / 16.0);
+  if (tid < 3) s.listed[tid] = 0;
   for (int i = tid; i < kBins; i += kSampleThreads) s.mass[i] = s.count[i] = 0;
   sync();
   u64 key = 0;
@@ -251,7 +259,7 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
   weigher.top = top;
   weigher.flat = top == INFINITY;
   weigher.max = static_cast<double>(top);
-  weigher.scale = 128 * 1.44269504088896340736 / static_cast<double>(temp);
+  weigher.scale = 16 * 1.44269504088896340736 / static_cast<double>(temp);
   // logits more than 46 T ln 2 below the maximum weigh less than 2^-45 (rounded down: some
   // that weigh 0 are computed, none that weighs more is left out)
   weigher.cut = static_cast<float>(fmax(weigher.max - 46 * 0.69314718055994530942 * static_cast<double>(temp), -3.5e38));
@@ -274,6 +282,16 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
     const float to_bin = 16.0f * fmaxf(1.0f, static_cast<float>(1.0 / static_cast<double>(temp)));
     auto bin_of = [&](float v) {
       return v == top ? 0 : static_cast<int>(fminf((top - v) * to_bin, static_cast<float>(kBins - 1)));
+    };
+    // 64-bit sums in shared memory as two 32-bit ones with a carry (6.3 a cycle and SM; the
+    // 64-bit atomic manages 1.1)
+    auto add_mass = [&](int b, u64 w) {
+      if (w == 0) return;
+      unsigned *word = reinterpret_cast<unsigned *>(&s.mass[b]);
+      const unsigned lo = static_cast<unsigned>(w);
+      const unsigned carry = atomicAdd(word, lo) + lo < lo;
+      const unsigned hi = static_cast<unsigned>(w >> 32) + carry;
+      if (hi) atomicAdd(word + 1, hi);
     };
     // the row's count and weight of digit or bin b
     auto gather = [&](int b, bool weights, unsigned *c, u64 *w) {
@@ -317,7 +335,7 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
           if (in[j]) {
             const int b = bin_of(v[j]);
             atomicAdd(&s.count[b], 1u);
-            if (w[j]) atomicAdd(&s.mass[b], w[j]);
+            add_mass(b, w[j]);
           }
       }
       sync();
@@ -336,88 +354,114 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
       while (take > 1 && static_cast<double>(front + (take - 1) * w) >= limit) take--;
       return min(take, equal);
     };
+    constexpr int kPer = kList / kSampleThreads;
+    // The row's logits in bins [lo, hi] and not below `floor_value`, as keys in s.merged, the
+    // largest first.  Returns their number; more than kList of them are not listed.
+    auto collect = [&](int which, int lo, int hi, float floor_value) -> unsigned {
+      for (int i = tid; i < n; i += kSampleThreads) {
+        const float v = slice[i];
+        if (v == -INFINITY || v < floor_value) continue;
+        const int b = bin_of(v);
+        if (b < lo || b > hi) continue;
+        const unsigned at = atomicAdd(&s.listed[which], 1u);
+        if (at < kList) s.list[at] = sample_key(v);
+      }
+      sync();  // after it nobody reads counts and weights of a bin any more
+      unsigned lens[split], size = 0;
+#pragma unroll
+      for (int k = 0; k < split; k++) {
+        lens[k] = split > 1 ? peer_u32(&s.listed[which], k) : s.listed[which];
+        size += lens[k];
+      }
+      if (size > kList) return size;
+      uint32_t got[kPer];
+      unsigned at = 0;
+#pragma unroll
+      for (int j = 0; j < kPer; j++) got[j] = 0;
+#pragma unroll
+      for (int k = 0; k < split; k++) {
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+          const unsigned i = tid + j * kSampleThreads - at;
+          if (i < lens[k]) got[j] = split > 1 ? peer_u32(&s.list[i], k) : s.list[i];
+        }
+        at += lens[k];
+      }
+      // bitonic sort (zeros, no logit's key, behind)
+      unsigned m = 32;
+      while (m < size) m <<= 1;
+#pragma unroll
+      for (int j = 0; j < kPer; j++)
+        if (tid + j * kSampleThreads < m) s.merged[tid + j * kSampleThreads] = got[j];
+      __syncthreads();
+      for (unsigned len = 2; len <= m; len <<= 1)
+        for (unsigned gap = len >> 1; gap > 0; gap >>= 1) {
+          if (tid < m / 2) {
+            const unsigned p0 = 2 * tid - (tid & (gap - 1)), p1 = p0 + gap;
+            const uint32_t x0 = s.merged[p0], x1 = s.merged[p1];
+            if ((x0 < x1) == ((p0 & len) == 0)) {
+              s.merged[p0] = x1;
+              s.merged[p1] = x0;
+            }
+          }
+          // up to 64 entries one warp does it all
+          if (m > 64)
+            __syncthreads();
+          else
+            __syncwarp();
+        }
+      __syncthreads();
+      return size;
+    };
+    // Of the first `stay` of the `size` keys in s.merged, with weight `acc` before them: those
+    // that have less than `limit` in front (limit >= 0), or with share >= 0 less than that share
+    // of their own weight.  Sets the results of a search.
+    auto choose = [&](unsigned size, unsigned stay, u64 acc, double limit, double share) {
+      if (limit >= 0.0 || share >= 0.0) {
+        u64 w[kPer], sum = 0, front;
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+          const unsigned i = tid * kPer + j;
+          w[j] = i < stay ? weigher(key_value(s.merged[i])) : 0;
+          sum += w[j];
+        }
+        const u64 all = block_scan(sum, &front, s.warp_sum);
+        if (share >= 0.0) limit = share * static_cast<double>(all);
+        unsigned kept = 0;
+        u64 f = acc + front;
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+          kept += __syncthreads_count(tid * kPer + j < stay && static_cast<double>(f) < limit);
+          f += w[j];
+        }
+        stay = max(kept, 1u);
+      }
+      const uint32_t key = s.merged[stay - 1];
+      unsigned above = 0, equal = 0;
+#pragma unroll
+      for (int j = 0; j < kPer; j++) {
+        const unsigned i = tid * kPer + j;
+        above += __syncthreads_count(i < size && s.merged[i] > key);
+        equal += __syncthreads_count(i < size && s.merged[i] == key);
+      }
+      if (tid == 0) {
+        s.edge = key;
+        s.take = stay - above;
+        s.equals = equal;
+        s.need = s.take < equal ? s.take : kAll;
+      }
+      __syncthreads();
+    };
     // The edge within bin s.bin (of s.size logits): the `want`-th largest of the bin, or with
     // limit >= 0 the last one that has less than `limit` in front of it, `acc` being the weight
     // of the bins before.  Sets s.edge, s.equals (logits equal to it), s.take (how many of them
     // stay) and s.need (the same, kAll if all do).
-    auto search = [&](bool weights, unsigned want, u64 acc, double limit) {
+    auto search = [&](int which, bool weights, unsigned want, u64 acc, double limit) {
       const int bin = s.bin;
-      const unsigned size = s.size;
       const float floor_value = edge ? key_value(edge) : -INFINITY;
-      if (tid == 0) s.listed = 0;
-      sync();  // (the counts and weights of the bins have been read by everyone)
-      if (size <= kList) {
-        for (int i = tid; i < n; i += kSampleThreads) {
-          const float v = slice[i];
-          if (v > -INFINITY && v >= floor_value && bin_of(v) == bin) s.list[atomicAdd(&s.listed, 1u)] = sample_key(v);
-        }
-        sync();
-        constexpr int kPer = kList / kSampleThreads;
-        uint32_t got[kPer];
-        unsigned lens[split], at = 0;
-#pragma unroll
-        for (int j = 0; j < kPer; j++) got[j] = 0;
-#pragma unroll
-        for (int k = 0; k < split; k++) lens[k] = split > 1 ? peer_u32(&s.listed, k) : s.listed;
-#pragma unroll
-        for (int k = 0; k < split; k++) {
-#pragma unroll
-          for (int j = 0; j < kPer; j++) {
-            const unsigned i = tid + j * kSampleThreads - at;
-            if (i < lens[k]) got[j] = split > 1 ? peer_u32(&s.list[i], k) : s.list[i];
-          }
-          at += lens[k];
-        }
-        sync();
-        // bitonic sort, largest first (zeros, no logit's key, behind)
-        unsigned m = 32;
-        while (m < size) m <<= 1;
-        for (int j = 0; j < kPer; j++)
-          if (tid + j * kSampleThreads < m) s.list[tid + j * kSampleThreads] = got[j];
-        __syncthreads();
-        for (unsigned len = 2; len <= m; len <<= 1)
-          for (unsigned gap = len >> 1; gap > 0; gap >>= 1) {
-            for (unsigned i = tid; i < m / 2; i += kSampleThreads) {
-              const unsigned lo = 2 * i - (i & (gap - 1)), hi = lo + gap;
-              const uint32_t x0 = s.list[lo], x1 = s.list[hi];
-              if ((x0 < x1) == ((lo & len) == 0)) {
-                s.list[lo] = x1;
-                s.list[hi] = x0;
-              }
-            }
-            __syncthreads();
-          }
-        // weights in that order: a thread has kPer neighbours
-        u64 w[kPer], sum = 0, front;
-        for (int j = 0; j < kPer; j++) {
-          const unsigned i = tid * kPer + j;
-          w[j] = weights && i < size ? weigher(key_value(s.list[i])) : 0;
-          sum += w[j];
-        }
-        block_scan(sum, &front, s.warp_sum);
-        unsigned stay = want;  // length of the prefix that stays
-        if (limit >= 0.0) {
-          stay = 0;
-          u64 f = acc + front;
-          for (int j = 0; j < kPer; j++) {
-            stay += __syncthreads_count(tid * kPer + j < size && static_cast<double>(f) < limit);
-            f += w[j];
-          }
-        }
-        const uint32_t key = s.list[stay - 1];
-        unsigned above = 0, equal = 0;
-        for (int j = 0; j < kPer; j++) {
-          const unsigned i = tid * kPer + j;
-          above += __syncthreads_count(i < size && s.list[i] > key);
-          equal += __syncthreads_count(i < size && s.list[i] == key);
-        }
-        if (tid == 0) {
-          s.edge = key;
-          s.take = stay - above;
-          s.equals = equal;
-          s.need = s.take < equal ? s.take : kAll;
-        }
-        __syncthreads();
+      if (s.size <= kList) {
+        const unsigned size = collect(which, bin, bin, floor_value);
+        choose(size, limit >= 0.0 ? size : want, acc, limit, -1.0);
         return;
       }
       // many logits in the bin: by the digits of their bits
@@ -434,8 +478,7 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
           if (shift < 24 && (k >> (shift + 8)) != (prefix >> (shift + 8))) continue;
           atomicAdd(&s.count[(k >> shift) & 255], 1u);
           if (weights) {
-            const u64 w = weigher(v);
-            if (w) atomicAdd(&s.mass[(k >> shift) & 255], w);
+            add_mass((k >> shift) & 255, weigher(v));
           }
         }
         sync();
@@ -475,8 +518,36 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
       __syncthreads();
     };
 
+    bool done = false;
+    if (by_count && top_k <= kList / 2) {
+      // The top_k-th largest of the threads' maxima is not above the top_k-th largest logit, and
+      // few logits lie between the two: everything from its bin on goes to the list.
+      if (best > -INFINITY) atomicAdd(&s.count[bin_of(best)], 1u);
+      sync();
+      gather(tid, false, &my_count, &my_mass);
+      all_count = block_scan(my_count, &count_before, s.warp_sum);
+      const u64 want = top_k;
+      if (want <= all_count) {
+        if (count_before < want && want <= count_before + my_count) s.bin = tid;
+        __syncthreads();
+        const unsigned size = collect(0, 0, s.bin, -INFINITY);
+        if (size <= kList) {
+          choose(size, top_k, 0, -1.0, by_mass ? fmax(static_cast<double>(top_p), 0.0) : -1.0);
+          edge = s.edge;
+          need = s.need;
+          done = true;
+        }
+      } else {
+        sync();  // everyone has read the counts
+      }
+      if (!done) {
+        __syncthreads();
+        s.mass[tid] = s.count[tid] = 0;
+        __syncthreads();
+      }
+    }
     u64 dropped = 0;  // weight of the logits equal to the edge that top-k leaves out
-    if (by_count) {
+    if (by_count && !done) {
       histogram(false, -INFINITY);
       const u64 want = top_k;
       if (want < all_count) {
@@ -486,18 +557,18 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
           s.before = static_cast<unsigned>(count_before);
         }
         __syncthreads();
-        search(false, static_cast<unsigned>(want - s.before), 0, -1.0);
+        search(1, false, static_cast<unsigned>(want - s.before), 0, -1.0);
         edge = s.edge;
         need = s.need;
         dropped = (s.equals - s.take) * weigher(key_value(edge));
       }
-    }
-    if (by_mass) {
-      if (by_count) {  // what top-k left; the arrays are free once everyone has read them
+      if (by_mass) {  // the arrays are free once everyone has read them
         sync();
         s.mass[tid] = s.count[tid] = 0;
         __syncthreads();
       }
+    }
+    if (by_mass && !done) {
       histogram(true, edge ? key_value(edge) : -INFINITY);
       const double limit = fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(all_mass - dropped);
       if (limit > 0.0) {
@@ -509,7 +580,7 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
         }
         __syncthreads();
         const u64 acc = s.sum;
-        search(true, 0, acc, limit);
+        search(2, true, 0, acc, limit);
         if (s.edge > edge) {
           edge = s.edge;
           need = s.need;
