@@ -104,21 +104,21 @@ __device__ __forceinline__ unsigned peer_u32(const unsigned *p, int cta) {
 // table of 16 doubles, which lie in different banks; of 128 only 6.9.)
 struct Weigher {
   double max, scale;      // scale = 16 / (T ln 2)
-  float top, cut;         // logits of at most `cut` weigh nothing
-  float floor;            // what those are taken for, so that the arithmetic stays in range
-  bool flat;              // the maximum is +infinity: those logits weigh 1, others nothing
+  float floor;            // 46 T ln 2 below the maximum: weighs 0, and so does what lies below
   const double *table;
-  // N at a time: a weight is a chain of ten dependent fp64 operations
+  // N weights plus kBias each (the bits of 2^52, which the rounding leaves in place).  N at a
+  // time: a weight is a chain of a dozen dependent fp64 operations of about 50 cycles each.
+  static constexpr u64 kBias = 0x4330000000000000ull;
   template <int N>
-  __device__ __forceinline__ void weigh(const float (&x)[N], u64 (&w)[N]) const {
-    double y[N], p[N], r[N];
+  __device__ __forceinline__ void biased(const float (&x)[N], u64 (&w)[N]) const {
+    double p[N], r[N];
     int k[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      y[i] = (max - static_cast<double>(fmaxf(x[i], floor))) * scale;
-      const double shifted = y[i] + 6755399441055744.0;  // 1.5 * 2^52
+      const double y = (max - static_cast<double>(fmaxf(x[i], floor))) * scale;
+      const double shifted = y + 6755399441055744.0;  // 1.5 * 2^52
       k[i] = __double2loint(shifted);
-      r[i] = (y[i] - (shifted - 6755399441055744.0)) * (-0.69314718055994530942 / 16);
+      r[i] = (y - (shifted - 6755399441055744.0)) * (-0.69314718055994530942 / 16);
     }
 #pragma unroll
     for (int i = 0; i < N; i++) p[i] = fma(r[i], 1.0 / 720, 1.0 / 120);
@@ -137,15 +137,14 @@ struct Weigher {
       // 2^(44 - k / 16) by the exponent (k / 16 <= 46), then rounding to an integer
       const double q = __hiloint2double(__double2hiint(p[i]) + ((44 - (k[i] >> 4)) << 20), __double2loint(p[i])) +
                        4503599627370496.0;  // 2^52
-      const u64 bits = static_cast<u64>(__double_as_longlong(q)) & 0xfffffffffffffull;
-      w[i] = x[i] == top ? kOne : (!flat && x[i] > cut ? bits : 0);
+      w[i] = static_cast<u64>(__double_as_longlong(q));
     }
   }
   __device__ __forceinline__ u64 operator()(float x) const {
     const float in[1] = {x};
     u64 w[1];
-    weigh(in, w);
-    return w[0];
+    biased(in, w);
+    return w[0] - kBias;
   }
 };
 
@@ -254,17 +253,29 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
     if (split > 1) cluster_barrier_all();  // the others may still read s.best
     return;
   }
-  const float top = key_value(static_cast<uint32_t>(key >> 32));
+  float top = key_value(static_cast<uint32_t>(key >> 32));
+  const double t = fmin(static_cast<double>(temp), 1e36);
+  const double reach = 46 * 0.69314718055994530942 * t;
+  const double scale = 16 * 1.44269504088896340736 / t;
+  // Weights need a finite maximum, room below it, and fp32 steps there that are small against
+  // the temperature.  +infinity: those logits become 0, the others -infinity.  A maximum near
+  // the lowest value (a row of masks), or far larger than the temperature: logits relative to it.
+  auto floor_of = [&](float from) { return nextafterf(static_cast<float>(from - reach), -INFINITY); };
+  if (top == INFINITY || top - reach < -3.4e38 ||
+      (static_cast<double>(top) - floor_of(top)) * scale > 46.9 * 16) {
+    __syncthreads();
+    for (int i = tid; i < n; i += kSampleThreads) {
+      const float v = slice[i];
+      slice[i] = top == INFINITY ? (v == INFINITY ? 0.0f : -INFINITY) : v - top;
+    }
+    best = best == -INFINITY ? best : (top == INFINITY ? (best == INFINITY ? 0.0f : -INFINITY) : best - top);
+    top = 0.0f;
+    __syncthreads();
+  }
   Weigher weigher;
-  weigher.top = top;
-  weigher.flat = top == INFINITY;
   weigher.max = static_cast<double>(top);
-  weigher.scale = 16 * 1.44269504088896340736 / static_cast<double>(temp);
-  // logits more than 46 T ln 2 below the maximum weigh less than 2^-45 (rounded down: some
-  // that weigh 0 are computed, none that weighs more is left out)
-  weigher.cut = static_cast<float>(fmax(weigher.max - 46 * 0.69314718055994530942 * static_cast<double>(temp), -3.5e38));
-  weigher.cut = weigher.cut > -3.3e38f ? nextafterf(weigher.cut, -INFINITY) : -INFINITY;
-  weigher.floor = weigher.cut > -INFINITY ? weigher.cut : -FLT_MAX;
+  weigher.scale = scale;
+  weigher.floor = floor_of(top);
   weigher.table = s.table;
   const int top_k = a.top_k ? a.top_k[row] : 0;
   const float top_p = a.top_p ? a.top_p[row] : 1.0f;
@@ -279,7 +290,7 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
     // bins of T / 16 below the maximum (of 1 / 16 above temperature 1, where the logits' own
     // spread is what matters), the last one open; float arithmetic is monotonic, so bins
     // respect the order.  -infinity takes no part.
-    const float to_bin = 16.0f * fmaxf(1.0f, static_cast<float>(1.0 / static_cast<double>(temp)));
+    const float to_bin = 16.0f * fmaxf(1.0f, static_cast<float>(1.0 / t));
     auto bin_of = [&](float v) {
       return v == top ? 0 : static_cast<int>(fminf((top - v) * to_bin, static_cast<float>(kBins - 1)));
     };
@@ -329,7 +340,11 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
           some |= in[j];
         }
         if (!some) continue;
-        if (weights) weigher.weigh(v, w);
+        if (weights) {
+          weigher.biased(v, w);
+#pragma unroll
+          for (int j = 0; j < 4; j++) w[j] -= Weigher::kBias;
+        }
 #pragma unroll
         for (int j = 0; j < 4; j++)
           if (in[j]) {
@@ -358,13 +373,29 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
     // The row's logits in bins [lo, hi] and not below `floor_value`, as keys in s.merged, the
     // largest first.  Returns their number; more than kList of them are not listed.
     auto collect = [&](int which, int lo, int hi, float floor_value) -> unsigned {
-      for (int i = tid; i < n; i += kSampleThreads) {
-        const float v = slice[i];
-        if (v == -INFINITY || v < floor_value) continue;
-        const int b = bin_of(v);
-        if (b < lo || b > hi) continue;
-        const unsigned at = atomicAdd(&s.listed[which], 1u);
-        if (at < kList) s.list[at] = sample_key(v);
+      // most logits lie far from the bins: a comparison with bounds one bin wider tells
+      float low = -FLT_MAX, high = INFINITY;
+      if (hi < kBins - 1) low = fmaxf(low, top - static_cast<float>(hi + 2) / to_bin * 1.0001f);
+      if (lo > 0) high = top - static_cast<float>(lo - 1) / to_bin * 0.9999f;
+      low = fmaxf(low, floor_value);
+      for (int i0 = tid; i0 < n; i0 += 8 * kSampleThreads) {
+        float v[8];
+        bool some = false;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const int i = i0 + j * kSampleThreads;
+          v[j] = i < n ? slice[i] : -INFINITY;
+          some |= v[j] >= low && v[j] <= high;
+        }
+        if (!some) continue;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          if (!(v[j] >= low && v[j] <= high)) continue;
+          const int b = bin_of(v[j]);
+          if (b < lo || b > hi) continue;
+          const unsigned at = atomicAdd(&s.listed[which], 1u);
+          if (at < kList) s.list[at] = sample_key(v[j]);
+        }
       }
       sync();  // after it nobody reads counts and weights of a bin any more
       unsigned lens[split], size = 0;
@@ -588,7 +619,7 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
           need = min(need, s.need);
         }
       } else {  // the first token only
-        edge = static_cast<uint32_t>(key >> 32);
+        edge = sample_key(top);
         need = 1;
       }
     }
@@ -615,28 +646,39 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
       }
     }
   }
+  const bool all_kept = edge == 0 && least == 0;
   // weights of four ids from i on, those beyond the thread's run 0; *rank_of counts the ids
   // equal to the edge
   auto weights_at = [&](int i, u64 (&w)[4], u64 *rank_of) {
     float v[4];
-    bool some = false;
+    bool in[4], some = false;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       v[j] = i + j < i1 ? slice[i + j] : -INFINITY;
-      if (v[j] < edge_value) v[j] = -INFINITY;
-      if (need != kAll && v[j] == edge_value && (*rank_of)++ >= need) v[j] = -INFINITY;
-      some |= v[j] > -INFINITY;
+      in[j] = v[j] > -INFINITY && v[j] >= edge_value;
+      if (need != kAll && in[j] && v[j] == edge_value && (*rank_of)++ >= need) in[j] = false;
+      some |= in[j];
     }
 #pragma unroll
     for (int j = 0; j < 4; j++) w[j] = 0;
     if (!some) return;
-    weigher.weigh(v, w);
+    weigher.biased(v, w);
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-      if (w[j] < least) w[j] = 0;
+    for (int j = 0; j < 4; j++) w[j] = in[j] && w[j] - Weigher::kBias >= least ? w[j] - Weigher::kBias : 0;
   };
   u64 mass = 0, before, r = eq_before, w4[4];
-  for (int i = i0; i < i1; i += 4) {
+  int i = i0;
+  if (all_kept) {
+    u64 biases = 0;
+    for (; i + 4 <= i1; i += 4) {
+      const float v[4] = {slice[i], slice[i + 1], slice[i + 2], slice[i + 3]};
+      weigher.biased(v, w4);
+      mass += (w4[0] + w4[1]) + (w4[2] + w4[3]);
+      biases += 4 * Weigher::kBias;
+    }
+    mass -= biases;
+  }
+  for (; i < i1; i += 4) {
     weights_at(i, w4, &r);
     mass += (w4[0] + w4[1]) + (w4[2] + w4[3]);
   }
@@ -662,7 +704,7 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
     u64 sum = before;
     int pick = -1;
     r = eq_before;
-    for (int i = i0; i < i1 && pick < 0; i += 4) {
+    for (i = i0; i < i1 && pick < 0; i += 4) {
       weights_at(i, w4, &r);
 #pragma unroll
       for (int j = 0; j < 4; j++) {
