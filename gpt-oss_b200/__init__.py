@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import pathlib
+import struct
 
 import numpy as np
 
@@ -166,9 +167,9 @@ def load_library() -> ctypes.CDLL:
         "gptoss_decode_set_kv": (c_int, [vp, c_int, c_int, c_int, c_int, c_int, vp, vp]),
         "gptoss_decode_get_kv": (c_int, [vp, c_int, c_int, c_int, c_int, c_int, vp, vp]),
         "gptoss_decode_rope_table": (c_int, [c_int, ctypes.c_float, ctypes.c_float, c_int, vp, fp]),
-        "gptoss_decode_rope_append": (c_int, [ctypes.POINTER(RopeArgs), vp]),
-        "gptoss_decode_prompt_attention": (c_int, [ctypes.POINTER(AttentionArgs), vp]),
-        "gptoss_decode_sample": (c_int, [ctypes.POINTER(SampleArgs), vp]),
+        "gptoss_decode_rope_append": (c_int, [vp, vp]),
+        "gptoss_decode_prompt_attention": (c_int, [vp, vp]),
+        "gptoss_decode_sample": (c_int, [vp, vp]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(lib, name)
@@ -208,8 +209,23 @@ def permute_static(slot_expert, slot_weight, n_rows, top_k, n_experts, expert_of
         raise MoeError(rc, lib.gptoss_moe_last_error(None).decode())
 
 
-# -- the handle-free operators of a prompt pass and of a drawn token
-_DTYPE_CODES = {"torch.bfloat16": 0, "torch.float16": 1, "torch.float32": 2}
+# -- the handle-free operators of a prompt pass and of a drawn token.  A decode step calls them
+# for every layer, so the checks are kept cheap: dtypes are compared by identity, devices by
+# index, and the argument structs are packed rather than filled field by field.
+_DTYPE_CODES = {}
+_ROPE_PACK = struct.Struct("@9P7qf8i0q").pack
+_ATTENTION_PACK = struct.Struct("@9P5qf8i0q").pack
+_SAMPLE_PACK = struct.Struct("@8Pq3i0q").pack
+
+
+def _dtype_codes():
+    """torch dtype -> GPTOSS_DTYPE_*, filled on the first call (the callers pass torch tensors)."""
+    if not _DTYPE_CODES:
+        import torch
+
+        _DTYPE_CODES.update({torch.bfloat16: 0, torch.float16: 1, torch.float32: 2,
+                             "int32": torch.int32, "int64": torch.int64, "float32": torch.float32})
+    return _DTYPE_CODES
 
 
 def _check_op(lib, rc):
@@ -218,46 +234,49 @@ def _check_op(lib, rc):
 
 
 def _dtype_code(t, what):
-    code = _DTYPE_CODES.get(str(t.dtype))
+    code = _dtype_codes().get(t.dtype)
     if code is None:
         raise TypeError(f"{what}: element type {t.dtype} is not supported")
     return code
 
 
 def _vector(t, what, dtype, n, device):
-    """Address of a contiguous 1-D tensor of n elements (None stays None)."""
+    """Address of a contiguous 1-D tensor of n elements (0 for None)."""
     if t is None:
-        return None
-    if str(t.dtype) != dtype:
-        raise TypeError(f"{what} must be {dtype}, not {t.dtype}")
-    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        return 0
+    if (t.dtype is not dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous()
+            or t.get_device() != device):
+        if t.dtype is not dtype:
+            raise TypeError(f"{what} must be {dtype}, not {t.dtype}")
+        if t.get_device() != device:
+            raise ValueError(f"{what} is on {t.device}, expected cuda:{device}")
         raise ValueError(f"{what} must be contiguous with {n} elements, not {tuple(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{what} is on {t.device}, expected {device}")
     return t.data_ptr()
 
 
-def _rows(t, what, dtype, device, heads=None, head_dim=None):
-    """(address, row stride) of a [rows, heads, head_dim] tensor with contiguous heads."""
+def _rows(t, what, dtype, device, heads, head_dim):
+    """(address, row stride, rows) of a [rows, heads, head_dim] tensor with contiguous heads."""
     if t is None:
-        return None, 0
-    if t.dtype != dtype:
+        return 0, 0, 0
+    if t.dtype is not dtype:
         raise TypeError(f"{what} must be {dtype}, not {t.dtype}")
-    if t.dim() != 3 or (heads is not None and tuple(t.shape[1:]) != (heads, head_dim)):
+    if t.get_device() != device:
+        raise ValueError(f"{what} is on {t.device}, expected cuda:{device}")
+    if t.dim() != 3:
         raise ValueError(f"{what} must be [rows, {heads}, {head_dim}], not {tuple(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{what} is on {t.device}, expected {device}")
     rows, h, d = t.shape
+    if h != heads or d != head_dim:
+        raise ValueError(f"{what} must be [rows, {heads}, {head_dim}], not {tuple(t.shape)}")
     s0, s1, s2 = t.stride()
-    if (d > 1 and s2 != 1) or (h > 1 and s1 != d):
+    if (s2 != 1 and d > 1) or (s1 != d and h > 1):
         raise ValueError(f"{what}: the heads of a row must be contiguous (strides {t.stride()})")
-    return t.data_ptr(), (s0 if rows > 1 else h * d)
+    return t.data_ptr(), (s0 if rows > 1 else h * d), rows
 
 
 def _on_gpu(t, what):
     if not t.is_cuda:
         raise ValueError(f"{what} must be on a GPU, it is on {t.device}")
-    return t.device
+    return t.get_device()
 
 
 def rope_table(rotary_dim, theta, scaling_factor=1.0, initial_context_length=4096):
@@ -280,33 +299,34 @@ def rope_append(q, k, v, pos, inv_freq, q_out=None, k_cache=None, v_cache=None, 
     row i); inv_freq float32 [rotary_dim / 2].  q_out may be q, and without slots k_cache may
     be k.  All tensors are on one GPU, `stream` is a stream of it (0: its default stream)."""
     lib = load_library()
-    first = next((t for t in (q, k, v) if t is not None), None)
+    first = q if q is not None else (k if k is not None else v)
     if first is None:
         raise ValueError("q, k and v are all None")
-    dev, dtype, rows, d = _on_gpu(first, "input"), first.dtype, first.shape[0], first.shape[-1]
+    dev, code, dtype = _on_gpu(first, "input"), _dtype_code(first, "input"), first.dtype
+    if first.dim() != 3:
+        raise ValueError("the inputs must be [rows, heads, head_dim]")
+    rows, _, d = first.shape
     kv = k if k is not None else v
     hq, hkv = (0 if q is None else q.shape[1]), (0 if kv is None else kv.shape[1])
-    qp, qs = _rows(q, "q", dtype, dev, hq, d)
-    kp, ks = _rows(k, "k", dtype, dev, hkv, d)
-    vp, vs = _rows(v, "v", dtype, dev, hkv, d)
-    qop, qos = _rows(q_out, "q_out", dtype, dev, hq, d)
-    kcp, kcs = _rows(k_cache, "k_cache", dtype, dev, hkv, d)
-    vcp, vcs = _rows(v_cache, "v_cache", dtype, dev, hkv, d)
-    for name, t in (("k", k), ("v", v)):
-        if t is not None and t.shape[0] != rows:
-            raise ValueError(f"{name} has {t.shape[0]} rows, expected {rows}")
-    if q_out is not None and q_out.shape[0] != rows:
-        raise ValueError(f"q_out has {q_out.shape[0]} rows, expected {rows}")
-    caches = [t.shape[0] for t in (k_cache, v_cache) if t is not None]
-    if len(set(caches)) > 1:
+    qp, qs, nq = _rows(q, "q", dtype, dev, hq, d)
+    kp, ks, nk = _rows(k, "k", dtype, dev, hkv, d)
+    vp, vs, nv = _rows(v, "v", dtype, dev, hkv, d)
+    qop, qos, nqo = _rows(q_out, "q_out", dtype, dev, hq, d)
+    kcp, kcs, nkc = _rows(k_cache, "k_cache", dtype, dev, hkv, d)
+    vcp, vcs, nvc = _rows(v_cache, "v_cache", dtype, dev, hkv, d)
+    for name, t, n in (("q", q, nq), ("k", k, nk), ("v", v, nv), ("q_out", q_out, nqo)):
+        if n != rows and t is not None:
+            raise ValueError(f"{name} has {n} rows, expected {rows}")
+    if k_cache is not None and v_cache is not None and nkc != nvc:
         raise ValueError("k_cache and v_cache have different numbers of rows")
-    args = RopeArgs(qp, kp, vp, qop, kcp, vcp, _vector(pos, "pos", "torch.int32", rows, dev),
-                    _vector(slots, "slots", "torch.int64", rows, dev),
-                    _vector(inv_freq, "inv_freq", "torch.float32", inv_freq.shape[0], dev),
-                    qs, ks, vs, qos, kcs, vcs, caches[0] if caches else 0, concentration, rows, hq,
-                    hkv, d, 2 * inv_freq.shape[0], interleaved, angle_f32,
-                    _dtype_code(first, "input"))
-    _check_op(lib, lib.gptoss_decode_rope_append(ctypes.byref(args), ctypes.c_void_p(stream)))
+    types = _DTYPE_CODES
+    half = inv_freq.shape[0]
+    args = _ROPE_PACK(qp, kp, vp, qop, kcp, vcp, _vector(pos, "pos", types["int32"], rows, dev),
+                      _vector(slots, "slots", types["int64"], rows, dev),
+                      _vector(inv_freq, "inv_freq", types["float32"], half, dev),
+                      qs, ks, vs, qos, kcs, vcs, nkc or nvc, concentration, rows, hq, hkv, d,
+                      2 * half, interleaved, angle_f32, code)
+    _check_op(lib, lib.gptoss_decode_rope_append(args, stream))
 
 
 def prompt_attention(q, k, v, q_start, kv_start, kv_len, out, sinks=None, scale=None, window=0,
@@ -318,26 +338,27 @@ def prompt_attention(q, k, v, q_start, kv_start, kv_len, out, sinks=None, scale=
     to 1 / sqrt(head_dim); window 0 = none; max_kv_len: the largest kv_len where the caller
     knows it; status: int32 [1] tensor or None."""
     lib = load_library()
-    dev, dtype = _on_gpu(q, "q"), q.dtype
+    dev, code, dtype = _on_gpu(q, "q"), _dtype_code(q, "q"), q.dtype
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError("q and k must have three dimensions")
     tokens, hq, d = q.shape
-    n_kv, hkv, _ = k.shape
-    qp, qs = _rows(q, "q", dtype, dev, hq, d)
-    kp, ks = _rows(k, "k", dtype, dev, hkv, d)
-    vp, vs = _rows(v, "v", dtype, dev, hkv, d)
-    op, os_ = _rows(out, "out", dtype, dev, hq, d)
-    if v.shape[0] != n_kv or out.shape[0] != tokens:
+    hkv = k.shape[1]
+    qp, qs, _ = _rows(q, "q", dtype, dev, hq, d)
+    kp, ks, n_kv = _rows(k, "k", dtype, dev, hkv, d)
+    vp, vs, n_v = _rows(v, "v", dtype, dev, hkv, d)
+    op, os_, n_out = _rows(out, "out", dtype, dev, hq, d)
+    if n_v != n_kv or n_out != tokens:
         raise ValueError("k and v, or q and out, have different numbers of rows")
     n = kv_len.shape[0]
-    args = AttentionArgs(qp, kp, vp, op, _vector(q_start, "q_start", "torch.int32", n + 1, dev),
-                         _vector(kv_start, "kv_start", "torch.int64", n, dev),
-                         _vector(kv_len, "kv_len", "torch.int32", n, dev),
-                         _vector(sinks, "sinks", "torch.float32", hq, dev),
-                         _vector(status, "status", "torch.int32", 1, dev), qs, ks, vs, os_, n_kv,
-                         d ** -0.5 if scale is None else scale, tokens, n, hq, hkv, d, window,
-                         max_kv_len, _dtype_code(q, "q"))
-    _check_op(lib, lib.gptoss_decode_prompt_attention(ctypes.byref(args), ctypes.c_void_p(stream)))
+    types = _DTYPE_CODES
+    args = _ATTENTION_PACK(qp, kp, vp, op, _vector(q_start, "q_start", types["int32"], n + 1, dev),
+                           _vector(kv_start, "kv_start", types["int64"], n, dev),
+                           _vector(kv_len, "kv_len", types["int32"], n, dev),
+                           _vector(sinks, "sinks", types["float32"], hq, dev),
+                           _vector(status, "status", types["int32"], 1, dev), qs, ks, vs, os_, n_kv,
+                           d ** -0.5 if scale is None else scale, tokens, n, hq, hkv, d, window,
+                           max_kv_len, code)
+    _check_op(lib, lib.gptoss_decode_prompt_attention(args, stream))
 
 
 def sample_tokens(logits, u, next_tokens, temperature=None, top_k=None, top_p=None, min_p=None,
@@ -347,19 +368,19 @@ def sample_tokens(logits, u, next_tokens, temperature=None, top_k=None, top_p=No
     min_p float32 [rows], top_k int32 [rows], pos int32 [rows]; None switches one off
     (temperature None = 1; a temperature <= 0 is the argmax)."""
     lib = load_library()
-    dev = _on_gpu(logits, "logits")
+    dev, code = _on_gpu(logits, "logits"), _dtype_code(logits, "logits")
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits must be [rows, vocab] with contiguous rows")
     rows, vocab = logits.shape
-    f32, i32 = "torch.float32", "torch.int32"
-    args = SampleArgs(logits.data_ptr(), _vector(u, "u", f32, rows, dev),
-                      _vector(temperature, "temperature", f32, rows, dev),
-                      _vector(top_k, "top_k", i32, rows, dev), _vector(top_p, "top_p", f32, rows, dev),
-                      _vector(min_p, "min_p", f32, rows, dev), _vector(pos, "pos", i32, rows, dev),
-                      _vector(next_tokens, "next_tokens", i32, rows, dev),
-                      logits.stride(0) if rows > 1 else vocab, rows, vocab,
-                      _dtype_code(logits, "logits"))
-    _check_op(lib, lib.gptoss_decode_sample(ctypes.byref(args), ctypes.c_void_p(stream)))
+    f32, i32 = _DTYPE_CODES["float32"], _DTYPE_CODES["int32"]
+    args = _SAMPLE_PACK(logits.data_ptr(), _vector(u, "u", f32, rows, dev),
+                        _vector(temperature, "temperature", f32, rows, dev),
+                        _vector(top_k, "top_k", i32, rows, dev),
+                        _vector(top_p, "top_p", f32, rows, dev),
+                        _vector(min_p, "min_p", f32, rows, dev), _vector(pos, "pos", i32, rows, dev),
+                        _vector(next_tokens, "next_tokens", i32, rows, dev),
+                        logits.stride(0) if rows > 1 else vocab, rows, vocab, code)
+    _check_op(lib, lib.gptoss_decode_sample(args, stream))
 
 
 class MoeEngine:

@@ -99,3 +99,21 @@ def test_getp_host_program_fails_loudly_without_gpu(pkg, tmp_path):
                          capture_output=True, text=True, timeout=120)
     assert res.returncode != 0
     assert "no sm_100 GPU" in res.stderr
+
+
+def test_operator_structs_match_header(pkg):
+    """Field order and size of the operators' argument structs, and of the packed form that the
+    binding passes."""
+    import struct
+
+    text = (pkg.HEADER_PATH.parent / "gptoss_decode_b200.h").read_text()
+    text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
+    for name, mirror, pack in (("gptoss_rope_args_t", pkg.RopeArgs, "@9P7qf8i0q"),
+                               ("gptoss_attention_args_t", pkg.AttentionArgs, "@9P5qf8i0q"),
+                               ("gptoss_sample_args_t", pkg.SampleArgs, "@8Pq3i0q")):
+        end = text.index("} " + name + ";")
+        body = text[text.rindex("typedef struct {", 0, end):end]
+        order = [w.strip(" *\n") for line in re.findall(r"(?:void|int|float|long long) ([^;]+);", body)
+                 for w in line.split(",")]
+        assert order == [f[0] for f in mirror._fields_]
+        assert ctypes.sizeof(mirror) == struct.calcsize(pack)
