@@ -72,6 +72,11 @@ class ModelConfig(ctypes.Structure):
                 ("swiglu_limit", ctypes.c_float)]
 
 
+class Sampling(ctypes.Structure):
+    """Mirror of gptoss_decode_sampling_t."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("u", "temperature", "top_k", "top_p", "min_p")]
+
+
 class RopeArgs(ctypes.Structure):
     """Mirror of gptoss_rope_args_t."""
     _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out", "k_cache", "v_cache", "pos",
@@ -166,6 +171,10 @@ def load_library() -> ctypes.CDLL:
         "gptoss_decode_set_tensor": (c_int, [vp, c_char_p, c_int, vp, c_int, c_int]),
         "gptoss_decode_set_kv": (c_int, [vp, c_int, c_int, c_int, c_int, c_int, vp, vp]),
         "gptoss_decode_get_kv": (c_int, [vp, c_int, c_int, c_int, c_int, c_int, vp, vp]),
+        "gptoss_decode_create_prefill": (c_int, [ctypes.POINTER(ModelConfig), c_int, c_int, c_int,
+                                                 ctypes.POINTER(vp)]),
+        "gptoss_decode_step_sample": (c_int, [vp, vp, vp, c_int, ctypes.POINTER(Sampling), vp, vp]),
+        "gptoss_decode_prefill": (c_int, [vp, vp, vp, vp, vp, c_int, ctypes.POINTER(Sampling), vp, vp]),
         "gptoss_decode_rope_table": (c_int, [c_int, ctypes.c_float, ctypes.c_float, c_int, vp, fp]),
         "gptoss_decode_rope_append": (c_int, [vp, vp]),
         "gptoss_decode_prompt_attention": (c_int, [vp, vp]),
@@ -588,14 +597,22 @@ class DecodeEngine:
     sequences (row i owns KV-cache slot i)."""
 
     def __init__(self, cfg: dict, max_batch: int, device: int = 0, ep_rank: int = 0,
-                 ep_size: int = 1):
+                 ep_size: int = 1, max_tokens: int | None = None):
+        """max_tokens: rows of one prefill pass (default: max_batch)."""
         self.lib = load_library()
         self.cfg = dict(cfg)
         self.max_batch = max_batch
+        self.max_tokens = max_batch if max_tokens is None else max_tokens
         c = ModelConfig(**cfg)
         h = ctypes.c_void_p()
-        rc = self.lib.gptoss_decode_create_ep(ctypes.byref(c), max_batch, device, ep_rank, ep_size,
-                                              ctypes.byref(h))
+        if max_tokens is None:
+            rc = self.lib.gptoss_decode_create_ep(ctypes.byref(c), max_batch, device, ep_rank,
+                                                  ep_size, ctypes.byref(h))
+        elif ep_size > 1:
+            raise ValueError("max_tokens is for engines with all experts local")
+        else:
+            rc = self.lib.gptoss_decode_create_prefill(ctypes.byref(c), max_batch, max_tokens,
+                                                       device, ctypes.byref(h))
         if rc != 0:
             raise MoeError(rc, (self.lib.gptoss_decode_last_error(None) or b"").decode())
         self.handle = h
@@ -633,17 +650,66 @@ class DecodeEngine:
         """The MoE engine inside, with MoeEngine's methods (weights, options, timers, EP)."""
         c = self.cfg
         cfg = MoeConfig(c["hidden_dim"], c["intermediate_dim"], c["n_experts"],
-                        c["experts_per_token"], c["n_layers"], self.max_batch, c["swiglu_limit"],
+                        c["experts_per_token"], c["n_layers"], self.max_tokens, c["swiglu_limit"],
                         ep_rank, ep_size, WEIGHTS_BF16, device)
         return MoeEngine.borrowed(ctypes.c_void_p(self.lib.gptoss_decode_moe(self.handle)), cfg)
 
-    def step(self, tokens, pos, stream: int = 0):
+    @staticmethod
+    def _sampling(sampling, n):
+        """(struct or None, arrays kept alive) from a dict of u, temperature, top_k, top_p, min_p."""
+        if sampling is None:
+            return None, None
+        unknown = set(sampling) - {"u", "temperature", "top_k", "top_p", "min_p"}
+        if unknown:
+            raise ValueError(f"unknown sampling settings: {sorted(unknown)}")
+        keep = {}
+        for name, value in sampling.items():
+            if value is not None:
+                a = np.ascontiguousarray(value, dtype=np.int32 if name == "top_k" else np.float32)
+                if a.shape != (n,):
+                    raise ValueError(f"{name} must have {n} entries, not {a.shape}")
+                keep[name] = a
+        s = Sampling(*[keep[n].ctypes.data if n in keep else None
+                       for n in ("u", "temperature", "top_k", "top_p", "min_p")])
+        return s, keep
+
+    def step(self, tokens, pos, stream: int = 0, sampling: dict | None = None):
+        """One token per row.  sampling: None for the argmax, or a dict with the uniform numbers
+        "u" and any of "temperature", "top_k", "top_p", "min_p" (one entry per row)."""
         tokens = np.ascontiguousarray(tokens, dtype=np.int32)
         pos = np.ascontiguousarray(pos, dtype=np.int32)
+        if tokens.ndim != 1 or pos.shape != tokens.shape:
+            raise ValueError("tokens and pos must be 1-D of one length")
         nxt = np.empty(tokens.shape[0], dtype=np.int32)
-        self._check(self.lib.gptoss_decode_step(self.handle, _ptr(tokens), _ptr(pos),
-                                                tokens.shape[0], _ptr(nxt),
-                                                ctypes.c_void_p(stream)))
+        if sampling is None:
+            self._check(self.lib.gptoss_decode_step(self.handle, _ptr(tokens), _ptr(pos),
+                                                    tokens.shape[0], _ptr(nxt),
+                                                    ctypes.c_void_p(stream)))
+            return nxt
+        s, keep = self._sampling(sampling, tokens.shape[0])
+        self._check(self.lib.gptoss_decode_step_sample(self.handle, _ptr(tokens), _ptr(pos),
+                                                       tokens.shape[0], ctypes.byref(s), _ptr(nxt),
+                                                       ctypes.c_void_p(stream)))
+        del keep
+        return nxt
+
+    def prefill(self, prompts, rows, pos0=None, stream: int = 0, sampling: dict | None = None):
+        """Feeds prompts[i] (token ids) to cache row rows[i] from position pos0[i] (default 0) on
+        and returns the token that follows each."""
+        prompts = [np.ascontiguousarray(p, dtype=np.int32).reshape(-1) for p in prompts]
+        n = len(prompts)
+        rows = np.ascontiguousarray(rows, dtype=np.int32)
+        pos0 = np.zeros(n, np.int32) if pos0 is None else np.ascontiguousarray(pos0, dtype=np.int32)
+        if rows.shape != (n,) or pos0.shape != (n,):
+            raise ValueError(f"rows and pos0 must have an entry for each of the {n} prompts")
+        tokens = np.concatenate(prompts) if n else np.empty(0, np.int32)
+        lens = np.array([p.shape[0] for p in prompts], dtype=np.int32)
+        nxt = np.empty(n, dtype=np.int32)
+        s, keep = self._sampling(sampling, n)
+        self._check(self.lib.gptoss_decode_prefill(
+            self.handle, _ptr(tokens), _ptr(rows), _ptr(pos0), _ptr(lens), n,
+            None if s is None else ctypes.byref(s), _ptr(nxt), ctypes.c_void_p(stream)))
+        del keep
         return nxt
 
     def logits(self, row: int) -> np.ndarray:

@@ -24,6 +24,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
 #include <atomic>
 #include <string>
 #include <vector>
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(256)
 argmax_rows_kernel(const float *__restrict__ logits, const int *__restrict__ pos,
                    int *__restrict__ next, int V) {
   const int row = blockIdx.x;
-  if (pos[row] < 0) {
+  if (pos && pos[row] < 0) {
     if (threadIdx.x == 0) next[row] = -1;
     return;
   }
@@ -401,13 +402,54 @@ argmax_rows_kernel(const float *__restrict__ logits, const int *__restrict__ pos
   if (threadIdx.x == 0) next[row] = si[0] == 0x7fffffff ? 0 : si[0];
 }
 
+// dst[to[i], :] = x[from[i], :]
+__global__ void __launch_bounds__(256)
+gather_last_rows_kernel(bf16 *__restrict__ dst, const bf16 *__restrict__ x,
+                        const int *__restrict__ from, const int *__restrict__ to, int n, int H) {
+  const int lane = threadIdx.x & 31;
+  const int i = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (i >= n) return;
+  const uint4 *s4 = reinterpret_cast<const uint4 *>(x + static_cast<size_t>(from[i]) * H);
+  uint4 *d4 = reinterpret_cast<uint4 *>(dst + static_cast<size_t>(to[i]) * H);
+  for (int p = lane; p < (H >> 3); p += 32) d4[p] = s4[p];
+}
+
 }  // namespace gptoss
 
 using namespace gptoss;
 
+// Host image of one pass over prompt tokens, copied to the device in one piece; sizes for
+// `rows` tokens and `seqs` sequences.
+struct PromptLayout {
+  size_t slots, kv_start, tokens, pos, q_start, kv_len, last_from, last_to, bytes;
+  PromptLayout(size_t rows, size_t seqs) {
+    size_t at = 0;
+    auto take = [&](size_t n, size_t size) {
+      const size_t here = at;
+      at += n * size;
+      return here;
+    };
+    slots = take(rows, 8);
+    kv_start = take(seqs, 8);
+    tokens = take(rows, 4);
+    pos = take(rows, 4);
+    q_start = take(seqs + 1, 4);
+    kv_len = take(seqs, 4);
+    last_from = take(seqs, 4);
+    last_to = take(seqs, 4);
+    bytes = at;
+  }
+};
+// One pass, on the device: `tokens` rows of `seqs` (pieces of) sequences.
+struct PromptPass {
+  int tokens, seqs, max_kv_len;
+  const long long *slots, *kv_start;
+  const int *q_start, *kv_len;
+};
+
 struct gptoss_decode {
   gptoss_model_config_t cfg;
-  int max_batch = 0, device = 0;
+  int max_batch = 0, max_rows = 0, device = 0;  // sequences; rows of one pass
   gptoss_moe *moe = nullptr;
   cublasHandle_t blas = nullptr;
   bool loaded = false;
@@ -422,6 +464,10 @@ struct gptoss_decode {
   float *qkv = nullptr, *q = nullptr, *proj = nullptr, *logits = nullptr;
   int *d_tokens = nullptr, *d_pos = nullptr, *d_next = nullptr, *status = nullptr;
   int *h_pinned = nullptr;  // tokens | pos | next, max_batch each
+  bf16 *last_x = nullptr;   // [max_batch, H] residual rows of the prompts' last tokens
+  // prompt passes and sampling settings: device copies and their pinned sources
+  unsigned char *prompt_dev = nullptr, *prompt_host = nullptr;
+  float *samp_dev = nullptr, *samp_host = nullptr;  // u | temperature | top_p | min_p | top_k
   // QKV and output projections on this library's tcgen05 kernel (one "expert" = all rows)
   bool own_gemm = true;
   int num_sms = 0, sched_B = -1, sched_cap = 0;
@@ -566,11 +612,17 @@ int gptoss_decode_destroy(gptoss_decode_t *h) {
   cudaFree(h->attn); cudaFree(h->k_cache); cudaFree(h->v_cache); cudaFree(h->qkv); cudaFree(h->q);
   cudaFree(h->proj); cudaFree(h->logits); cudaFree(h->d_tokens); cudaFree(h->d_pos);
   cudaFree(h->d_next); cudaFree(h->status); cudaFree(h->lin_sched); cudaFree(h->ones);
-  cudaFree(h->qkv_bf); cudaFree(h->proj_bf);
+  cudaFree(h->qkv_bf); cudaFree(h->proj_bf); cudaFree(h->last_x); cudaFree(h->prompt_dev);
+  cudaFree(h->samp_dev);
+  if (h->prompt_host) cudaFreeHost(h->prompt_host);
+  if (h->samp_host) cudaFreeHost(h->samp_host);
   if (h->h_pinned) cudaFreeHost(h->h_pinned);
   delete h;
   return GPTOSS_OK;
 }
+
+static int decode_create(const gptoss_model_config_t *cfg, int max_batch, int max_rows, int device,
+                         int ep_rank, int ep_size, gptoss_decode_t **out);
 
 int gptoss_decode_create(const gptoss_model_config_t *cfg, int max_batch, int device,
                          gptoss_decode_t **out) {
@@ -579,6 +631,17 @@ int gptoss_decode_create(const gptoss_model_config_t *cfg, int max_batch, int de
 
 int gptoss_decode_create_ep(const gptoss_model_config_t *cfg, int max_batch, int device,
                             int ep_rank, int ep_size, gptoss_decode_t **out) {
+  return decode_create(cfg, max_batch, max_batch, device, ep_rank, ep_size, out);
+}
+
+int gptoss_decode_create_prefill(const gptoss_model_config_t *cfg, int max_batch, int max_tokens,
+                                 int device, gptoss_decode_t **out) {
+  if (max_tokens < max_batch) return dfail(nullptr, GPTOSS_E_INVALID, "max_tokens %d < max_batch %d", max_tokens, max_batch);
+  return decode_create(cfg, max_batch, max_tokens, device, 0, 1, out);
+}
+
+static int decode_create(const gptoss_model_config_t *cfg, int max_batch, int max_rows, int device,
+                         int ep_rank, int ep_size, gptoss_decode_t **out) {
   if (!cfg || !out) return dfail(nullptr, GPTOSS_E_INVALID, "null argument");
   *out = nullptr;
   const gptoss_model_config_t &c = *cfg;
@@ -598,7 +661,7 @@ int gptoss_decode_create_ep(const gptoss_model_config_t *cfg, int max_batch, int
   mc.n_experts = c.n_experts;
   mc.experts_per_token = c.experts_per_token;
   mc.n_layers = c.n_layers;
-  mc.max_tokens = max_batch;
+  mc.max_tokens = max_rows;
   mc.swiglu_limit = c.swiglu_limit;
   mc.ep_rank = ep_rank;
   mc.ep_size = ep_size < 1 ? 1 : ep_size;
@@ -610,6 +673,7 @@ int gptoss_decode_create_ep(const gptoss_model_config_t *cfg, int max_batch, int
   gptoss_decode *h = new gptoss_decode();
   h->cfg = c;
   h->max_batch = max_batch;
+  h->max_rows = max_rows;
   h->device = device;
   h->moe = moe;
   h->have.assign(c.n_layers + 1, 0u);
@@ -621,6 +685,7 @@ int gptoss_decode_create_ep(const gptoss_model_config_t *cfg, int max_batch, int
   std::string err;
   const size_t V = c.vocab_size, H = c.hidden_dim, L = c.n_layers, D = c.head_dim;
   const size_t dq = c.n_attn_heads * D, dkv = c.n_kv_heads * D, B = max_batch, S = c.seq_len;
+  const size_t R = max_rows;
   cudaError_t e = cudaSuccess;
   auto A = [&](cudaError_t r) { if (e == cudaSuccess) e = r; };
   A(dalloc(&h->emb, V * H)); A(dalloc(&h->unemb, V * H));
@@ -628,25 +693,31 @@ int gptoss_decode_create_ep(const gptoss_model_config_t *cfg, int max_batch, int
   A(dalloc(&h->rms_attn, L * H)); A(dalloc(&h->rms_ffn, L * H)); A(dalloc(&h->rms_out, H));
   A(dalloc(&h->b_qkv, L * (dq + 2 * dkv))); A(dalloc(&h->b_o, L * H));
   A(dalloc(&h->sinks, L * c.n_attn_heads)); A(dalloc(&h->inv_freq, D / 2));
-  A(dalloc(&h->x, B * H)); A(dalloc(&h->t, B * H)); A(dalloc(&h->attn, B * dq));
+  A(dalloc(&h->x, R * H)); A(dalloc(&h->t, R * H)); A(dalloc(&h->attn, R * dq));
   A(dalloc(&h->k_cache, L * B * S * dkv)); A(dalloc(&h->v_cache, L * B * S * dkv));
-  A(dalloc(&h->qkv, B * (dq + 2 * dkv))); A(dalloc(&h->q, B * dq)); A(dalloc(&h->proj, B * H));
+  A(dalloc(&h->qkv, B * (dq + 2 * dkv))); A(dalloc(&h->q, R * dq)); A(dalloc(&h->proj, B * H));
   A(dalloc(&h->logits, B * V));
   A(dalloc(&h->d_tokens, B)); A(dalloc(&h->d_pos, B)); A(dalloc(&h->d_next, B));
   A(dalloc(&h->status, 1));
-  h->sched_cap = (max_batch + 255) / 256 + 1;
+  h->sched_cap = (max_rows + 255) / 256 + 1;
   A(dalloc(&h->lin_sched, 3 * static_cast<size_t>(h->sched_cap) + 1));
-  A(dalloc(&h->ones, B));
-  A(dalloc(&h->qkv_bf, B * (dq + 2 * dkv)));
-  A(dalloc(&h->proj_bf, B * H));
+  A(dalloc(&h->ones, R));
+  A(dalloc(&h->qkv_bf, R * (dq + 2 * dkv)));
+  A(dalloc(&h->proj_bf, R * H));
+  const PromptLayout prompt(R, B);
+  A(dalloc(&h->last_x, B * H));
+  A(dalloc(&h->prompt_dev, prompt.bytes));
+  A(dalloc(&h->samp_dev, 5 * B));
+  A(cudaMallocHost(reinterpret_cast<void **>(&h->prompt_host), prompt.bytes));
+  A(cudaMallocHost(reinterpret_cast<void **>(&h->samp_host), 5 * B * sizeof(float)));
   A(cudaDeviceGetAttribute(&h->num_sms, cudaDevAttrMultiProcessorCount, device));
   A(cudaMallocHost(reinterpret_cast<void **>(&h->h_pinned), 3 * B * sizeof(int)));
   if (e == cudaSuccess) e = cudaMemset(h->status, 0, sizeof(int));
-  if (e == cudaSuccess) e = cudaMemset(h->x, 0, B * H * sizeof(bf16));
+  if (e == cudaSuccess) e = cudaMemset(h->x, 0, R * H * sizeof(bf16));
   if (e != cudaSuccess) return bail(GPTOSS_E_CUDA, std::string("allocation: ") + cudaGetErrorString(e));
   {
-    std::vector<float> one(B, 1.0f);
-    e = cudaMemcpy(h->ones, one.data(), B * sizeof(float), cudaMemcpyHostToDevice);
+    std::vector<float> one(R, 1.0f);
+    e = cudaMemcpy(h->ones, one.data(), R * sizeof(float), cudaMemcpyHostToDevice);
     if (e != cudaSuccess) return bail(GPTOSS_E_CUDA, cudaGetErrorString(e));
   }
   std::vector<float> inv(c.head_dim / 2);
@@ -837,8 +908,8 @@ static int build_linear_maps(gptoss_decode *h) {
   if (!rc) rc = make_tmap_2d_bf16(&h->tm_unemb, h->unemb, H, c.vocab_size, kTileK, 128, &err);
   const uint32_t boxes[3] = {128, 32, 8};
   for (int i = 0; i < 3 && !rc; i++) {
-    rc = make_tmap_2d_bf16(&h->tm_t[i], h->t, H, h->max_batch, kTileK, boxes[i], &err) ||
-         make_tmap_2d_bf16(&h->tm_attn[i], h->attn, dq, h->max_batch, kTileK, boxes[i], &err);
+    rc = make_tmap_2d_bf16(&h->tm_t[i], h->t, H, h->max_rows, kTileK, boxes[i], &err) ||
+         make_tmap_2d_bf16(&h->tm_attn[i], h->attn, dq, h->max_rows, kTileK, boxes[i], &err);
   }
   if (rc) return dfail(h, GPTOSS_E_CUDA, "tensor maps of the projections: %s", err.c_str());
   h->maps_ready = true;
@@ -886,96 +957,15 @@ static int linear_own(gptoss_decode *h, const CUtensorMap &tw, const CUtensorMap
   return GPTOSS_OK;
 }
 
-int gptoss_decode_step(gptoss_decode_t *h, const int *tokens, const int *pos, int B, int *next,
-                       void *stream) {
-  if (!h || !tokens || !pos || !next) return GPTOSS_E_INVALID;
-  if (!h->loaded) return dfail(h, GPTOSS_E_STATE, "weights not loaded");
-  if (B < 0 || B > h->max_batch) return dfail(h, GPTOSS_E_CAPACITY, "batch %d > max_batch %d", B, h->max_batch);
-  if (B == 0) return GPTOSS_OK;
+// the tcgen05 kernel writes whole 16-byte segments: row lengths must be multiples of 8
+static bool own_linear(const gptoss_decode *h) {
   const gptoss_model_config_t &c = h->cfg;
-  for (int i = 0; i < B; i++)
-    if (pos[i] >= c.seq_len) return dfail(h, GPTOSS_E_CAPACITY, "row %d: position %d >= seq_len %d", i, pos[i], c.seq_len);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  DCK(h, cudaSetDevice(h->device));
-  const int H = c.hidden_dim, D = c.head_dim, Hq = c.n_attn_heads, Hkv = c.n_kv_heads;
-  const int dq = Hq * D, dkv = Hkv * D, S = c.seq_len, V = c.vocab_size;
-  int *hp = h->h_pinned;
-  memcpy(hp, tokens, B * sizeof(int));
-  memcpy(hp + h->max_batch, pos, B * sizeof(int));
-  DCK(h, cudaMemcpyAsync(h->d_tokens, hp, B * sizeof(int), cudaMemcpyHostToDevice, st));
-  DCK(h, cudaMemcpyAsync(h->d_pos, hp + h->max_batch, B * sizeof(int), cudaMemcpyHostToDevice, st));
-  const int warps = 8;
-  embed_rows_kernel<<<(B + warps - 1) / warps, warps * 32, 0, st>>>(h->x, h->emb, h->d_tokens,
-                                                                   h->d_pos, B, H, V, h->status);
-  DCK(h, cudaGetLastError());
-  int rc;
-  // the tcgen05 kernel writes whole 16-byte segments: row lengths must be multiples of 8
-  const bool own = h->own_gemm && ((dq + 2 * dkv) % 8 == 0) && (dq % 8 == 0);
-  if (own) {
-    if (!h->maps_ready && (rc = build_linear_maps(h))) return rc;
-    if (h->sched_B != B && (rc = build_linear_schedule(h, B, st))) return rc;
-  }
-  for (int l = 0; l < c.n_layers; l++) {
-    DCK(h, launch_rmsnorm(h->t, h->x, h->rms_attn + static_cast<size_t>(l) * H, h->d_pos, B, H, st, nullptr));
-    if (own)
-      rc = linear_own(h, h->tm_wqkv[l], h->tm_t, h->b_qkv + static_cast<size_t>(l) * (dq + 2 * dkv),
-                      h->qkv_bf, dq + 2 * dkv, H, st);
-    else
-      rc = gemm_xwt(h, h->t, h->w_qkv + static_cast<size_t>(l) * (dq + 2 * dkv) * H, h->qkv, B,
-                    dq + 2 * dkv, H, st);
-    if (rc) return rc;
-    bf16 *kc = h->k_cache + static_cast<size_t>(l) * h->max_batch * S * dkv;
-    bf16 *vc = h->v_cache + static_cast<size_t>(l) * h->max_batch * S * dkv;
-    if (own)
-      qkv_rope_cache_kernel<true><<<B, 256, 0, st>>>(h->qkv_bf, nullptr, h->d_pos, h->inv_freq,
-                                                     h->concentration, h->q, kc, vc, B, Hq, Hkv, D, S);
-    else
-      qkv_rope_cache_kernel<false><<<B, 256, 0, st>>>(
-          h->qkv, h->b_qkv + static_cast<size_t>(l) * (dq + 2 * dkv), h->d_pos, h->inv_freq,
-          h->concentration, h->q, kc, vc, B, Hq, Hkv, D, S);
-    DCK(h, cudaGetLastError());
-    // sliding window on even layers (run.cpp:619)
-    const int window = (c.sliding_window > 0 && (l % 2 == 0)) ? c.sliding_window : 0;
-    // one CTA per (row, KV head): the group's query heads are the rows of the MMA tiles
-    const int grid = B * Hkv, threads = kAttnWarps * 32;
-    const float *sinks = h->sinks + static_cast<size_t>(l) * Hq;
-    if (D == 32)
-      attn_decode_kernel<32><<<grid, threads, 0, st>>>(h->q, kc, vc, sinks, h->d_pos, h->attn, B, Hq, Hkv, S, window);
-    else if (D == 64)
-      attn_decode_kernel<64><<<grid, threads, 0, st>>>(h->q, kc, vc, sinks, h->d_pos, h->attn, B, Hq, Hkv, S, window);
-    else
-      attn_decode_kernel<128><<<grid, threads, 0, st>>>(h->q, kc, vc, sinks, h->d_pos, h->attn, B, Hq, Hkv, S, window);
-    DCK(h, cudaGetLastError());
-    const size_t n = static_cast<size_t>(B) * H;
-    if (own) {
-      if ((rc = linear_own(h, h->tm_wo[l], h->tm_attn, h->b_o + static_cast<size_t>(l) * H,
-                           h->proj_bf, H, dq, st)))
-        return rc;
-      bias_residual_kernel<true><<<static_cast<unsigned>((n + 255) / 256), 256, 0, st>>>(
-          h->x, h->proj_bf, nullptr, h->d_pos, B, H);
-    } else {
-      if ((rc = gemm_xwt(h, h->attn, h->w_o + static_cast<size_t>(l) * H * dq, h->proj, B, H, dq, st)))
-        return rc;
-      bias_residual_kernel<false><<<static_cast<unsigned>((n + 255) / 256), 256, 0, st>>>(
-          h->x, h->proj, h->b_o + static_cast<size_t>(l) * H, h->d_pos, B, H);
-    }
-    DCK(h, cudaGetLastError());
-    DCK(h, launch_rmsnorm(h->t, h->x, h->rms_ffn + static_cast<size_t>(l) * H, h->d_pos, B, H, st, nullptr));
-    rc = gptoss_moe_forward(h->moe, l, h->t, h->x, h->d_pos, B, st);
-    if (rc) return dfail(h, rc, "MoE layer %d: %s", l, gptoss_moe_last_error(h->moe));
-  }
-  DCK(h, launch_rmsnorm(h->t, h->x, h->rms_out, h->d_pos, B, H, st, nullptr));
-  // fp32 logits: own kernel when the rows of the logits are 16-byte multiples, else cuBLAS
-  if (own && V % 4 == 0)
-    rc = linear_own(h, h->tm_unemb, h->tm_t, nullptr, h->logits, V, H, st, /*f32_out=*/true);
-  else
-    rc = gemm_xwt(h, h->t, h->unemb, h->logits, B, V, H, st);
-  if (rc) return rc;
-  argmax_rows_kernel<<<B, 256, 0, st>>>(h->logits, h->d_pos, h->d_next, V);
-  DCK(h, cudaGetLastError());
-  DCK(h, cudaMemcpyAsync(hp + 2 * h->max_batch, h->d_next, B * sizeof(int), cudaMemcpyDeviceToHost, st));
-  DCK(h, cudaStreamSynchronize(st));
-  memcpy(next, hp + 2 * h->max_batch, B * sizeof(int));
+  const int dq = c.n_attn_heads * c.head_dim, dkv = c.n_kv_heads * c.head_dim;
+  return h->own_gemm && (dq + 2 * dkv) % 8 == 0 && dq % 8 == 0;
+}
+
+// What the step's kernels and the MoE engine's reported since the last look (synchronises).
+static int read_status(gptoss_decode *h) {
   int dev_status = 0;
   DCK(h, cudaMemcpy(&dev_status, h->status, sizeof(int), cudaMemcpyDeviceToHost));
   if (dev_status) {
@@ -986,6 +976,314 @@ int gptoss_decode_step(gptoss_decode_t *h, const int *tokens, const int *pos, in
   if (gptoss_moe_take_status(h->moe) != GPTOSS_OK)
     return dfail(h, GPTOSS_E_DEVICE, "MoE block: %s", gptoss_moe_last_error(h->moe));
   return GPTOSS_OK;
+}
+
+// Rotary positions, cache append and attention of one layer for the rows of a prompt pass:
+// h->qkv_bf -> h->attn.  The angles are rounded as in the step's kernel, so that a sequence's
+// keys do not depend on how it was brought in.
+static int prompt_attend(gptoss_decode *h, const PromptPass &pass, const int *pos, bf16 *kc, bf16 *vc,
+                         const float *sinks, int window, cudaStream_t st) {
+  const gptoss_model_config_t &c = h->cfg;
+  const long long dq = static_cast<long long>(c.n_attn_heads) * c.head_dim;
+  const long long dkv = static_cast<long long>(c.n_kv_heads) * c.head_dim, ld = dq + 2 * dkv;
+  gptoss_rope_args_t r = {};
+  r.q = h->qkv_bf;
+  r.k = h->qkv_bf + dq;
+  r.v = h->qkv_bf + dq + dkv;
+  r.q_out = h->q;  // (the step's fp32 q buffer, used for bf16 here)
+  r.k_cache = kc;
+  r.v_cache = vc;
+  r.pos = pos;
+  r.slots = pass.slots;
+  r.inv_freq = h->inv_freq;
+  r.q_stride = r.k_stride = r.v_stride = ld;
+  r.q_out_stride = dq;
+  r.k_cache_stride = r.v_cache_stride = dkv;
+  r.n_slots = static_cast<long long>(h->max_batch) * c.seq_len;
+  r.concentration = h->concentration;
+  r.n_rows = pass.tokens;
+  r.n_q_heads = c.n_attn_heads;
+  r.n_kv_heads = c.n_kv_heads;
+  r.head_dim = r.rotary_dim = c.head_dim;
+  r.angle_f32 = 1;
+  r.dtype = GPTOSS_DTYPE_BF16;
+  int rc = gptoss_decode_rope_append(&r, st);
+  if (rc) return dfail(h, rc, "%s", gptoss_decode_last_error(nullptr));
+  gptoss_attention_args_t a = {};
+  a.q = h->q;
+  a.k = kc;
+  a.v = vc;
+  a.out = h->attn;
+  a.q_start = pass.q_start;
+  a.kv_start = pass.kv_start;
+  a.kv_len = pass.kv_len;
+  a.sinks = sinks;
+  a.status = h->status;
+  a.q_stride = a.out_stride = dq;
+  a.k_stride = a.v_stride = dkv;
+  a.n_kv_rows = r.n_slots;
+  a.scale = 1.0f / sqrtf(static_cast<float>(c.head_dim));
+  a.n_tokens = pass.tokens;
+  a.n_seqs = pass.seqs;
+  a.n_q_heads = c.n_attn_heads;
+  a.n_kv_heads = c.n_kv_heads;
+  a.head_dim = c.head_dim;
+  a.window = window;
+  a.max_kv_len = pass.max_kv_len;
+  a.dtype = GPTOSS_DTYPE_BF16;
+  rc = gptoss_decode_prompt_attention(&a, st);
+  return rc ? dfail(h, rc, "%s", gptoss_decode_last_error(nullptr)) : GPTOSS_OK;
+}
+
+// Embedding and all layers for B rows whose tokens and positions are on the device.  pass:
+// the rows are pieces of prompts (see PromptPass); nullptr: row i is the next token of sequence i.
+static int run_layers(gptoss_decode *h, int B, const int *tokens, const int *pos, const PromptPass *pass,
+                      cudaStream_t st) {
+  const gptoss_model_config_t &c = h->cfg;
+  const int H = c.hidden_dim, D = c.head_dim, Hq = c.n_attn_heads, Hkv = c.n_kv_heads;
+  const int dq = Hq * D, dkv = Hkv * D, S = c.seq_len, V = c.vocab_size;
+  const int warps = 8;
+  embed_rows_kernel<<<(B + warps - 1) / warps, warps * 32, 0, st>>>(h->x, h->emb, tokens, pos,
+                                                                   B, H, V, h->status);
+  DCK(h, cudaGetLastError());
+  int rc;
+  const bool own = own_linear(h);
+  if (own) {
+    if (!h->maps_ready && (rc = build_linear_maps(h))) return rc;
+    if (h->sched_B != B && (rc = build_linear_schedule(h, B, st))) return rc;
+  }
+  for (int l = 0; l < c.n_layers; l++) {
+    DCK(h, launch_rmsnorm(h->t, h->x, h->rms_attn + static_cast<size_t>(l) * H, pos, B, H, st, nullptr));
+    if (own)
+      rc = linear_own(h, h->tm_wqkv[l], h->tm_t, h->b_qkv + static_cast<size_t>(l) * (dq + 2 * dkv),
+                      h->qkv_bf, dq + 2 * dkv, H, st);
+    else
+      rc = gemm_xwt(h, h->t, h->w_qkv + static_cast<size_t>(l) * (dq + 2 * dkv) * H, h->qkv, B,
+                    dq + 2 * dkv, H, st);
+    if (rc) return rc;
+    bf16 *kc = h->k_cache + static_cast<size_t>(l) * h->max_batch * S * dkv;
+    bf16 *vc = h->v_cache + static_cast<size_t>(l) * h->max_batch * S * dkv;
+    // sliding window on even layers (run.cpp:619)
+    const int window = (c.sliding_window > 0 && (l % 2 == 0)) ? c.sliding_window : 0;
+    const float *sinks = h->sinks + static_cast<size_t>(l) * Hq;
+    if (pass) {
+      if ((rc = prompt_attend(h, *pass, pos, kc, vc, sinks, window, st))) return rc;
+    } else {
+      if (own)
+        qkv_rope_cache_kernel<true><<<B, 256, 0, st>>>(h->qkv_bf, nullptr, pos, h->inv_freq,
+                                                       h->concentration, h->q, kc, vc, B, Hq, Hkv, D, S);
+      else
+        qkv_rope_cache_kernel<false><<<B, 256, 0, st>>>(
+            h->qkv, h->b_qkv + static_cast<size_t>(l) * (dq + 2 * dkv), pos, h->inv_freq,
+            h->concentration, h->q, kc, vc, B, Hq, Hkv, D, S);
+      DCK(h, cudaGetLastError());
+      // one CTA per (row, KV head): the group's query heads are the rows of the MMA tiles
+      const int grid = B * Hkv, threads = kAttnWarps * 32;
+      if (D == 32)
+        attn_decode_kernel<32><<<grid, threads, 0, st>>>(h->q, kc, vc, sinks, pos, h->attn, B, Hq, Hkv, S, window);
+      else if (D == 64)
+        attn_decode_kernel<64><<<grid, threads, 0, st>>>(h->q, kc, vc, sinks, pos, h->attn, B, Hq, Hkv, S, window);
+      else
+        attn_decode_kernel<128><<<grid, threads, 0, st>>>(h->q, kc, vc, sinks, pos, h->attn, B, Hq, Hkv, S, window);
+      DCK(h, cudaGetLastError());
+    }
+    const size_t n = static_cast<size_t>(B) * H;
+    if (own) {
+      if ((rc = linear_own(h, h->tm_wo[l], h->tm_attn, h->b_o + static_cast<size_t>(l) * H,
+                           h->proj_bf, H, dq, st)))
+        return rc;
+      bias_residual_kernel<true><<<static_cast<unsigned>((n + 255) / 256), 256, 0, st>>>(
+          h->x, h->proj_bf, nullptr, pos, B, H);
+    } else {
+      if ((rc = gemm_xwt(h, h->attn, h->w_o + static_cast<size_t>(l) * H * dq, h->proj, B, H, dq, st)))
+        return rc;
+      bias_residual_kernel<false><<<static_cast<unsigned>((n + 255) / 256), 256, 0, st>>>(
+          h->x, h->proj, h->b_o + static_cast<size_t>(l) * H, pos, B, H);
+    }
+    DCK(h, cudaGetLastError());
+    DCK(h, launch_rmsnorm(h->t, h->x, h->rms_ffn + static_cast<size_t>(l) * H, pos, B, H, st, nullptr));
+    rc = gptoss_moe_forward(h->moe, l, h->t, h->x, pos, B, st);
+    if (rc) return dfail(h, rc, "MoE layer %d: %s", l, gptoss_moe_last_error(h->moe));
+  }
+  return GPTOSS_OK;
+}
+
+// Final norm of B residual rows, logits, and the next tokens into h->d_next: the argmax, or a
+// draw.  pos: inactive rows (NULL: none).
+static int finish_rows(gptoss_decode *h, const bf16 *x, int B, const int *pos,
+                       const gptoss_decode_sampling_t *sampling, cudaStream_t st) {
+  const gptoss_model_config_t &c = h->cfg;
+  const int H = c.hidden_dim, V = c.vocab_size;
+  int rc;
+  DCK(h, launch_rmsnorm(h->t, x, h->rms_out, pos, B, H, st, nullptr));
+  // fp32 logits: own kernel when the rows of the logits are 16-byte multiples, else cuBLAS
+  if (own_linear(h) && V % 4 == 0) {
+    if (h->sched_B != B && (rc = build_linear_schedule(h, B, st))) return rc;
+    rc = linear_own(h, h->tm_unemb, h->tm_t, nullptr, h->logits, V, H, st, /*f32_out=*/true);
+  } else {
+    rc = gemm_xwt(h, h->t, h->unemb, h->logits, B, V, H, st);
+  }
+  if (rc) return rc;
+  if (!sampling) {
+    argmax_rows_kernel<<<B, 256, 0, st>>>(h->logits, pos, h->d_next, V);
+    DCK(h, cudaGetLastError());
+    return GPTOSS_OK;
+  }
+  const size_t n = B, stride = h->max_batch;
+  gptoss_sample_args_t a = {};
+  auto put = [&](int i, const void *src) -> float * {
+    if (!src) return nullptr;
+    memcpy(h->samp_host + i * stride, src, n * sizeof(float));
+    return h->samp_dev + i * stride;
+  };
+  a.logits = h->logits;
+  a.u = put(0, sampling->u);
+  a.temperature = put(1, sampling->temperature);
+  a.top_p = put(2, sampling->top_p);
+  a.min_p = put(3, sampling->min_p);
+  a.top_k = reinterpret_cast<const int *>(put(4, sampling->top_k));
+  DCK(h, cudaMemcpyAsync(h->samp_dev, h->samp_host, 5 * stride * sizeof(float), cudaMemcpyHostToDevice, st));
+  a.pos = pos;
+  a.next = h->d_next;
+  a.stride = a.vocab = V;
+  a.n_rows = B;
+  a.dtype = GPTOSS_DTYPE_FP32;
+  rc = gptoss_decode_sample(&a, st);
+  return rc ? dfail(h, rc, "%s", gptoss_decode_last_error(nullptr)) : GPTOSS_OK;
+}
+
+// The drawn or greedy tokens to the host, and whatever the kernels reported.
+static int read_next(gptoss_decode *h, int n, int *next, cudaStream_t st) {
+  int *hp = h->h_pinned;
+  DCK(h, cudaMemcpyAsync(hp + 2 * h->max_batch, h->d_next, n * sizeof(int), cudaMemcpyDeviceToHost, st));
+  DCK(h, cudaStreamSynchronize(st));
+  memcpy(next, hp + 2 * h->max_batch, n * sizeof(int));
+  return read_status(h);
+}
+
+static int check_sampling(gptoss_decode *h, const gptoss_decode_sampling_t *s) {
+  if (!s) return GPTOSS_OK;
+  if (!s->u) return dfail(h, GPTOSS_E_INVALID, "sampling needs the uniform numbers u");
+  if (h->cfg.vocab_size > (1 << 18))
+    return dfail(h, GPTOSS_E_CAPACITY, "sampling takes vocabularies of up to 262144, this one has %d", h->cfg.vocab_size);
+  return GPTOSS_OK;
+}
+
+int gptoss_decode_step(gptoss_decode_t *h, const int *tokens, const int *pos, int B, int *next,
+                       void *stream) {
+  return gptoss_decode_step_sample(h, tokens, pos, B, nullptr, next, stream);
+}
+
+int gptoss_decode_step_sample(gptoss_decode_t *h, const int *tokens, const int *pos, int B,
+                              const gptoss_decode_sampling_t *sampling, int *next, void *stream) {
+  if (!h || !tokens || !pos || !next) return GPTOSS_E_INVALID;
+  if (!h->loaded) return dfail(h, GPTOSS_E_STATE, "weights not loaded");
+  if (B < 0 || B > h->max_batch) return dfail(h, GPTOSS_E_CAPACITY, "batch %d > max_batch %d", B, h->max_batch);
+  if (int rc = check_sampling(h, sampling)) return rc;
+  if (B == 0) return GPTOSS_OK;
+  const gptoss_model_config_t &c = h->cfg;
+  for (int i = 0; i < B; i++)
+    if (pos[i] >= c.seq_len) return dfail(h, GPTOSS_E_CAPACITY, "row %d: position %d >= seq_len %d", i, pos[i], c.seq_len);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  DCK(h, cudaSetDevice(h->device));
+  int *hp = h->h_pinned;
+  memcpy(hp, tokens, B * sizeof(int));
+  memcpy(hp + h->max_batch, pos, B * sizeof(int));
+  DCK(h, cudaMemcpyAsync(h->d_tokens, hp, B * sizeof(int), cudaMemcpyHostToDevice, st));
+  DCK(h, cudaMemcpyAsync(h->d_pos, hp + h->max_batch, B * sizeof(int), cudaMemcpyHostToDevice, st));
+  int rc;
+  if ((rc = run_layers(h, B, h->d_tokens, h->d_pos, nullptr, st)) ||
+      (rc = finish_rows(h, h->x, B, h->d_pos, sampling, st)))
+    return rc;
+  return read_next(h, B, next, st);
+}
+
+int gptoss_decode_prefill(gptoss_decode_t *h, const int *tokens, const int *rows, const int *pos0,
+                          const int *lens, int n_seqs, const gptoss_decode_sampling_t *sampling,
+                          int *next, void *stream) {
+  if (!h) return GPTOSS_E_INVALID;
+  if (n_seqs < 0 || (n_seqs > 0 && (!tokens || !rows || !pos0 || !lens || !next)))
+    return dfail(h, GPTOSS_E_INVALID, "prefill: null argument or negative count");
+  if (!h->loaded) return dfail(h, GPTOSS_E_STATE, "weights not loaded");
+  if (h->moe->ep_size > 1)
+    return dfail(h, GPTOSS_E_STATE, "prefill: the ranks of expert parallelism step together, prompts go through gptoss_decode_step there");
+  if (n_seqs > h->max_batch) return dfail(h, GPTOSS_E_CAPACITY, "prefill: %d sequences > max_batch %d", n_seqs, h->max_batch);
+  if (int rc = check_sampling(h, sampling)) return rc;
+  const gptoss_model_config_t &c = h->cfg;
+  const size_t S = c.seq_len;
+  if (!own_linear(h)) return dfail(h, GPTOSS_E_STATE, "prefill: the projections' shapes need the step's fallback path");
+  if (static_cast<size_t>(h->max_batch) * S > INT32_MAX - 256)
+    return dfail(h, GPTOSS_E_CAPACITY, "prefill: max_batch * seq_len is above 2^31 - 257");
+  std::vector<char> used(h->max_batch, 0);
+  long long total = 0;
+  for (int i = 0; i < n_seqs; i++) {
+    if (rows[i] < 0 || rows[i] >= h->max_batch || used[rows[i]])
+      return dfail(h, GPTOSS_E_INVALID, "prefill: sequence %d: row %d is out of range or given twice", i, rows[i]);
+    used[rows[i]] = 1;
+    if (lens[i] < 1 || pos0[i] < 0) return dfail(h, GPTOSS_E_INVALID, "prefill: sequence %d: no tokens or a negative position", i);
+    if (static_cast<long long>(pos0[i]) + lens[i] > c.seq_len)
+      return dfail(h, GPTOSS_E_CAPACITY, "prefill: sequence %d ends at %lld > seq_len %d", i,
+                   static_cast<long long>(pos0[i]) + lens[i], c.seq_len);
+    total += lens[i];
+  }
+  for (long long i = 0; i < total; i++)
+    if (tokens[i] < 0 || tokens[i] >= c.vocab_size)
+      return dfail(h, GPTOSS_E_INVALID, "prefill: token %lld is %d, outside the vocabulary", i, tokens[i]);
+  if (n_seqs == 0) return GPTOSS_OK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  DCK(h, cudaSetDevice(h->device));
+  const PromptLayout at(h->max_rows, h->max_batch);
+  unsigned char *hp = h->prompt_host, *dp = h->prompt_dev;
+  auto host = [&](size_t off) { return reinterpret_cast<int *>(hp + off); };
+  auto dev = [&](size_t off) { return reinterpret_cast<int *>(dp + off); };
+  int seq = 0, done = 0;  // tokens of sequence `seq` that went through so far
+  const int *next_token = tokens;
+  while (seq < n_seqs) {
+    // as many tokens as a pass takes; a prompt that does not fit goes on in the next pass, on
+    // top of what is in the cache by then
+    PromptPass pass = {};
+    int last = 0;
+    while (seq < n_seqs && pass.tokens < h->max_rows) {
+      const int n = std::min(lens[seq] - done, h->max_rows - pass.tokens);
+      const long long base = static_cast<long long>(rows[seq]) * c.seq_len;
+      host(at.q_start)[pass.seqs] = pass.tokens;
+      host(at.kv_len)[pass.seqs] = pos0[seq] + done + n;
+      reinterpret_cast<long long *>(hp + at.kv_start)[pass.seqs] = base;
+      for (int j = 0; j < n; j++) {
+        const int p = pos0[seq] + done + j, r = pass.tokens + j;
+        host(at.tokens)[r] = *next_token++;
+        host(at.pos)[r] = p;
+        reinterpret_cast<long long *>(hp + at.slots)[r] = base + p;
+      }
+      pass.max_kv_len = std::max(pass.max_kv_len, pos0[seq] + done + n);
+      pass.tokens += n;
+      pass.seqs++;
+      done += n;
+      if (done == lens[seq]) {
+        host(at.last_from)[last] = pass.tokens - 1;
+        host(at.last_to)[last++] = seq;
+        seq++;
+        done = 0;
+      }
+    }
+    host(at.q_start)[pass.seqs] = pass.tokens;
+    DCK(h, cudaMemcpyAsync(dp, hp, at.bytes, cudaMemcpyHostToDevice, st));
+    pass.slots = reinterpret_cast<const long long *>(dp + at.slots);
+    pass.kv_start = reinterpret_cast<const long long *>(dp + at.kv_start);
+    pass.q_start = dev(at.q_start);
+    pass.kv_len = dev(at.kv_len);
+    int rc = run_layers(h, pass.tokens, dev(at.tokens), dev(at.pos), &pass, st);
+    if (rc) return rc;
+    if (last > 0) {
+      gather_last_rows_kernel<<<(last + 7) / 8, 256, 0, st>>>(h->last_x, h->x, dev(at.last_from),
+                                                              dev(at.last_to), last, c.hidden_dim);
+      DCK(h, cudaGetLastError());
+    }
+    // the pinned image is written again for the next pass
+    if (seq < n_seqs) DCK(h, cudaStreamSynchronize(st));
+  }
+  int rc = finish_rows(h, h->last_x, n_seqs, nullptr, sampling, st);
+  return rc ? rc : read_next(h, n_seqs, next, st);
 }
 
 int gptoss_decode_get_logits(gptoss_decode_t *h, int row, float *logits_host) {

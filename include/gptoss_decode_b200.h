@@ -123,8 +123,44 @@ int gptoss_decode_get_kv(gptoss_decode_t *h, int layer, int row0, int n_rows, in
  * run.cpp:780-791).  Synchronises the stream before returning. */
 int gptoss_decode_step(gptoss_decode_t *h, const int *tokens, const int *pos, int batch,
                        int *next, void *stream);
-/* fp32 logits [vocab_size] of batch row `row` from the last step. */
+/* fp32 logits [vocab_size] of batch row `row` from the last step (after a prefill: of the last
+ * token of its sequence number `row`). */
 int gptoss_decode_get_logits(gptoss_decode_t *h, int row, float *logits_host);
+
+/* How next tokens are drawn (host arrays, one entry per row of the step or per sequence of the
+ * prefill; NULL: 1, no limit, no limit, no limit; u is required): see gptoss_decode_sample. */
+typedef struct {
+  const float *u;
+  const float *temperature;
+  const int *top_k;
+  const float *top_p;
+  const float *min_p;
+} gptoss_decode_sampling_t;
+/* gptoss_decode_step with the next tokens drawn instead of taken as argmax (sampling NULL: the
+ * same as gptoss_decode_step). */
+int gptoss_decode_step_sample(gptoss_decode_t *h, const int *tokens, const int *pos, int batch,
+                              const gptoss_decode_sampling_t *sampling, int *next, void *stream);
+
+/* An engine whose passes take up to max_tokens rows (at least max_batch): prompts are fed
+ * max_tokens tokens at a time by gptoss_decode_prefill.  Engines of the other create calls have
+ * max_tokens = max_batch.  All experts local. */
+int gptoss_decode_create_prefill(const gptoss_model_config_t *cfg, int max_batch, int max_tokens,
+                                 int device, gptoss_decode_t **out);
+/*
+ * Whole prompts instead of a token per step (the reference feeds them through its decode
+ * step, getp_run.cpp:969-979).  Sequence i of n_seqs owns the next lens[i] entries of `tokens`
+ * (packed, host) and goes to cache row rows[i], positions pos0[i] .. pos0[i] + lens[i] - 1;
+ * pos0[i] > 0 continues what that row holds.  The rows of one call are different.  next[i]
+ * receives the token after the last one of sequence i: the argmax, or drawn as `sampling` says.
+ * Same arithmetic as the step except for the order of sums in the attention and its
+ * probabilities, which are rounded to bf16 there too; the cache it leaves is what the steps
+ * leave.  Prompts longer than max_tokens, and as many of them as do not fit, go through in
+ * several passes.  All tokens and positions are checked first; a call that is refused has
+ * changed nothing.  Synchronises the stream.  Not under expert parallelism (GPTOSS_E_STATE).
+ */
+int gptoss_decode_prefill(gptoss_decode_t *h, const int *tokens, const int *rows, const int *pos0,
+                          const int *lens, int n_seqs, const gptoss_decode_sampling_t *sampling,
+                          int *next, void *stream);
 /* The MoE engine inside (for its options, taps and stage timers). */
 gptoss_moe_t *gptoss_decode_moe(gptoss_decode_t *h);
 

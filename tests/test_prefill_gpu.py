@@ -1,0 +1,211 @@
+"""Prompts brought in by the prefill against the same prompts fed token by token, against the
+reference's recorded logits, and drawn tokens against a draw from the step's own logits.
+
+Tolerances.  Prefill and step run the same GEMMs row by row; their attention sums in another
+order with probabilities rounded to bf16 in both, so the residual stream differs by roundings
+to bf16 that fall the other way: the limits of the decode tests for logits against the fp32
+reference (2e-2 largest, 2e-3 mean, logits of std 0.23) hold for each side, and twice that
+between the two.
+"""
+import numpy as np
+import pytest
+
+from test_decode_gpu import LOGIT_MAX_ABS, LOGIT_MEAN_ABS, _golden
+from test_sample_gpu import _draw
+
+
+def _engine(pkg, cfg, seed, tmp_path, max_batch, max_tokens=None):
+    from gpt_oss_b200 import synth
+
+    path = tmp_path / "model.bin"
+    if not path.exists():
+        synth.write_model_bin(path, cfg, seed)
+    eng = pkg.DecodeEngine(cfg, max_batch, max_tokens=max_tokens)
+    eng.load_bin(np.asarray(np.memmap(path, dtype=np.uint8, mode="r")))
+    return eng
+
+
+def _close(a, b):
+    err = np.abs(a.astype(np.float64) - b)
+    assert err.max() <= 2 * LOGIT_MAX_ABS and err.mean() <= 2 * LOGIT_MEAN_ABS, (err.max(), err.mean())
+
+
+def _feed(eng, tokens, row, pos0=0):
+    nxt = None
+    for i, t in enumerate(tokens):
+        tok, pos = np.full(eng.max_batch, -1, np.int32), np.full(eng.max_batch, -1, np.int32)
+        tok[row], pos[row] = t, pos0 + i
+        nxt = eng.step(tok, pos)[row]
+    return int(nxt), eng.logits(row)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["tiny", "mini"])
+@pytest.mark.parametrize("max_tokens", [None, 5, 64])
+def test_prefill_matches_reference_logits(pkg, tmp_path, name, max_tokens):
+    """The golden tokens up to several positions, in one or more passes, then a step."""
+    from gpt_oss_b200 import synth
+
+    g = _golden(name)
+    cfg = synth.TINY_MODEL if name == "tiny" else synth.MINI_MODEL
+    eng = _engine(pkg, cfg, int(g["seed"]), tmp_path, 4, max_tokens)
+    tokens, probes = g["tokens"], g["probes"]
+    for n in (1, 2, 13, len(tokens) - 1):
+        eng.prefill([tokens[:n]], [2])
+        err = np.abs(eng.logits(0)[probes].astype(np.float64) - g["probe_logits"][n - 1])
+        assert err.max() <= LOGIT_MAX_ABS and err.mean() <= LOGIT_MEAN_ABS
+        tok, pos = np.full(4, -1, np.int32), np.full(4, -1, np.int32)
+        tok[2], pos[2] = tokens[n], n  # the step goes on from the cache that the prefill left
+        eng.step(tok, pos)
+        err = np.abs(eng.logits(2)[probes].astype(np.float64) - g["probe_logits"][n])
+        assert err.max() <= LOGIT_MAX_ABS and err.mean() <= LOGIT_MEAN_ABS
+    eng.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_tokens", [8, 37, 400])
+def test_several_prompts_and_continuations(pkg, tmp_path, max_tokens):
+    """Prompts of different lengths beyond the window, two of them continued, in passes of
+    several sizes; a row outside the call keeps its cache."""
+    import torch
+
+    from gpt_oss_b200 import synth
+
+    # every expert is selected, so no near-tie in the router separates the two ways
+    cfg = dict(synth.MINI_MODEL, vocab_size=900, sliding_window=21, n_layers=3, seq_len=160, n_attn_heads=6,
+               n_kv_heads=2, n_experts=4, experts_per_token=4)
+    rng = np.random.default_rng(1)
+    lens = [70, 1, 33, 100]
+    prompts = [rng.integers(0, 900, n, dtype=np.int32) for n in lens]
+    more = [rng.integers(0, 900, n, dtype=np.int32) for n in (17, 2)]
+    steps = _engine(pkg, cfg, 5, tmp_path, 6)
+    want = [_feed(steps, p, r) for p, r in zip(prompts, (4, 0, 2, 5))]
+    want_more = [_feed(steps, m, r, p0) for m, r, p0 in zip(more, (4, 2), (70, 33))]
+    eng = _engine(pkg, cfg, 5, tmp_path, 6, max_tokens)
+    dev, dkv = torch.device("cuda:0"), cfg["n_kv_heads"] * cfg["head_dim"]
+    marks = [torch.randn(1, 8, dkv, device=dev).bfloat16() for _ in range(2)]
+    eng.set_kv(1, 3, 0, *marks)
+    nxt = eng.prefill(prompts, [4, 0, 2, 5])
+    for i, (token, logits) in enumerate(want):
+        _close(eng.logits(i), logits)
+        assert nxt[i] == token or logits[token] - logits[nxt[i]] <= 4 * LOGIT_MAX_ABS
+    nxt = eng.prefill(more, [4, 2], pos0=[70, 33])
+    for i, (token, logits) in enumerate(want_more):
+        _close(eng.logits(i), logits)
+    # caches: the first layer's keys and values come from the same projection rows; a rotated
+    # key is rounded to bf16 once, after fp32 sums that may be contracted differently
+    for layer in range(3):
+        for row, n in ((4, 87), (0, 1), (2, 35), (5, 100)):
+            a = [torch.zeros(1, n, dkv, dtype=torch.bfloat16, device=dev) for _ in range(4)]
+            steps.get_kv(layer, row, 0, a[0], a[1])
+            eng.get_kv(layer, row, 0, a[2], a[3])
+            for x, y in ((a[0], a[2]), (a[1], a[3])):
+                diff = (x.float() - y.float()).abs()
+                if layer == 0:
+                    assert (diff <= x.float().abs() * 2.0 ** -7 + 1e-6).all()
+                else:
+                    assert diff.max() <= 0.05 * x.float().abs().max()
+    kept = [torch.zeros(1, 8, dkv, dtype=torch.bfloat16, device=dev) for _ in range(2)]
+    eng.get_kv(1, 3, 0, *kept)
+    assert torch.equal(kept[0], marks[0]) and torch.equal(kept[1], marks[1])
+    steps.close()
+    eng.close()
+
+
+@pytest.mark.gpu
+def test_full_chain_of_prompt_steps_and_draws(pkg, tmp_path):
+    """Prefill with drawn tokens, then sampled steps: every token is the draw from the logits
+    that the engine reports, and settings that leave one token give the greedy one."""
+    from gpt_oss_b200 import synth
+
+    cfg = dict(synth.MINI_MODEL, vocab_size=1200, n_layers=2)
+    eng = _engine(pkg, cfg, 9, tmp_path, 4, 48)
+    rng = np.random.default_rng(3)
+    prompts = [rng.integers(0, 1200, n, dtype=np.int32) for n in (20, 3, 41)]
+    greedy = eng.prefill(prompts, [0, 1, 3])
+    one = eng.prefill(prompts, [0, 1, 3], sampling=dict(u=rng.random(3), top_k=[1, 1, 1]))
+    assert (greedy == one).all()
+
+    def settings(n):
+        return dict(u=rng.random(n, dtype=np.float32), temperature=rng.uniform(0.3, 1.2, n).astype(np.float32),
+                    top_k=rng.integers(0, 60, n), top_p=rng.uniform(0.3, 1.0, n).astype(np.float32),
+                    min_p=rng.uniform(0.0, 0.1, n).astype(np.float32))
+
+    def check(rows, got, s):
+        for i, r in enumerate(rows):
+            f = lambda k: float(np.float64(np.float32(s[k][r])))  # noqa: E731
+            want, margin = _draw(eng.logits(r), f("u"), f("temperature"), int(s["top_k"][r]), f("top_p"), f("min_p"))
+            assert margin > 1e-11 and got[r] == want
+
+    s = settings(3)
+    nxt = eng.prefill(prompts, [0, 1, 3], sampling=s)
+    check([0, 1, 2], nxt, s)
+    where = {0: 20, 1: 3, 3: 41}
+    token = {0: nxt[0], 1: nxt[1], 3: nxt[2]}
+    for _ in range(4):
+        tok, pos = np.full(4, -1, np.int32), np.full(4, -1, np.int32)
+        for r in where:
+            tok[r], pos[r] = token[r], where[r]
+        s = settings(4)
+        out = eng.step(tok, pos, sampling=s)
+        assert out[2] == -1
+        check([0, 1, 3], out, s)
+        for r in where:
+            where[r] += 1
+            token[r] = out[r]
+    # the same step again, greedy: sampling leaves the plain step as it was
+    plain = eng.step(tok, pos)
+    assert all(plain[r] == eng.logits(r).argmax() for r in where)
+    assert (eng.step(tok, pos, sampling=dict(u=np.zeros(4), temperature=np.zeros(4))) == plain).all()
+    eng.close()
+
+
+@pytest.mark.gpu
+def test_refusals_change_nothing(pkg, tmp_path):
+    from gpt_oss_b200 import synth
+
+    cfg = dict(synth.MINI_MODEL, vocab_size=300, n_layers=1, seq_len=64)
+    eng = _engine(pkg, cfg, 2, tmp_path, 3, 16)
+    ok = np.arange(10, dtype=np.int32)
+    want = eng.prefill([ok], [1])
+    for args, code in (((([ok], [3])), pkg.GPTOSS_E_INVALID), ((([ok], [-1])), pkg.GPTOSS_E_INVALID),
+                       ((([ok, ok], [1, 1])), pkg.GPTOSS_E_INVALID),
+                       ((([ok, ok[:0]], [0, 1])), pkg.GPTOSS_E_INVALID),
+                       ((([ok], [1], [-1])), pkg.GPTOSS_E_INVALID),
+                       ((([ok], [1], [55])), pkg.GPTOSS_E_CAPACITY),
+                       ((([ok, ok, ok, ok], [0, 1, 2, 0])), pkg.GPTOSS_E_CAPACITY),
+                       ((([ok, np.array([5, 300])], [0, 1])), pkg.GPTOSS_E_INVALID),
+                       ((([np.array([-1])], [1])), pkg.GPTOSS_E_INVALID)):
+        with pytest.raises(pkg.MoeError) as ei:
+            eng.prefill(*args)
+        assert ei.value.code == code
+    with pytest.raises(pkg.MoeError, match="u"):
+        eng.prefill([ok], [1], sampling=dict(temperature=[1.0]))
+    with pytest.raises(ValueError, match="unknown"):
+        eng.prefill([ok], [1], sampling=dict(u=[0.5], topk=[1]))
+    with pytest.raises(ValueError, match="entries"):
+        eng.step(ok[:2], np.array([0, 1]), sampling=dict(u=[0.5]))
+    assert eng.prefill([], []).shape == (0,)
+    # the row still continues where it was: the next step gives what a fresh engine gives
+    tok, pos = np.array([-1, 7, -1], np.int32), np.array([-1, 10, -1], np.int32)
+    after = eng.step(tok, pos)[1]
+    other = _engine(pkg, cfg, 2, tmp_path, 3, 16)
+    assert (other.prefill([ok], [1]) == want).all() and other.step(tok, pos)[1] == after
+    eng.close()
+    other.close()
+
+
+def test_create_refuses_fewer_tokens_than_rows(pkg):
+    from gpt_oss_b200 import synth
+
+    with pytest.raises(pkg.MoeError) as ei:
+        pkg.DecodeEngine(synth.MINI_MODEL, 8, max_tokens=4)
+    assert ei.value.code == pkg.GPTOSS_E_INVALID
+    with pytest.raises(ValueError, match="local"):
+        pkg.DecodeEngine(synth.MINI_MODEL, 8, ep_size=2, max_tokens=64)
+
+
+def test_null_handles(pkg):
+    lib = pkg.load_library()
+    assert lib.gptoss_decode_prefill(None, None, None, None, None, 0, None, None, None) == pkg.GPTOSS_E_INVALID
+    assert lib.gptoss_decode_step_sample(None, None, None, 1, None, None, None) == pkg.GPTOSS_E_INVALID
