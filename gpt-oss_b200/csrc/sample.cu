@@ -43,7 +43,8 @@ constexpr int kSampleMaxSplit = 8;     // CTAs of a row
 constexpr int kSampleMaxVocab = 1 << 18;
 constexpr int kBins = 512;
 constexpr int kList = 1024;
-constexpr unsigned kAll = 0xffffffffu;        // no limit among equal logits
+constexpr unsigned kAll = 0xffffffffu;        // no limit among equal logits; no id
+constexpr uint32_t kKeyNegInf = 0x007fffffu;  // sample_key(-infinity)
 constexpr u64 kOne = 1ull << 44;              // weight of the likeliest token
 
 // Order-preserving bits of a logit (never NaN or -0 here).
@@ -55,7 +56,7 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 // NaN counts as -infinity, -0 as +0
-__device__ __forceinline__ float clean(float x) { return x == x ? x + 0.0f : -INFINITY; }
+__device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY) + 0.0f; }
 __device__ __forceinline__ float logit_at(const float *p) { return *p; }
 __device__ __forceinline__ float logit_at(const bf16 *p) { return __bfloat162float(*p); }
 __device__ __forceinline__ float logit_at(const __half *p) { return __half2float(*p); }
@@ -69,7 +70,9 @@ struct SampleShared {
   unsigned count[kBins];           // cluster reads: logits of a bin
   uint32_t list[kList];            // cluster reads: keys that the CTA contributes to a list
   u64 warp_sum[kSampleWarps];
-  u64 best;                        // cluster reads: key and ~id of the CTA's largest logit
+  float warp_max[kSampleWarps];
+  uint32_t best;                   // cluster reads: key of the CTA's largest logit
+  unsigned first;                  // cluster reads: lowest id of the largest logit
   u64 sum;                         // cluster reads: the CTA's weight
   unsigned listed[3];              // cluster reads: lengths of the CTA's lists
   unsigned equal;                  // cluster reads: logits equal to the edge in the CTA
@@ -197,16 +200,8 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
   constexpr int kVec = 16 / sizeof(T);
   const int head = min(n, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / static_cast<int>(sizeof(T)));
   float *slice = slice_mem + ((kVec - head) & 3);
-  float best = -INFINITY;
-  int best_id = 0x7fffffff;
-  auto keep = [&](int i, float v) {
-    slice[i] = v;
-    if (v > best) {  // a thread's ids ascend
-      best = v;
-      best_id = id0 + i;
-    }
-  };
-  if (tid < head) keep(tid, clean(logit_at(x + tid)));
+  float best = -INFINITY;  // of the logits that this thread loads
+  if (tid < head) best = slice[tid] = clean(logit_at(x + tid));
   const int vecs = (n - head) / kVec;
   const uint4 *xv = reinterpret_cast<const uint4 *>(x + head);
 #pragma unroll 4
@@ -221,39 +216,51 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
     for (int j = 0; j < kVec; j += 4)
       *reinterpret_cast<float4 *>(slice + i + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
 #pragma unroll
-    for (int j = 0; j < kVec; j++)
-      if (f[j] > best) {
-        best = f[j];
-        best_id = id0 + i + j;
-      }
+    for (int j = 0; j < kVec; j++) best = fmaxf(best, f[j]);
   }
-  for (int i = head + vecs * kVec + tid; i < n; i += kSampleThreads) keep(i, clean(logit_at(x + i)));
+  for (int i = head + vecs * kVec + tid; i < n; i += kSampleThreads) {
+    slice[i] = clean(logit_at(x + i));
+    best = fmaxf(best, slice[i]);
+  }
   {
-    u64 key = best_id == 0x7fffffff ? 0 : static_cast<u64>(sample_key(best)) << 32 | (0xffffffffu - best_id);
+    float all = best;
 #pragma unroll
-    for (int i = 16; i > 0; i >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, i));
-    if (lane == 0) s.warp_sum[tid >> 5] = key;
+    for (int i = 16; i > 0; i >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, i));
+    if (lane == 0) s.warp_max[tid >> 5] = all;
     __syncthreads();
     if (tid == 0) {
-      for (int w = 1; w < kSampleWarps; w++) key = max(key, s.warp_sum[w]);
-      s.best = key;
+      for (int w = 1; w < kSampleWarps; w++) all = fmaxf(all, s.warp_max[w]);
+      s.best = sample_key(all);
+      s.first = kAll;
     }
   }
   if (tid < 16) s.table[tid] = exp2(-tid / 16.0);
   if (tid < 3) s.listed[tid] = 0;
   for (int i = tid; i < kBins; i += kSampleThreads) s.mass[i] = s.count[i] = 0;
   sync();
-  u64 key = 0;
+  uint32_t key = 0;
 #pragma unroll
-  for (int c = 0; c < split; c++) key = max(key, split > 1 ? peer_u64(&s.best, c) : s.best);
+  for (int c = 0; c < split; c++) key = max(key, split > 1 ? peer_u32(&s.best, c) : s.best);
   const float temp = a.temperature ? a.temperature[row] : 1.0f;
-  const bool greedy = !(temp > 0.0f);
-  if (greedy || key == 0) {
-    if (rank == 0 && tid == 0) a.next[row] = key == 0 ? 0 : static_cast<int>(0xffffffffu - static_cast<uint32_t>(key));
-    if (split > 1) cluster_barrier_all();  // the others may still read s.best
+  if (!(temp > 0.0f) || key == kKeyNegInf) {
+    // greedy: the lowest id of the largest logit (-infinity everywhere: the first id)
+    const float want = key_value(key);
+    unsigned mine = kAll;
+    for (int i = tid; i < n && mine == kAll; i += kSampleThreads)
+      if (slice[i] == want) mine = id0 + i;
+    mine = __reduce_min_sync(0xffffffffu, mine);
+    if (lane == 0 && mine != kAll) atomicMin(&s.first, mine);
+    sync();
+    if (rank == 0 && tid == 0) {
+      unsigned id = kAll;
+#pragma unroll
+      for (int c = 0; c < split; c++) id = min(id, split > 1 ? peer_u32(&s.first, c) : s.first);
+      a.next[row] = static_cast<int>(id);
+    }
+    if (split > 1) cluster_barrier_all();  // nobody leaves while its shared memory is read
     return;
   }
-  float top = key_value(static_cast<uint32_t>(key >> 32));
+  float top = key_value(key);
   const double t = fmin(static_cast<double>(temp), 1e36);
   const double reach = 46 * 0.69314718055994530942 * t;
   const double scale = 16 * 1.44269504088896340736 / t;
@@ -291,9 +298,10 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
     // spread is what matters), the last one open; float arithmetic is monotonic, so bins
     // respect the order.  -infinity takes no part.
     const float to_bin = 16.0f * fmaxf(1.0f, static_cast<float>(1.0 / t));
-    auto bin_of = [&](float v) {
-      return v == top ? 0 : static_cast<int>(fminf((top - v) * to_bin, static_cast<float>(kBins - 1)));
+    auto place = [&](float v) {  // in bins
+      return v == top ? 0.0f : fminf((top - v) * to_bin, static_cast<float>(kBins - 1));
     };
+    auto bin_of = [&](float v) { return static_cast<int>(place(v)); };
     // 64-bit sums in shared memory as two 32-bit ones with a carry (6.3 a cycle and SM; the
     // 64-bit atomic manages 1.1)
     auto add_mass = [&](int b, u64 w) {
@@ -325,8 +333,17 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
     static_assert(kBins == kSampleThreads, "a thread per bin in the scans");
     unsigned my_count;
     u64 my_mass, count_before, mass_before, all_count, all_mass;
-    // Counts (and weights) of the bins, of the logits from `least` on.
-    auto histogram = [&](bool weights, float least) {
+    // Logits outside [low, high] are in none of the bins lo .. hi (bounds one bin wider).
+    auto bounds = [&](int lo, int hi, float floor_value, float *low, float *high) {
+      *low = fmaxf(floor_value, hi < kBins - 1 ? top - static_cast<float>(hi + 2) / to_bin * 1.0001f : -FLT_MAX);
+      *high = lo > 0 ? top - static_cast<float>(lo - 1) / to_bin * 0.9999f : INFINITY;
+      *low = fmaxf(*low, -FLT_MAX);
+    };
+    // Counts (and weights) of the bins, of the logits from `least` on; with bin >= 0 of that
+    // bin's logits alone, in kBins parts of it.
+    auto histogram = [&](bool weights, float least, int bin) {
+      float low = fmaxf(least, -FLT_MAX), high = INFINITY;
+      if (bin >= 0) bounds(bin, bin, least, &low, &high);
       for (int i0 = tid; i0 < n; i0 += 4 * kSampleThreads) {
         float v[4];
         bool in[4];
@@ -336,7 +353,7 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
         for (int j = 0; j < 4; j++) {
           const int i = i0 + j * kSampleThreads;
           v[j] = i < n ? slice[i] : -INFINITY;
-          in[j] = v[j] > -INFINITY && v[j] >= least;
+          in[j] = v[j] >= low && v[j] <= high;
           some |= in[j];
         }
         if (!some) continue;
@@ -346,17 +363,28 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
           for (int j = 0; j < 4; j++) w[j] -= Weigher::kBias;
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (in[j]) {
-            const int b = bin_of(v[j]);
-            atomicAdd(&s.count[b], 1u);
-            add_mass(b, w[j]);
+        for (int j = 0; j < 4; j++) {
+          if (!in[j]) continue;
+          const float p = place(v[j]);
+          int b = static_cast<int>(p);
+          if (bin >= 0) {
+            if (b != bin) continue;
+            b = static_cast<int>((p - static_cast<float>(bin)) * kBins);
           }
+          atomicAdd(&s.count[b], 1u);
+          add_mass(b, w[j]);
+        }
       }
       sync();
       gather(tid, weights, &my_count, &my_mass);
       all_count = block_scan(my_count, &count_before, s.warp_sum);
       all_mass = block_scan(my_mass, &mass_before, s.warp_sum);
+    };
+    // The arrays are cleared for another histogram once everyone has read them.
+    auto clear = [&]() {
+      sync();
+      s.mass[tid] = s.count[tid] = 0;
+      __syncthreads();
     };
 
     // How many of the `equal` logits of weight w have less than `limit` in front of them, with
@@ -370,14 +398,12 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
       return min(take, equal);
     };
     constexpr int kPer = kList / kSampleThreads;
-    // The row's logits in bins [lo, hi] and not below `floor_value`, as keys in s.merged, the
-    // largest first.  Returns their number; more than kList of them are not listed.
-    auto collect = [&](int which, int lo, int hi, float floor_value) -> unsigned {
-      // most logits lie far from the bins: a comparison with bounds one bin wider tells
-      float low = -FLT_MAX, high = INFINITY;
-      if (hi < kBins - 1) low = fmaxf(low, top - static_cast<float>(hi + 2) / to_bin * 1.0001f);
-      if (lo > 0) high = top - static_cast<float>(lo - 1) / to_bin * 0.9999f;
-      low = fmaxf(low, floor_value);
+    // The row's logits in bins [lo, hi] (part >= 0: in that part of the one bin) and not below
+    // `floor_value`, as keys in s.merged, the largest first.  Returns their number; more than kList of them are not listed.
+    auto collect = [&](int which, int lo, int hi, int part, float floor_value) -> unsigned {
+      // most logits lie far from the bins: a comparison tells
+      float low, high;
+      bounds(lo, hi, floor_value, &low, &high);
       for (int i0 = tid; i0 < n; i0 += 8 * kSampleThreads) {
         float v[8];
         bool some = false;
@@ -391,8 +417,10 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
           if (!(v[j] >= low && v[j] <= high)) continue;
-          const int b = bin_of(v[j]);
+          const float p = place(v[j]);
+          const int b = static_cast<int>(p);
           if (b < lo || b > hi) continue;
+          if (part >= 0 && static_cast<int>((p - static_cast<float>(b)) * kBins) != part) continue;
           const unsigned at = atomicAdd(&s.listed[which], 1u);
           if (at < kList) s.list[at] = sample_key(v[j]);
         }
@@ -490,12 +518,32 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
     auto search = [&](int which, bool weights, unsigned want, u64 acc, double limit) {
       const int bin = s.bin;
       const float floor_value = edge ? key_value(edge) : -INFINITY;
-      if (s.size <= kList) {
-        const unsigned size = collect(which, bin, bin, floor_value);
+      int part = -1;
+      if (s.size > kList && bin < kBins - 1) {
+        // many logits in the bin: the same once more, in parts of the bin
+        clear();
+        histogram(weights, floor_value, bin);
+        const bool here = limit < 0.0 ? count_before < want && want <= count_before + my_count
+                                      : static_cast<double>(acc + mass_before) < limit &&
+                                            static_cast<double>(acc + mass_before + my_mass) >= limit;
+        if (here) {
+          s.bin = tid;
+          s.size = my_count;
+          s.before = static_cast<unsigned>(count_before);
+          s.above = mass_before;
+        }
+        __syncthreads();
+        part = s.bin;
+        want -= limit < 0.0 ? s.before : 0u;
+        acc += s.above;
+      }
+      const unsigned in_part = s.size;
+      if (in_part <= kList) {
+        const unsigned size = collect(which, bin, bin, part, floor_value);
         choose(size, limit >= 0.0 ? size : want, acc, limit, -1.0);
         return;
       }
-      // many logits in the bin: by the digits of their bits
+      // still many (equal ones, or the open bin): by the digits of their bits
       uint32_t prefix = 0;
       u64 heavy = 0;
       for (int shift = 24; shift >= 0; shift -= 8) {
@@ -505,6 +553,7 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
         for (int i = tid; i < n; i += kSampleThreads) {
           const float v = slice[i];
           if (v == -INFINITY || v < floor_value || bin_of(v) != bin) continue;
+          if (part >= 0 && static_cast<int>((place(v) - static_cast<float>(bin)) * kBins) != part) continue;
           const uint32_t k = sample_key(v);
           if (shift < 24 && (k >> (shift + 8)) != (prefix >> (shift + 8))) continue;
           atomicAdd(&s.count[(k >> shift) & 255], 1u);
@@ -561,7 +610,7 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
       if (want <= all_count) {
         if (count_before < want && want <= count_before + my_count) s.bin = tid;
         __syncthreads();
-        const unsigned size = collect(0, 0, s.bin, -INFINITY);
+        const unsigned size = collect(0, 0, s.bin, -1, -INFINITY);
         if (size <= kList) {
           choose(size, top_k, 0, -1.0, by_mass ? fmax(static_cast<double>(top_p), 0.0) : -1.0);
           edge = s.edge;
@@ -579,7 +628,7 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
     }
     u64 dropped = 0;  // weight of the logits equal to the edge that top-k leaves out
     if (by_count && !done) {
-      histogram(false, -INFINITY);
+      histogram(false, -INFINITY, -1);
       const u64 want = top_k;
       if (want < all_count) {
         if (count_before < want && want <= count_before + my_count) {
@@ -593,14 +642,10 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
         need = s.need;
         dropped = (s.equals - s.take) * weigher(key_value(edge));
       }
-      if (by_mass) {  // the arrays are free once everyone has read them
-        sync();
-        s.mass[tid] = s.count[tid] = 0;
-        __syncthreads();
-      }
+      if (by_mass) clear();
     }
     if (by_mass && !done) {
-      histogram(true, edge ? key_value(edge) : -INFINITY);
+      histogram(true, edge ? key_value(edge) : -INFINITY, -1);
       const double limit = fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(all_mass - dropped);
       if (limit > 0.0) {
         // the bin in which the weight reaches the limit
