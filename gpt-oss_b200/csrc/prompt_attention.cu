@@ -3,28 +3,41 @@
 //
 //   o = sum_t p_t v_t / (sum_t p_t + 2^(sink' - m)),   p_t = 2^(c q.k_t - m),  c = scale log2 e
 //
-// A tile is 128 rows of one MMA: kTok = 128 / group query tokens times the `group` query heads
+// A tile is 128 rows of one MMA: tok = 128 / group query tokens times the `group` query heads
 // that share a KV head, so K and V are read once for the whole group and a sequence of a few
-// tokens still fills rows.  A job is two tiles (A and B, consecutive tokens) of one sequence and
-// KV head over the same stream of blocks of 128 keys.  CTAs are persistent, one per SM:
-//   warps 0-3, 4-7  softmax of tile A, of tile B: a thread owns a row (a TMEM lane)
-//   warp 8          TMA: Q of both tiles, then K and V blocks into two rings
-//   warps 9, 10     the MMAs of tile A and of tile B, S = Q K^T and O += P V
-//   warp 11         the jobs, a few ahead of the others
-// S comes from TMEM into registers whole (128 per thread), so the row maximum costs no second
-// read; P goes back to TMEM as the MMA's 16-bit row operand, V is read in place as an N-major
-// operand.  The maximum that scales a row is only moved when it grows by more than 8 (a factor
-// of 256; fp32 sums and 16-bit floating-point P lose nothing by that), so O is rarely rescaled
-// and the thread that owns the row does it itself.
+// tokens still fills rows.  A job is two tiles (consecutive tokens) of one sequence and KV head
+// over the same stream of units of KEYS keys.  One CTA per SM:
+//   warps 0-15   softmax, eight per tile: two warps share 32 rows, a thread has a row (a TMEM
+//                lane) and half of a unit's keys
+//   warp 16      the jobs (a CTA takes over the work of CTAs that have not started, longest
+//                jobs first), TMA: Q of both tiles, then K and V units into two rings
+//   warps 17, 18 the MMAs of either tile, S = Q K^T a unit ahead of O += P V
+// S comes from TMEM into registers whole, so the row maximum costs no second read, and S is
+// free for the next unit's scores while P is being made; P goes back to TMEM as the MMA's
+// 16-bit row operand, V is read in place as an N-major operand.  The maximum that scales a row
+// is only moved when it grows by more than 8 (a factor of 256; fp32 sums and 16-bit
+// floating-point P lose nothing by that), so O is rarely rescaled, and by its own softmax warps.
 //
-// What bounds it: an exponential per (row, key), 16 per cycle and SM, is 1024 cycles per tile
-// and block; the two MMAs take 256 each at head_dim 64 and 512 each at 128.  Two tiles keep
-// the exponentials going while the other tile's MMAs run; at head_dim <= 64 there is room in
-// TMEM for P beside S, and the next S is computed while P is still being made.
+// What bounds it: an exponential per (row, key), 16 per cycle and SM.  64 keys of both tiles
+// are 1024 cycles of exponentials against 256 of MMAs at head_dim 64 and 512 at 128; masking,
+// maximum, scaling, sum and packing are issued beside them.  A few of the exponentials are
+// therefore computed on the FMA pipes: one in 8 pairs at head_dim 64 with 128 keys (one prompt
+// of 8192 tokens, 64/8 heads: 662 us, 69 % of what the exponentials alone would take; 756 with
+// none, 790 with one in four), one in 16 at 128 (one prompt of 4096 tokens, 32/4 heads: 133 us, 1.03 PFLOP/s;
+// 143 with one in 8).  Handing S over earlier is slower (784 us): the late arrival keeps the two
+// tiles out of phase.
+//
+// KEYS: 128 where TMEM holds S, P and O of both tiles (head_dim <= 64), 64 at 128.  A narrow
+// window leaves most of a unit of 128 masked, so 64 are taken there too.  Time with 64 and 128
+// keys of 10 packed prompts (13626 tokens), 64/8 heads of 64, by window: 128 tokens 127 and 150 us, 256 166 and
+// 176, 512 228 and 229, 1024 330 and 301, 2048 474 and 420.
 //
 // Few tiles and long contexts: a cluster of up to 8 CTAs shares one pair of tiles, each taking
-// an equal run of key blocks; the partial (m, l, O) are joined through distributed shared
-// memory, in rank order, so the result does not depend on timing and no workspace is needed.
+// an equal run of units; the partial (m, l, O) are joined through distributed shared memory, in
+// rank order, so the result does not depend on timing and no workspace is needed.  Only as far
+// as SMs would be idle otherwise: a cluster waits until that many SMs are free at once, and
+// four packed pieces of prompts (3690 tokens, 32/4 heads of 128, contexts up to 16130) took 264
+// us with whole jobs, 309 with every job in two parts and 471 in four.
 //
 // Probabilities are rounded to the 16-bit type for the second product (tensor cores take both
 // operands in one type); their sum is taken in fp32 before that rounding.
@@ -40,29 +53,27 @@ namespace gptoss {
 
 constexpr int kAttnThreads = 640;
 constexpr int kAttnSoftmaxWarps = 16;
-constexpr int kKeys = 128;            // keys per unit
 constexpr int kAttnTmemCols = 512;
 constexpr int kAttnMaxSplit = 8;      // CTAs of a cluster that share a pair of tiles
+constexpr int kAttnNarrow = 512;      // widest window that takes units of 64 keys at head_dim <= 64
 constexpr int kJobs = 4;              // jobs that may be at work in different warps
 
-template <int D>
+template <int D, int KEYS>
 struct AttnShape {
   static constexpr int kBox = D < 64 ? D : 64;            // elements of one swizzled row
   static constexpr int kPanels = D / kBox;                // 64-wide panels of a head
   static constexpr int kQPanelBytes = 128 * kBox * 2;
-  static constexpr int kPanelBytes = kKeys * kBox * 2;    // a panel of K or V
+  static constexpr int kPanelBytes = KEYS * kBox * 2;     // a panel of K or V
   static constexpr int kQBytes = kPanels * kQPanelBytes;
   static constexpr int kUnitBytes = kPanels * kPanelBytes;
-  static constexpr int kStages = D == 128 ? 2 : 4;        // units of K and of V in flight
+  static constexpr int kStages = 4;                       // units of K and of V in flight
   static constexpr int kRingBytes = kStages * kUnitBytes;
-  // TMEM: S of tile x at column 128 x.  P beside S (2 x 64 columns, then O 2 x D), or in the
-  // place of the S that it was made from.
-  static constexpr bool kApart = D <= 64;
-  static constexpr int kIssuers = kApart ? 2 : 1;         // warps that issue MMAs
-  static constexpr int kColP = kApart ? 256 : 0;
-  static constexpr int kStrideP = kApart ? 64 : 128;
-  static constexpr int kColO = kApart ? 384 : 256;
-  static constexpr int kStrideO = kApart ? 64 : 128;
+  // TMEM columns: S of both tiles (KEYS each), P of both (KEYS / 2), O of both (D)
+  static constexpr int kColP = 2 * KEYS;
+  static constexpr int kColO = D == 128 ? 256 : 384;
+  static_assert(3 * KEYS <= kColO && kColO + 2 * D <= kAttnTmemCols, "TMEM");
+  // every kPolyStep-th pair of exponentials is computed on the FMA pipes
+  static constexpr int kPolyStep = D == 128 ? 16 : KEYS == 64 ? 6 : 8;
   static constexpr int kOperandBytes = 2 * kQBytes + 2 * kRingBytes;
   // fp32 partial outputs of both tiles take the operands' place in a split launch
   static constexpr int kSmemBytes = 1024 + (kOperandBytes > 256 * D * 4 ? kOperandBytes : 256 * D * 4);
@@ -171,9 +182,9 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volati
 // matching swizzle: groups of 8 rows are 8 * row bytes apart.  For an operand read along its
 // rows (K major) the leading offset is unused; for one read across them (V: N major) it is the
 // distance of the 64-wide panels.
-template <int D>
+template <int D, int KEYS>
 __device__ __forceinline__ uint64_t attn_desc(uint32_t addr) {
-  typedef AttnShape<D> S;
+  typedef AttnShape<D, KEYS> S;
   uint64_t d = 0;
   d |= static_cast<uint64_t>((addr & 0x3ffff) >> 4);
   d |= static_cast<uint64_t>(S::kPanels > 1 ? S::kPanelBytes >> 4 : 1) << 16;
@@ -194,12 +205,13 @@ __device__ __forceinline__ uint32_t part_offset(int row, int piece) {
   return static_cast<uint32_t>((row * (D / 4) + (piece ^ (row & 7))) * 16);
 }
 // The job of a slot (a pair of tiles) and KV head, for this CTA's share of the keys.
+template <int KEYS>
 __device__ bool attn_find_job(const gptoss_attention_args_t &a, int tok, int slot, int kvh, int rank,
                               int split, int lane, AttnJob *job) {
   AttnRows r;
   if (!attn_find_rows(a, 2 * tok, slot, lane, &r)) return false;
   if (lane != 0) return true;
-  const int units = (r.keys + kKeys - 1) / kKeys;
+  const int units = (r.keys + KEYS - 1) / KEYS;
   job->kvh = kvh;
   job->q_row0 = r.q_row0;
   job->kv_row0 = static_cast<int>(r.kv_row0);
@@ -216,8 +228,8 @@ __device__ bool attn_find_job(const gptoss_attention_args_t &a, int tok, int slo
     const long long p = static_cast<long long>(r.first_pos) + x * tok;
     const long long from = a.window > 0 ? max(0ll, p - a.window + 1) : 0;
     const long long to = p + n;  // may be <= 0
-    const int b = static_cast<int>(from / kKeys);
-    const int e = to > 0 ? static_cast<int>((to + kKeys - 1) / kKeys) : 0;
+    const int b = static_cast<int>(from / KEYS);
+    const int e = to > 0 ? static_cast<int>((to + KEYS - 1) / KEYS) : 0;
     job->begin[x] = max(b, job->unit0);
     job->end[x] = max(job->begin[x], min(e, job->unit1));
   }
@@ -267,13 +279,13 @@ struct Ring {
   }
 };
 
-template <typename T, int D>
+template <typename T, int D, int KEYS>
 __global__ void __launch_bounds__(kAttnThreads, 1)
 prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
                         const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, const gptoss_attention_args_t a,
                         int group, int tok, int n_slots, int split) {
-  typedef AttnShape<D> S;
+  typedef AttnShape<D, KEYS> S;
   constexpr bool kHalf = !std::is_same<T, bf16>::value;
   extern __shared__ unsigned char smem_raw[];
   __shared__ AttnBarriers bar;
@@ -302,7 +314,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
   } else if (threadIdx.x == 0) {
     for (int j = 0; j < kJobs; j++) {
       mbar_init(&bar.job_full[j], 1);
-      mbar_init(&bar.job_empty[j], kAttnSoftmaxWarps + S::kIssuers);
+      mbar_init(&bar.job_empty[j], kAttnSoftmaxWarps + 2);
     }
     mbar_init(&bar.steal, 1);
     mbar_init(&bar.v_tail, 1);
@@ -316,9 +328,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
     }
     for (int s = 0; s < S::kStages; s++) {
       mbar_init(&bar.k_full[s], 1);
-      mbar_init(&bar.k_empty[s], S::kIssuers);
+      mbar_init(&bar.k_empty[s], 2);
       mbar_init(&bar.v_full[s], 1);
-      mbar_init(&bar.v_empty[s], S::kIssuers);
+      mbar_init(&bar.v_empty[s], 2);
     }
     abort_word = 0;
     mbar_fence_init();
@@ -381,7 +393,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
         while (ok && have && !found) {
           // the last slots first: a long prompt's last tiles see the most keys
           const uint32_t up = pair / a.n_kv_heads;
-          found = attn_find_job(a, tok, n_slots - 1 - static_cast<int>(up),
+          found = attn_find_job<KEYS>(a, tok, n_slots - 1 - static_cast<int>(up),
                                 static_cast<int>(pair - up * a.n_kv_heads), rank, split, lane, &job);
           if (!found) {
             ask();
@@ -409,8 +421,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
         load_q(0);
         const int unit0 = job.unit0, unit1 = job.unit1;
         for (int u = unit0; ok && u < unit1; u++) {
-          const int rel = u * kKeys;
-          const bool tail = rel + kKeys > job.keys;
+          const int rel = u * KEYS;
+          const bool tail = rel + KEYS > job.keys;
           unsigned char *k = sm_k + ring.slot * S::kUnitBytes, *v = sm_v + ring.slot * S::kUnitBytes;
           ok = warp_wait(&bar.k_empty[ring.slot], ring.phase ^ 1u, abort_flag);
           if (ok && elect_one()) {
@@ -437,7 +449,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
             tail_phase ^= 1u;
             constexpr int kRowChunks = S::kBox * 2 / 16;
             for (int p = 0; ok && p < S::kPanels; p++)
-              for (int c = (job.keys - rel) * kRowChunks + lane; c < kKeys * kRowChunks; c += 32)
+              for (int c = (job.keys - rel) * kRowChunks + lane; c < KEYS * kRowChunks; c += 32)
                 *reinterpret_cast<uint4 *>(v + p * S::kPanelBytes + c * 16) = make_uint4(0, 0, 0, 0);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -448,116 +460,80 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
         ask();
         answer();
       }
-    } else if (warp < 17 + S::kIssuers) {
+    } else if (warp < 19) {
       // -------------------------------------------------------------- MMAs
-      // With P beside S a warp per tile issues; the tiles then never wait for each other.  With
-      // P in S's place a tile's next scores follow its values, the MMAs are on the tile's
-      // critical path, and one warp keeps the two tiles' batches apart (interleaved they would
-      // both take twice as long and the exponentials would wait for both).
+      // A warp per tile issues; the tiles never wait for each other's softmax.
       code = kStatusWaitTimeoutMma;
-      constexpr uint32_t idesc_s = attn_idesc(kHalf, kKeys, false);
+      constexpr uint32_t idesc_s = attn_idesc(kHalf, KEYS, false);
       constexpr uint32_t idesc_o = attn_idesc(kHalf, D, true);
-      const uint64_t desc_q = attn_desc<D>(smem_u32(sm_q));
-      const uint64_t desc_k = attn_desc<D>(smem_u32(sm_k));
-      const uint64_t desc_v = attn_desc<D>(smem_u32(sm_v));
+      const uint64_t desc_q = attn_desc<D, KEYS>(smem_u32(sm_q));
+      const uint64_t desc_k = attn_desc<D, KEYS>(smem_u32(sm_k));
+      const uint64_t desc_v = attn_desc<D, KEYS>(smem_u32(sm_v));
       Ring<S::kStages> kr, vr;
-      struct Tile {
-        int x, begin, end;
-        uint32_t q_phase, free_phase, p_phase;
-      };
-      auto scores = [&](Tile &t, int u, bool last_reader) {  // S = Q K_u^T
-        ok = ok && warp_wait(&bar.k_full[kr.slot], kr.phase, abort_flag);
-        const bool active = u >= t.begin && u < t.end;
-        if (active) {
-          if (u == t.begin) {
-            ok = ok && warp_wait(&bar.q_full[t.x], t.q_phase, abort_flag);
-            t.q_phase ^= 1u;
-          }
-          // S is free again once its readers have it in registers; where P takes its place, the
-          // product that read that P was issued before (one warp's products run in order)
-          if (S::kApart) {
-            ok = ok && warp_wait(&bar.s_free[t.x], t.free_phase, abort_flag);
-            t.free_phase ^= 1u;
-          }
-          tc_fence_after();
-        }
-        if (ok && elect_one()) {
-          if (active) {
-            const uint64_t dq = desc_q + (t.x * S::kQBytes >> 4);
-            const uint64_t dk = desc_k + (kr.slot * S::kUnitBytes >> 4);
-#pragma unroll
-            for (int k = 0; k < D / 16; k++) {
-              constexpr int kPerPanel = S::kBox / 16;
-              umma_bf16(tmem + t.x * 128,
-                        dq + (((k / kPerPanel) * S::kQPanelBytes + (k % kPerPanel) * 32) >> 4),
-                        dk + (((k / kPerPanel) * S::kPanelBytes + (k % kPerPanel) * 32) >> 4),
-                        idesc_s, k != 0);
-            }
-            umma_commit(&bar.s_full[t.x]);
-            if (u == t.end - 1) umma_commit(&bar.q_empty[t.x]);
-          }
-          if (last_reader) umma_commit(&bar.k_empty[kr.slot]);
-        }
-        __syncwarp();
-      };
-      auto values = [&](Tile &t, int u, bool last_reader) {  // O += P V_u
-        ok = ok && warp_wait(&bar.v_full[vr.slot], vr.phase, abort_flag);
-        const bool active = u >= t.begin && u < t.end;
-        if (active) {
-          ok = ok && warp_wait(&bar.p_full[t.x], t.p_phase, abort_flag);
-          t.p_phase ^= 1u;
-          tc_fence_after();
-        }
-        if (ok && elect_one()) {
-          if (active) {
-            const uint64_t dv = desc_v + (vr.slot * S::kUnitBytes >> 4);
-#pragma unroll
-            for (int k = 0; k < kKeys / 16; k++)
-              umma_ta(tmem + S::kColO + t.x * S::kStrideO, tmem + S::kColP + t.x * S::kStrideP + k * 8,
-                      dv + ((k * 16 * S::kBox * 2) >> 4), idesc_o, k != 0 ? 1u : (u > t.begin ? 1u : 0u));
-          }
-          if (last_reader) umma_commit(&bar.v_empty[vr.slot]);
-          // last: who has waited for it has waited for everything before it
-          if (active) umma_commit(&bar.o_full[t.x]);
-        }
-        __syncwarp();
-      };
-      Tile t0 = {S::kApart ? warp - 17 : 0, 0, 0, 0u, 1u, 0u}, t1 = {1, 0, 0, 0u, 1u, 0u};
+      const int x = warp - 17;
+      const uint64_t dq = desc_q + (x * S::kQBytes >> 4);
+      uint32_t q_phase = 0, free_phase = 1, p_phase = 0;
       for (; have_job(); done_job()) {
         const AttnJob &job = jobs[jr.slot];
-        const int unit0 = job.unit0, unit1 = job.unit1;
-        t0.begin = job.begin[t0.x];
-        t0.end = job.end[t0.x];
-        t1.begin = job.begin[1];
-        t1.end = job.end[1];
-        if (S::kApart) {
-          for (int u = unit0; ok && u <= unit1; u++) {
-            if (u < unit1) {
-              scores(t0, u, true);
-              kr.next();
+        const int begin = job.begin[x], end = job.end[x], unit0 = job.unit0, unit1 = job.unit1;
+        auto scores = [&](int u) {  // S = Q K_u^T
+          ok = ok && warp_wait(&bar.k_full[kr.slot], kr.phase, abort_flag);
+          const bool active = u >= begin && u < end;
+          if (active) {
+            if (u == begin) {
+              ok = ok && warp_wait(&bar.q_full[x], q_phase, abort_flag);
+              q_phase ^= 1u;
             }
-            if (u > unit0) {
-              values(t0, u - 1, true);
-              vr.next();
+            // free once its readers have the last S in registers
+            ok = ok && warp_wait(&bar.s_free[x], free_phase, abort_flag);
+            free_phase ^= 1u;
+            tc_fence_after();
+          }
+          if (ok && elect_one()) {
+            if (active) {
+              const uint64_t dk = desc_k + (kr.slot * S::kUnitBytes >> 4);
+#pragma unroll
+              for (int k = 0; k < D / 16; k++) {
+                constexpr int kPerPanel = S::kBox / 16;
+                umma_bf16(tmem + x * KEYS,
+                          dq + (((k / kPerPanel) * S::kQPanelBytes + (k % kPerPanel) * 32) >> 4),
+                          dk + (((k / kPerPanel) * S::kPanelBytes + (k % kPerPanel) * 32) >> 4),
+                          idesc_s, k != 0);
+              }
+              umma_commit(&bar.s_full[x]);
+              if (u == end - 1) umma_commit(&bar.q_empty[x]);
             }
+            umma_commit(&bar.k_empty[kr.slot]);
           }
-        } else {
-          if (unit0 < unit1) {
-            scores(t0, unit0, false);
-            scores(t1, unit0, true);
-            kr.next();
+          __syncwarp();
+          kr.next();
+        };
+        auto values = [&](int u) {  // O += P V_u
+          ok = ok && warp_wait(&bar.v_full[vr.slot], vr.phase, abort_flag);
+          const bool active = u >= begin && u < end;
+          if (active) {
+            ok = ok && warp_wait(&bar.p_full[x], p_phase, abort_flag);
+            p_phase ^= 1u;
+            tc_fence_after();
           }
-          for (int u = unit0; ok && u < unit1; u++) {
-            const bool more = u + 1 < unit1;
-            values(t0, u, false);
-            if (more) scores(t0, u + 1, false);
-            values(t1, u, true);
-            if (more) {
-              scores(t1, u + 1, true);
-              kr.next();
+          if (ok && elect_one()) {
+            if (active) {
+              const uint64_t dv = desc_v + (vr.slot * S::kUnitBytes >> 4);
+#pragma unroll
+              for (int k = 0; k < KEYS / 16; k++)
+                umma_ta(tmem + S::kColO + x * D, tmem + S::kColP + x * (KEYS / 2) + k * 8,
+                        dv + ((k * 16 * S::kBox * 2) >> 4), idesc_o, k != 0 ? 1u : (u > begin ? 1u : 0u));
             }
-            vr.next();
+            umma_commit(&bar.v_empty[vr.slot]);
+            // last: who has waited for it has waited for everything before it
+            if (active) umma_commit(&bar.o_full[x]);
           }
+          __syncwarp();
+          vr.next();
+        };
+        for (int u = unit0; ok && u <= unit1; u++) {  // the scores a unit ahead of the values
+          if (u < unit1) scores(u);
+          if (u > unit0) values(u - 1);
         }
       }
     }
@@ -565,14 +541,15 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
     // ---------------------------------------------------------------- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     code = kStatusWaitTimeoutEpilogue;
-    // two warps per 32 rows: a thread has a row and 64 of a unit's 128 keys
+    // two warps per 32 rows: a thread has a row and half of a unit's keys
+    constexpr int kMine = KEYS / 2, kParts = kMine / 32;
     const int x = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const int row_tok = row / group;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t col_s = tmem + lanes + x * 128 + half * 64;
-    const uint32_t col_p = tmem + lanes + S::kColP + x * S::kStrideP + half * 32;
-    const uint32_t col_o = tmem + lanes + S::kColO + x * S::kStrideO + half * (D / 2);
+    const uint32_t col_s = tmem + lanes + x * KEYS + half * kMine;
+    const uint32_t col_p = tmem + lanes + S::kColP + x * (KEYS / 2) + half * (kMine / 2);
+    const uint32_t col_o = tmem + lanes + S::kColO + x * D + half * (D / 2);
     const float c = a.scale * kLog2e;
     uint32_t s_phase = 0, o_phase = 0, parity = 0;
     // Hands over a value of the thread's row and returns that of the thread with the row's other
@@ -604,20 +581,20 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
         s_phase ^= 1u;
         if (!ok) break;
         tc_fence_after();
-        uint32_t s[2][32], p[2][16];
+        uint32_t s[kParts][32], p[kParts][16];
         if (warp_live) {
-          tmem_ld32(col_s, s[0]);
-          tmem_ld32(col_s + 32, s[1]);
-          tmem_ld_wait32(s[0]);
-          tmem_ld_wait32(s[1]);
+#pragma unroll
+          for (int q = 0; q < kParts; q++) tmem_ld32(col_s + 32 * q, s[q]);
+#pragma unroll
+          for (int q = 0; q < kParts; q++) tmem_ld_wait32(s[q]);
         }
         float scale_o = 1.f;
         if (warp_live) {
-          const int key0 = (begin + i) * kKeys + half * 64;
-          if (key0 + 63 > last_min || key0 < first_max) {
+          const int key0 = (begin + i) * KEYS + half * kMine;
+          if (key0 + kMine - 1 > last_min || key0 < first_max) {
             // one bit per key, so that a key costs a bit test and a select
 #pragma unroll
-            for (int q = 0; q < 2; q++) {
+            for (int q = 0; q < kParts; q++) {
               const int lo = first - key0 - 32 * q, hi = last - key0 - 32 * q;
               const uint32_t from = lo <= 0 ? 0xffffffffu : (lo > 31 ? 0u : 0xffffffffu << lo);
               const uint32_t upto = hi >= 31 ? 0xffffffffu : (hi < 0 ? 0u : (2u << hi) - 1u);
@@ -627,21 +604,22 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
                 if (!(seen & (1u << e))) s[q][e] = 0xff800000u;
             }
           }
-          float mx[4];
+          float mx[2 * kParts];
 #pragma unroll
-          for (int q = 0; q < 4; q++) {
+          for (int q = 0; q < 2 * kParts; q++) {
             const uint32_t *v = &s[q >> 1][(q & 1) * 16];
             mx[q] = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
 #pragma unroll
             for (int e = 2; e < 16; e += 2)
               mx[q] = max3(mx[q], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
           }
-          float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+          float top = fmaxf(mx[0], mx[1]);
+          if (kParts > 1) top = fmaxf(top, fmaxf(mx[2 * kParts - 2], mx[2 * kParts - 1]));
+          top *= c;
           top = fmaxf(top, both(top));
-          if (S::kApart) {  // (the barrier in `both` has seen every lane's S in registers)
-            tc_fence_before();
-            if (lane == 0) mbar_arrive(&bar.s_free[x]);
-          }
+          // (the barrier in `both` has seen every lane's S in registers)
+          tc_fence_before();
+          if (lane == 0) mbar_arrive(&bar.s_free[x]);
           if (top > m + 8.f) {
             scale_o = fast_exp2(m - top);
             l *= scale_o;
@@ -651,13 +629,12 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
           const uint64_t c2 = f32x2(c, c), base2 = f32x2(-base, -base);
           uint64_t sum = 0;
 #pragma unroll
-          for (int q = 0; q < 2; q++)
+          for (int q = 0; q < kParts; q++)
 #pragma unroll
             for (int e = 0; e < 16; e++) {
               float2 y = f32x2_parts(f32x2_fma(
                   f32x2(__uint_as_float(s[q][2 * e]), __uint_as_float(s[q][2 * e + 1])), c2, base2));
-              // an eighth of the exponentials on the FMA pipes (see poly_exp2)
-              if (e % 8 == 1)
+              if (e % S::kPolyStep == S::kPolyStep - 1)
                 y = poly_exp2<kHalf ? 4 : 3>(y);
               else
                 y = make_float2(fast_exp2(y.x), fast_exp2(y.y));
@@ -667,7 +644,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
           const float2 sums = f32x2_parts(sum);
           l += sums.x + sums.y;
         }
-        if (S::kApart && !warp_live && lane == 0) mbar_arrive(&bar.s_free[x]);
+        if (!warp_live && lane == 0) mbar_arrive(&bar.s_free[x]);
         if (i > 0) {  // the product of the unit before has read P and written O
           ok = warp_wait(&bar.o_full[x], o_phase, abort_flag);
           o_phase ^= 1u;
@@ -686,8 +663,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
               tmem_st16(col_o + d, o);
             }
           }
-          tmem_st16(col_p, p[0]);
-          tmem_st16(col_p + 16, p[1]);
+#pragma unroll
+          for (int q = 0; q < kParts; q++) tmem_st16(col_p + 16 * q, p[q]);
           tmem_st_wait();
         }
         tc_fence_before();
@@ -763,8 +740,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
     const int x = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     if (quarter * 32 < part_rows) {
-      const uint32_t col_o = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + S::kColO +
-                             x * S::kStrideO + half * (D / 2);
+      const uint32_t col_o = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + S::kColO + x * D + half * (D / 2);
       if (half == 0) {
         part_m[x * 128 + row] = m;
         part_l[x * 128 + row] = l;
@@ -836,9 +812,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int KEYS>
 static int attention_launch(const gptoss_attention_args_t &a, int sms, cudaStream_t st) {
-  typedef AttnShape<D> S;
+  typedef AttnShape<D, KEYS> S;
   const int group = a.n_q_heads / a.n_kv_heads, tok = 128 / group;
   const long long slots = a.n_tokens / (2 * tok) + static_cast<long long>(a.n_seqs);
   if (slots > INT32_MAX) return decode_error(GPTOSS_E_CAPACITY, "prompt_attention: too many rows and sequences");
@@ -850,20 +826,20 @@ static int attention_launch(const gptoss_attention_args_t &a, int sms, cudaStrea
   const uint64_t rows = a.n_kv_rows ? a.n_kv_rows : 1;
   int rc = make_tmap_rows(&map_q, a.q, fp16, D, a.n_q_heads, a.n_tokens, a.q_stride, S::kBox, group,
                           tok, &err);
-  if (!rc) rc = make_tmap_rows(&map_k, k, fp16, D, a.n_kv_heads, rows, a.k_stride, S::kBox, 1, kKeys, &err);
-  if (!rc) rc = make_tmap_rows(&map_v, v, fp16, D, a.n_kv_heads, rows, a.v_stride, S::kBox, 1, kKeys, &err);
+  if (!rc) rc = make_tmap_rows(&map_k, k, fp16, D, a.n_kv_heads, rows, a.k_stride, S::kBox, 1, KEYS, &err);
+  if (!rc) rc = make_tmap_rows(&map_v, v, fp16, D, a.n_kv_heads, rows, a.v_stride, S::kBox, 1, KEYS, &err);
   if (rc) return decode_error(rc, "prompt_attention: %s", err.c_str());
   // Split the keys of a pair of tiles over a cluster while that leaves every CTA an SM of its
-  // own and at least two blocks.
+  // own and at least 256 keys.
   long long most = a.max_kv_len > 0 ? a.max_kv_len : INT32_MAX;
   if (a.window > 0) most = std::min(most, static_cast<long long>(a.window) + 2 * tok);
-  const long long blocks = (most + kKeys - 1) / kKeys;
+  const long long blocks = (most + 127) / 128;
   int split = 1;
   while (split < kAttnMaxSplit && slots * a.n_kv_heads * split * 2 <= sms && blocks >= 4 * split) split *= 2;
   const long long units = slots * a.n_kv_heads;
   const long long grid = units * split;
   if (grid > INT32_MAX) return decode_error(GPTOSS_E_CAPACITY, "prompt_attention: too many rows for one launch");
-  auto kernel = prompt_attention_kernel<T, D>;
+  auto kernel = prompt_attention_kernel<T, D, KEYS>;
   // the kernel's warps share out the registers of a launch with 96 each: with fewer they would
   // wait for more for ever
   cudaFuncAttributes fa = {};
@@ -889,7 +865,9 @@ static int attention_launch(const gptoss_attention_args_t &a, int sms, cudaStrea
 }
 
 // Few query rows per sequence go to the kernel of token_attention.cu: when a sequence has on
-// average at most the tokens that fill 16 rows.
+// average at most the tokens that fill 16 rows, one job there.  (64/8 heads of 64: one token each
+// of 64 sequences with up to 7747 keys 160 us here and 100 there, one of 131071 keys 150 and 59.
+// With more tokens a sequence that kernel reads its K and V once for every 16 rows.)
 static bool rows_are_few(const gptoss_attention_args_t &a) {
   const int group = a.n_q_heads / a.n_kv_heads;
   return group <= 16 && a.n_tokens <= static_cast<long long>(a.n_seqs) * (16 / group);
@@ -897,9 +875,11 @@ static bool rows_are_few(const gptoss_attention_args_t &a) {
 
 template <typename T>
 static int attention_for(const gptoss_attention_args_t &a, int sms, cudaStream_t st) {
-  if (a.head_dim == 32) return attention_launch<T, 32>(a, sms, st);
-  if (a.head_dim == 64) return attention_launch<T, 64>(a, sms, st);
-  return attention_launch<T, 128>(a, sms, st);
+  if (a.head_dim == 128) return attention_launch<T, 128, 64>(a, sms, st);
+  const bool narrow = a.window > 0 && a.window <= kAttnNarrow;
+  if (a.head_dim == 32)
+    return narrow ? attention_launch<T, 32, 64>(a, sms, st) : attention_launch<T, 32, 128>(a, sms, st);
+  return narrow ? attention_launch<T, 64, 64>(a, sms, st) : attention_launch<T, 64, 128>(a, sms, st);
 }
 
 }  // namespace gptoss
@@ -929,8 +909,8 @@ extern "C" int gptoss_decode_prompt_attention(const gptoss_attention_args_t *arg
   auto bad = [](long long stride) { return stride % 8 != 0 || stride >= (1ll << 38); };
   if (bad(a.q_stride) || bad(a.k_stride) || bad(a.v_stride) || bad(a.out_stride))
     return decode_error(GPTOSS_E_INVALID, "prompt_attention: row strides must be multiples of 8 elements");
-  // row coordinates of the copies, a block past the last row included, are 32-bit
-  if (a.n_kv_rows > INT32_MAX - 2 * kKeys)
+  // row coordinates of the copies, a unit past the last row included, are 32-bit
+  if (a.n_kv_rows > INT32_MAX - 256)
     return decode_error(GPTOSS_E_CAPACITY, "prompt_attention: more than 2^31 - 257 K / V rows");
   if (a.n_tokens == 0 || a.n_seqs == 0) return GPTOSS_OK;
   if (!a.q || !a.out || !a.q_start || !a.kv_start || !a.kv_len || (a.n_kv_rows > 0 && (!a.k || !a.v)))

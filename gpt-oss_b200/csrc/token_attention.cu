@@ -10,8 +10,14 @@
 // CTAs' through distributed shared memory, always in the same order.
 //
 // The tcgen05 kernel of prompt_attention.cu needs 128 rows per tile and several hand-shakes per
-// block of keys; on 8 rows its warps wait for each other most of the time (one token of
-// 131071 keys, 64/8 heads of 64: 145 us there).
+// block of keys; on 8 rows its warps wait for each other most of the time.
+//
+// What bounds it: the read of K and V.  One token each of 64 sequences with 1 to 7747 keys, 64/8
+// heads of 64: 100 us, 77 % of a copy's rate (the last jobs run alone); one token of 131071
+// keys: 59 us, 69 % (its 8 clusters of 16 CTAs are 128 CTAs, two to an SM, and leave SMs idle).
+// Three blocks are in flight per warp: with two the long token takes 86 us instead of 74 (both
+// with a graph launch), with four an SM holds fewer CTAs (256 sequences of 512 keys: 102 instead
+// of 74).  Clusters of 8 take 88 us for the long token.
 #include <algorithm>
 #include <type_traits>
 
