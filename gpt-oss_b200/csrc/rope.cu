@@ -198,8 +198,8 @@ template <typename T, int V>
 static void rope_launch(const gptoss_rope_args_t &a, int sms, cudaStream_t st) {
   // rows per CTA: enough CTAs for two waves before a CTA takes more rows
   int rows_per_cta = 1;
-  while (rows_per_cta < kRopeRows && a.n_rows >= 4 * rows_per_cta * sms) rows_per_cta *= 2;
-  const int grid = (a.n_rows + rows_per_cta - 1) / rows_per_cta;
+  while (rows_per_cta < kRopeRows && a.n_rows / (4 * rows_per_cta) >= sms) rows_per_cta *= 2;
+  const int grid = (a.n_rows - 1) / rows_per_cta + 1;
   // threads: the items of a row in as few equal passes as fit
   const int most = a.interleaved ? 384 : 256;
   const int unit = a.interleaved ? (V < 2 ? 2 : V) : 2 * V;
