@@ -59,19 +59,41 @@ struct AttnRows {
 
 // Slots: a slot covers `span` tokens; sequence i's slots start at q_start[i] / span + i, which
 // leaves room for a partial slot per sequence and needs no prefix sum.  One warp finds the
-// slot's sequence by counting the starts at or before it.  Returns (warp-uniform, all lanes
-// get the rows) whether there is anything to do for the slot.
+// slot's sequence by counting the starts at or before it, 128 of them at a time: among more
+// sequences every 128th part is looked at first.  The slots (of all KV heads) together check
+// every entry of q_start, 32 each; starts that do not ascend give some sequence or none, never
+// rows outside the tensors.  Returns (warp-uniform, all lanes get the rows) whether there is
+// anything to do for the slot.
 __device__ __forceinline__ bool attn_find_rows(const gptoss_attention_args_t &a, int span, int slot,
-                                               int lane, AttnRows *rows) {
-  int below = 0, broken = 0;
-#pragma unroll 4
-  for (int i = lane; i < a.n_seqs; i += 32) {
-    const int q0 = __ldg(a.q_start + i), q1 = __ldg(a.q_start + i + 1);
-    broken |= q0 < 0 || q1 < q0 || q1 > a.n_tokens;
-    below += q0 / span + i <= slot;
+                                               int kvh, int lane, AttnRows *rows) {
+  const long long mine = (static_cast<long long>(slot) * a.n_kv_heads + kvh) * 32 + lane;
+  int from = 0, to = 0;
+  if (mine < a.n_seqs) {
+    from = __ldg(a.q_start + mine);
+    to = __ldg(a.q_start + mine + 1);
   }
-  below = __reduce_add_sync(0xffffffffu, below);
-  if (broken) set_status(a.status, kStatusBadIndex);
+  int below = 0, among = a.n_seqs;
+  while (true) {
+    const int step = (among - 1) / 128 + 1;
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const long long at = static_cast<long long>(lane + 32 * k) * step;
+      if (at < among) {
+        const int i = below + static_cast<int>(at);
+        n += __ldg(a.q_start + i) / span <= slot - i;
+      }
+    }
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (step == 1) {
+      below += n;
+      break;
+    }
+    if (n == 0) break;  // (only among all of them, and then the first start is not 0)
+    below += (n - 1) * step;
+    among = min(step, among - (n - 1) * step);
+  }
+  if (from < 0 || to < from || to > a.n_tokens) set_status(a.status, kStatusBadIndex);
   const int seq = below - 1;
   if (seq < 0) return false;
   const int q0 = __ldg(a.q_start + seq), q1 = __ldg(a.q_start + seq + 1);

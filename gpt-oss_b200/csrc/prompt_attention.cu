@@ -20,24 +20,24 @@
 //
 // What bounds it: an exponential per (row, key), 16 per cycle and SM.  64 keys of both tiles
 // are 1024 cycles of exponentials against 256 of MMAs at head_dim 64 and 512 at 128; masking,
-// maximum, scaling, sum and packing are issued beside them.  A few of the exponentials are
-// therefore computed on the FMA pipes: one in 8 pairs at head_dim 64 with 128 keys (one prompt
-// of 8192 tokens, 64/8 heads: 662 us, 69 % of what the exponentials alone would take; 756 with
-// none, 790 with one in four), one in 16 at 128 (one prompt of 4096 tokens, 32/4 heads: 133 us, 1.03 PFLOP/s;
-// 143 with one in 8).  Handing S over earlier is slower (784 us): the late arrival keeps the two
-// tiles out of phase.
+// maximum, scaling, sum and packing are issued beside them.  With units of 128 keys one in five
+// pairs of exponentials is therefore computed on the FMA pipes (one prompt of 8192 tokens, 64/8
+// heads of 64: 656 us, 73 % of the exponentials' rate; 740 with none, 680 with one in four); with
+// units of 64 keys that gains nothing (one prompt of 4096 tokens, 32/4 heads of 128: 137 us, 1.0
+// PFLOP/s; 143 with one in eight).  Handing S over earlier is slower (784 us): the late arrival
+// keeps the two tiles out of phase.
 //
 // KEYS: 128 where TMEM holds S, P and O of both tiles (head_dim <= 64), 64 at 128.  A narrow
 // window leaves most of a unit of 128 masked, so 64 are taken there too.  Time with 64 and 128
-// keys of 10 packed prompts (13626 tokens), 64/8 heads of 64, by window: 128 tokens 127 and 150 us, 256 166 and
-// 176, 512 228 and 229, 1024 330 and 301, 2048 474 and 420.
+// keys of 10 packed prompts (13626 tokens), 64/8 heads of 64, by window: 32 tokens 117 and 125
+// us, 128 133 and 156, 256 170 and 182, 512 231 and 231, 1024 332 and 303, 2048 471 and 418.
 //
 // Few tiles and long contexts: a cluster of up to 8 CTAs shares one pair of tiles, each taking
 // an equal run of units; the partial (m, l, O) are joined through distributed shared memory, in
 // rank order, so the result does not depend on timing and no workspace is needed.  Only as far
 // as SMs would be idle otherwise: a cluster waits until that many SMs are free at once, and
 // four packed pieces of prompts (3690 tokens, 32/4 heads of 128, contexts up to 16130) took 264
-// us with whole jobs, 309 with every job in two parts and 471 in four.
+// us with whole jobs (250 now), 309 with every job in two parts and 471 in four.
 //
 // Probabilities are rounded to the 16-bit type for the second product (tensor cores take both
 // operands in one type); their sum is taken in fp32 before that rounding.
@@ -72,8 +72,8 @@ struct AttnShape {
   static constexpr int kColP = 2 * KEYS;
   static constexpr int kColO = D == 128 ? 256 : 384;
   static_assert(3 * KEYS <= kColO && kColO + 2 * D <= kAttnTmemCols, "TMEM");
-  // every kPolyStep-th pair of exponentials is computed on the FMA pipes
-  static constexpr int kPolyStep = D == 128 ? 16 : KEYS == 64 ? 6 : 8;
+  // every kPolyStep-th of 16 pairs of exponentials is computed on the FMA pipes
+  static constexpr int kPolyStep = KEYS == 64 ? 17 : 5;
   static constexpr int kOperandBytes = 2 * kQBytes + 2 * kRingBytes;
   // fp32 partial outputs of both tiles take the operands' place in a split launch
   static constexpr int kSmemBytes = 1024 + (kOperandBytes > 256 * D * 4 ? kOperandBytes : 256 * D * 4);
@@ -209,7 +209,7 @@ template <int KEYS>
 __device__ bool attn_find_job(const gptoss_attention_args_t &a, int tok, int slot, int kvh, int rank,
                               int split, int lane, AttnJob *job) {
   AttnRows r;
-  if (!attn_find_rows(a, 2 * tok, slot, lane, &r)) return false;
+  if (!attn_find_rows(a, 2 * tok, slot, kvh, lane, &r)) return false;
   if (lane != 0) return true;
   const int units = (r.keys + KEYS - 1) / KEYS;
   job->kvh = kvh;
@@ -574,6 +574,13 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
       const int first = static_cast<int>(max(first_ll, -1ll));
       const int last_min = __shfl_sync(0xffffffffu, last, 0);
       const int first_max = __shfl_sync(0xffffffffu, first, 31);
+      // one bit per key, so that masking a key costs a bit test and a select
+      auto seen_keys = [&](int q, int key0) {
+        const int lo = first - key0 - 32 * q, hi = last - key0 - 32 * q;
+        const uint32_t from = lo <= 0 ? 0xffffffffu : (lo > 31 ? 0u : 0xffffffffu << lo);
+        const uint32_t upto = hi >= 31 ? 0xffffffffu : (hi < 0 ? 0u : (2u << hi) - 1u);
+        return from & upto;
+      };
       m = -INFINITY;
       l = 0.f;
       for (int i = 0; i < n; i++) {
@@ -591,14 +598,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
         float scale_o = 1.f;
         if (warp_live) {
           const int key0 = (begin + i) * KEYS + half * kMine;
-          if (key0 + kMine - 1 > last_min || key0 < first_max) {
-            // one bit per key, so that a key costs a bit test and a select
+          const bool masked = key0 + kMine - 1 > last_min || key0 < first_max;
+          if (masked) {
 #pragma unroll
             for (int q = 0; q < kParts; q++) {
-              const int lo = first - key0 - 32 * q, hi = last - key0 - 32 * q;
-              const uint32_t from = lo <= 0 ? 0xffffffffu : (lo > 31 ? 0u : 0xffffffffu << lo);
-              const uint32_t upto = hi >= 31 ? 0xffffffffu : (hi < 0 ? 0u : (2u << hi) - 1u);
-              const uint32_t seen = from & upto;
+              const uint32_t seen = seen_keys(q, key0);
 #pragma unroll
               for (int e = 0; e < 32; e++)
                 if (!(seen & (1u << e))) s[q][e] = 0xff800000u;
@@ -641,6 +645,15 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
               sum = f32x2_add(sum, f32x2(y.x, y.y));
               p[q][e] = pack16(y.x, y.y, static_cast<T *>(nullptr));
             }
+          if (!kHalf && masked) {  // poly_exp2's 2^-125 (0 in fp16) of masked keys
+#pragma unroll
+            for (int q = 0; q < kParts; q++) {
+              const uint32_t seen = seen_keys(q, key0);
+#pragma unroll
+              for (int e = S::kPolyStep - 1; e < 16; e += S::kPolyStep)
+                p[q][e] &= (seen & (1u << (2 * e)) ? 0xffffu : 0u) | (seen & (2u << (2 * e)) ? 0xffff0000u : 0u);
+            }
+          }
           const float2 sums = f32x2_parts(sum);
           l += sums.x + sums.y;
         }

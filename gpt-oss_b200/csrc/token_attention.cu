@@ -87,7 +87,7 @@ token_attention_kernel(const gptoss_attention_args_t a, int group, int span, int
   const int slot = unit / a.n_kv_heads, kvh = unit - slot * a.n_kv_heads;
   if (warp == 0) {
     AttnRows r;
-    const bool yes = attn_find_rows(a, span, slot, lane, &r);
+    const bool yes = attn_find_rows(a, span, slot, kvh, lane, &r);
     if (lane == 0) {
       found = yes;
       if (yes) job = r;

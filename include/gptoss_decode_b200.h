@@ -236,9 +236,11 @@ int gptoss_decode_rope_append(const gptoss_rope_args_t *args, void *stream);
  * anything (NaN included); those that some query sees must be finite.
  * Heads are contiguous, rows are `*_stride` elements apart; addresses and strides in bytes
  * are multiples of 16.  head_dim 32, 64 or 128; n_q_heads a multiple of n_kv_heads, at most
- * 128 times it.  q_start is ascending from 0 to n_tokens; a sequence whose entries
- * break that, whose keys leave [0, n_kv_rows) or whose kv_len is negative is left unwritten
- * and reported as status 104.  Rows that belong to no sequence are left unwritten too.
+ * 128 times it; out does not overlap the inputs.  q_start is ascending from 0; its last entry
+ * may be below n_tokens.  A sequence whose keys leave [0, n_kv_rows) or whose kv_len is negative
+ * is left unwritten and reported as status 104; so are entries of q_start that do not ascend or
+ * pass n_tokens, and then it is open which rows of out are written.  Rows that belong to no
+ * sequence are left unwritten.  Sinks are finite or -infinity (no sink).
  * max_kv_len: an upper bound on kv_len that the host knows (0 = not known); it only chooses
  * how the work is split.
  */

@@ -344,3 +344,70 @@ def test_too_many_rows_and_nothing_to_do(pkg):
     for change in (dict(n_tokens=0, q=None, out=None), dict(n_seqs=0, q_start=None)):
         a = _c_args(pkg, **change)
         assert lib.gptoss_decode_prompt_attention(ctypes.byref(a), None) == pkg.GPTOSS_OK
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d,window", [("bfloat16", 64, 0), ("bfloat16", 64, 100), ("float16", 32, 0),
+                                            ("bfloat16", 128, 0)])
+def test_huge_values_behind_a_query_have_no_weight(pkg, dtype, d, window):
+    """A key that a query may not see weighs exactly nothing, even where its value is near the
+    type's largest: the queries before it match as if it were not there."""
+    import torch
+
+    dev = torch.device("cuda:0")
+    q_lens, kv_lens, seen = [300], [300], 250
+    q, k, v, sinks, out, whole, starts = _make(torch, dev, 14, q_lens, kv_lens, 8, 1, d, dtype)
+    v[starts[0] + seen:starts[0] + 300] = torch.finfo(v.dtype).max / 2
+    q_start, kv_start, kv_len = _index(torch, dev, q_lens, starts, kv_lens)
+    want, mag, keys = _reference(q, k, v, q_lens, starts, kv_lens, sinks, d ** -0.5, window)
+    pkg.prompt_attention(q, k, v, q_start, kv_start, kv_len, out, sinks=sinks, window=window,
+                         stream=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    _check(out[:seen], want[:seen], mag[:seen], keys[:seen], dtype, 10.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [2, 6])
+def test_thousands_of_sequences(pkg, most):
+    """More sequences than one look at their starts covers, some without a query; a bad one late
+    in the list is reported and the others stand."""
+    import torch
+
+    dev = torch.device("cuda:0")
+    rng = np.random.default_rng(most)
+    q_lens = [int(n) for n in rng.integers(0, most + 1, 2900)]
+    kv_lens = [n + int(rng.integers(0, 9)) for n in q_lens]
+    q, k, v, sinks, out, whole, starts = _make(torch, dev, 15, q_lens, kv_lens, 8, 1, 32, "bfloat16", gap=1)
+    q_start, kv_start, kv_len = _index(torch, dev, q_lens, starts, kv_lens)
+    bad = max(i for i, n in enumerate(q_lens) if n)
+    kv_len[bad] = -1
+    want, mag, keys = _reference(q, k, v, q_lens, starts, kv_lens, sinks, 32 ** -0.5, 0)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    pkg.prompt_attention(q, k, v, q_start, kv_start, kv_len, out, sinks=sinks, status=status,
+                         stream=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert status.item() == 104
+    at = sum(q_lens[:bad])
+    assert (out[at:at + q_lens[bad]] == 9.0).all()
+    _check(out[:at], want[:at], mag[:at], keys[:at], "bfloat16", 10.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("starts_of", [[0, 5, 3, 10, 12], [0, -4, 3, 8, 12], [2, 5, 8, 10, 12], [0, 5, 8, 40, 12]])
+@pytest.mark.parametrize("group", [1, 32])
+def test_starts_that_do_not_ascend(pkg, starts_of, group):
+    """Reported, and nothing is written outside the rows."""
+    import torch
+
+    dev = torch.device("cuda:0")
+    q, k, v, sinks, out, whole, starts = _make(torch, dev, 16, [3, 3, 3, 3], [30, 30, 30, 30], group, 1, 64,
+                                               "bfloat16", pad=8)
+    q_start, kv_start, kv_len = _index(torch, dev, [3, 3, 3, 3], starts, [30, 30, 30, 30])
+    q_start.copy_(torch.tensor(starts_of, dtype=torch.int32))
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    pkg.prompt_attention(q, k, v, q_start, kv_start, kv_len, out, status=status,
+                         stream=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert status.item() == (0 if starts_of[0] == 2 else 104)
+    assert (whole[:, group * 64:] == 9.0).all()
+    assert torch.isfinite(out.float()).all()
