@@ -465,6 +465,7 @@ struct gptoss_decode {
   int *d_tokens = nullptr, *d_pos = nullptr, *d_next = nullptr, *status = nullptr;
   int *h_pinned = nullptr;  // tokens | pos | next, max_batch each
   bf16 *last_x = nullptr;   // [max_batch, H] residual rows of the prompts' last tokens
+  std::vector<char> row_used;  // [max_batch] cache rows that a prefill has seen
   // prompt passes and sampling settings: device copies and their pinned sources
   unsigned char *prompt_dev = nullptr, *prompt_host = nullptr;
   float *samp_dev = nullptr, *samp_host = nullptr;  // u | temperature | top_p | min_p | top_k
@@ -674,6 +675,7 @@ static int decode_create(const gptoss_model_config_t *cfg, int max_batch, int ma
   h->cfg = c;
   h->max_batch = max_batch;
   h->max_rows = max_rows;
+  h->row_used.resize(max_batch);
   h->device = device;
   h->moe = moe;
   h->have.assign(c.n_layers + 1, 0u);
@@ -1214,7 +1216,8 @@ int gptoss_decode_prefill(gptoss_decode_t *h, const int *tokens, const int *rows
   if (!own_linear(h)) return dfail(h, GPTOSS_E_STATE, "prefill: the projections' shapes need the step's fallback path");
   if (static_cast<size_t>(h->max_batch) * S > INT32_MAX - 256)
     return dfail(h, GPTOSS_E_CAPACITY, "prefill: max_batch * seq_len is above 2^31 - 257");
-  std::vector<char> used(h->max_batch, 0);
+  std::vector<char> &used = h->row_used;  // (allocated with the engine: nothing throws here)
+  std::fill(used.begin(), used.end(), 0);
   long long total = 0;
   for (int i = 0; i < n_seqs; i++) {
     if (rows[i] < 0 || rows[i] >= h->max_batch || used[rows[i]])
@@ -1273,7 +1276,10 @@ int gptoss_decode_prefill(gptoss_decode_t *h, const int *tokens, const int *rows
     pass.q_start = dev(at.q_start);
     pass.kv_len = dev(at.kv_len);
     int rc = run_layers(h, pass.tokens, dev(at.tokens), dev(at.pos), &pass, st);
-    if (rc) return rc;
+    if (rc) {
+      cudaStreamSynchronize(st);  // the next call writes the pinned image again
+      return rc;
+    }
     if (last > 0) {
       gather_last_rows_kernel<<<(last + 7) / 8, 256, 0, st>>>(h->last_x, h->x, dev(at.last_from),
                                                               dev(at.last_to), last, c.hidden_dim);

@@ -273,10 +273,10 @@ int gptoss_decode_prompt_attention(const gptoss_attention_args_t *args, void *st
  * A NaN in one of the last two is no limit either.
  * next[r] is the lowest kept id whose running sum of kept weights, in the order of the ids,
  * exceeds u[r] times their total, u in [0, 1) (values outside are clamped, NaN counts as 0).
- * T <= 0 or NaN: the largest logit, lowest id among equals.  NaN logits count as -infinity,
- * which is never drawn; a row with nothing else gives 0, as the argmax of the step does.
- * Where logits are +infinity those alone are kept, with equal weight, as far as top_k and
- * top_p leave them.  Rows with pos[r] < 0 give -1.
+ * T <= 0 or NaN: the largest logit, lowest id among equals; above 1e36 it counts as 1e36.
+ * NaN logits count as -infinity, which is never drawn; a row with nothing else gives 0, as the
+ * argmax of the step does.  Where logits are +infinity those alone are kept, with equal weight,
+ * as far as top_k and top_p leave them.  Rows with pos[r] < 0 give -1.
  * Weights are formed in fp64 and summed as multiples of 2^-44 in 64-bit integers, so sums do
  * not depend on their order and a draw does not either; a weight below 2^-45 counts as 0.
  * logits [n_rows, vocab], rows `stride` elements apart, in bf16, fp16 or fp32; vocab up to
