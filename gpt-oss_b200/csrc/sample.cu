@@ -9,16 +9,20 @@
 // A cluster of up to 8 CTAs holds a row in its shared memory: the logits are read from HBM
 // once, and what follows runs on chip:
 //   1. load, maximum (joined over the cluster)
-//   2. where top-k or top-p is set: counts and weights of kBins bins of equal width below the
-//      maximum, summed over the cluster; the bin in which top-k ends, then (with the weight of
-//      what top-k kept) the bin in which top-p ends.  The few logits of such a bin go to a list
-//      that every CTA ranks for itself; a bin with more than kList logits (many equal ones, or
-//      a temperature that is high for their spread) is searched by the digits of their bits
+//   2. a top-k of up to kList / 2: the top_k-th largest of the threads' maxima bounds it from
+//      below; the logits from there on go to a list that every CTA sorts for itself, and top-p
+//      is then found in that list too.  Otherwise: counts (top-k) or counts and weights (top-p)
+//      of kBins bins of equal width below the maximum, summed over the cluster, and the bin in
+//      which the limit falls; its logits go to the list.  A bin with more than kList of them is
+//      cut into kBins parts first, and where a part still has more (equal logits, or what lies
+//      beyond the last bin) it is searched by the digits of their bits
 //   3. running sums in the order of the ids: threads own consecutive ids, block and cluster
 //      prefix; the thread in whose run the drawn value falls walks its run again
-// What bounds it: for large batches the read from HBM (two CTAs per SM, so that one loads while
-// the other computes) and the weights' fp64 arithmetic, about ten operations each; for a few
-// rows the cluster barriers between the steps.
+// What bounds it: for large batches the weights' arithmetic, 54 instructions a logit, 14 of them
+// fp64 (two CTAs per SM, so that one loads while the other computes; 512 rows of 201088 by
+// temperature 288 us, 1.4 TB/s); with top-p without top-k the weights once more and the shared
+// atomics of the bins (96 rows of 50257: 64 us); for a few rows the cluster barriers between the
+// steps, 1.3 us each (one row of 201088 with all limits 20 us, 64 rows of mixed settings 99).
 //
 // A weight has to be good to about 2^-44 relative, not to fp32's 2^-24: with 200000 kept tokens
 // a draw lies within 2^-24 of some running sum every few rows, and would then pick the wrong one.
@@ -399,7 +403,8 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
     };
     constexpr int kPer = kList / kSampleThreads;
     // The row's logits in bins [lo, hi] (part >= 0: in that part of the one bin) and not below
-    // `floor_value`, as keys in s.merged, the largest first.  Returns their number; more than kList of them are not listed.
+    // `floor_value`, as keys in s.merged, the largest first.  Returns their number; more than
+    // kList of them are not listed.
     auto collect = [&](int which, int lo, int hi, int part, float floor_value) -> unsigned {
       // most logits lie far from the bins: a comparison tells
       float low, high;
