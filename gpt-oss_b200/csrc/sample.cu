@@ -66,7 +66,7 @@ __device__ __forceinline__ float logit_at(const bf16 *p) { return __bfloat162flo
 __device__ __forceinline__ float logit_at(const __half *p) { return __half2float(*p); }
 
 struct SampleShared {
-  double table[16];                // 2^(-j / 16)
+  double table[16];                // 2^(44 - j / 16)
   union {
     u64 mass[kBins];               // cluster reads: weight of a bin in this CTA's part of the row
     uint32_t merged[kList];        // the cluster's lists together, largest first
@@ -103,9 +103,9 @@ __device__ __forceinline__ unsigned peer_u32(const unsigned *p, int cta) {
   return v;
 }
 
-// Weights: 2^(44 - y), y = (max - x) / (T ln 2), rounded to an integer.  y = k / 16 + r with
-// an integer k: 2^(-k/16) from a table and an exponent, 2^-r by its Taylor polynomial of
-// degree 6 (|r| <= 1/32: below 1e-15 relative).  All in fp64; the two additions of a power of
+// Weights: 2^(44 - y), y = (max - x) / (T ln 2), rounded to an integer.  16 y = k + r with an
+// integer k: 2^(44 - k/16) from a table and an exponent, 2^(-r/16) by its Taylor polynomial of
+// degree 6 (|r| <= 1/2: below 1e-15 relative).  All in fp64; the two additions of a power of
 // two round to integers and leave them in the low bits, which spares the slow conversions.
 // (Per SM and cycle: 64 fp64 operations, 16 conversions of fp32 to fp64, and 15.6 lookups in a
 // table of 16 doubles, which lie in different banks; of 128 only 6.9.)
@@ -118,33 +118,36 @@ struct Weigher {
   static constexpr u64 kBias = 0x4330000000000000ull;
   template <int N>
   __device__ __forceinline__ void biased(const float (&x)[N], u64 (&w)[N]) const {
+    constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52
+    constexpr double c1 = -0.69314718055994530942 / 16, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4,
+                     c5 = c4 * c1 / 5, c6 = c5 * c1 / 6;
     double p[N], r[N];
     int k[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const double y = (max - static_cast<double>(fmaxf(x[i], floor))) * scale;
-      const double shifted = y + 6755399441055744.0;  // 1.5 * 2^52
+      const double d = max - static_cast<double>(fmaxf(x[i], floor));
+      const double shifted = fma(d, scale, kRound);
       k[i] = __double2loint(shifted);
-      r[i] = (y - (shifted - 6755399441055744.0)) * (-0.69314718055994530942 / 16);
+      r[i] = fma(d, scale, kRound - shifted);
     }
 #pragma unroll
-    for (int i = 0; i < N; i++) p[i] = fma(r[i], 1.0 / 720, 1.0 / 120);
+    for (int i = 0; i < N; i++) p[i] = fma(r[i], c6, c5);
 #pragma unroll
-    for (int i = 0; i < N; i++) p[i] = fma(p[i], r[i], 1.0 / 24);
+    for (int i = 0; i < N; i++) p[i] = fma(p[i], r[i], c4);
 #pragma unroll
-    for (int i = 0; i < N; i++) p[i] = fma(p[i], r[i], 1.0 / 6);
+    for (int i = 0; i < N; i++) p[i] = fma(p[i], r[i], c3);
 #pragma unroll
-    for (int i = 0; i < N; i++) p[i] = fma(p[i], r[i], 0.5);
+    for (int i = 0; i < N; i++) p[i] = fma(p[i], r[i], c2);
+#pragma unroll
+    for (int i = 0; i < N; i++) p[i] = fma(p[i], r[i], c1);
 #pragma unroll
     for (int i = 0; i < N; i++) p[i] = fma(p[i], r[i], 1.0);
 #pragma unroll
-    for (int i = 0; i < N; i++) p[i] = fma(p[i], r[i], 1.0) * table[k[i] & 15];
-#pragma unroll
     for (int i = 0; i < N; i++) {
-      // 2^(44 - k / 16) by the exponent (k / 16 <= 46), then rounding to an integer
-      const double q = __hiloint2double(__double2hiint(p[i]) + ((44 - (k[i] >> 4)) << 20), __double2loint(p[i])) +
-                       4503599627370496.0;  // 2^52
-      w[i] = static_cast<u64>(__double_as_longlong(q));
+      // times 2^(44 - k / 16) (the whole part, at most 47, by the exponent), rounded to an integer
+      const double at = table[k[i] & 15];
+      const double power = __hiloint2double(__double2hiint(at) - ((k[i] & ~15) << 16), __double2loint(at));
+      w[i] = static_cast<u64>(__double_as_longlong(fma(p[i], power, 4503599627370496.0)));  // 2^52
     }
   }
   __device__ __forceinline__ u64 operator()(float x) const {
@@ -198,6 +201,12 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
   }
   const int id0 = min(a.vocab, rank * per), n = min(a.vocab, id0 + per) - id0;
   const T *x = static_cast<const T *>(a.logits) + row * a.stride + id0;
+  // the row's settings, on their way while the logits are
+  const float temp = a.temperature ? a.temperature[row] : 1.0f;
+  const int top_k = a.top_k ? a.top_k[row] : 0;
+  const float top_p = a.top_p ? a.top_p[row] : 1.0f;
+  const float min_p = a.min_p ? a.min_p[row] : 0.0f;
+  const float u0 = a.u[row];
   // ------------------------------------------------------------------ 1. load, maximum
   // 16-byte loads from the first 16-byte boundary on; the slice starts so far into its buffer
   // that those end up on 16-byte boundaries there too
@@ -238,14 +247,16 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
       s.first = kAll;
     }
   }
-  if (tid < 16) s.table[tid] = exp2(-tid / 16.0);
+  if (tid < 16) s.table[tid] = exp2(44 - tid / 16.0);
   if (tid < 3) s.listed[tid] = 0;
   for (int i = tid; i < kBins; i += kSampleThreads) s.mass[i] = s.count[i] = 0;
+  const double t = fmin(static_cast<double>(temp), 1e36);
+  const double reach = 46 * 0.69314718055994530942 * t;
+  const double scale = 16 * 1.44269504088896340736 / t;
   sync();
   uint32_t key = 0;
 #pragma unroll
   for (int c = 0; c < split; c++) key = max(key, split > 1 ? peer_u32(&s.best, c) : s.best);
-  const float temp = a.temperature ? a.temperature[row] : 1.0f;
   if (!(temp > 0.0f) || key == kKeyNegInf) {
     // greedy: the lowest id of the largest logit (-infinity everywhere: the first id)
     const float want = key_value(key);
@@ -265,9 +276,6 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
     return;
   }
   float top = key_value(key);
-  const double t = fmin(static_cast<double>(temp), 1e36);
-  const double reach = 46 * 0.69314718055994530942 * t;
-  const double scale = 16 * 1.44269504088896340736 / t;
   // Weights need a finite maximum, room below it, and fp32 steps there that are small against
   // the temperature.  +infinity: those logits become 0, the others -infinity.  A maximum near
   // the lowest value (a row of masks), or far larger than the temperature: logits relative to it.
@@ -288,9 +296,6 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
   weigher.scale = scale;
   weigher.floor = floor_of(top);
   weigher.table = s.table;
-  const int top_k = a.top_k ? a.top_k[row] : 0;
-  const float top_p = a.top_p ? a.top_p[row] : 1.0f;
-  const float min_p = a.min_p ? a.min_p[row] : 0.0f;
   const bool by_count = top_k > 0 && top_k < a.vocab, by_mass = top_p < 1.0f;
   // kept: keys above `edge`, and the first `need` ids of those equal to it
   uint32_t edge = 0;
@@ -747,24 +752,39 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
       total += sums[c];
     }
   }
-  const float u0 = a.u[row];
+  // nobody leaves while its shared memory is read; what follows needs none of the others
+  if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   const float u = u0 > 0.0f ? fminf(u0, 0.99999994f) : 0.0f;
   const u64 target = static_cast<u64>(static_cast<double>(u) * static_cast<double>(total));
-  if (before <= target && target < before + mass) {
-    u64 sum = before;
-    int pick = -1;
-    r = eq_before;
-    for (i = i0; i < i1 && pick < 0; i += 4) {
-      weights_at(i, w4, &r);
+  // the thread in whose run the target falls has its warp walk the run, an id per lane
+  const unsigned here = __ballot_sync(0xffffffffu, before <= target && target < before + mass);
+  if (here) {
+    const int owner = __ffs(here) - 1;
+    const int from = __shfl_sync(0xffffffffu, i0, owner), to = __shfl_sync(0xffffffffu, i1, owner);
+    u64 sum = __shfl_sync(0xffffffffu, before, owner);
+    u64 rank_of = __shfl_sync(0xffffffffu, eq_before, owner);
+    for (int at = from; at < to; at += 32) {
+      const float v = at + lane < to ? slice[at + lane] : -INFINITY;
+      const unsigned equal = __ballot_sync(0xffffffffu, v == edge_value);
+      bool in = v > -INFINITY && v >= edge_value;
+      if (need != kAll && v == edge_value) in = in && rank_of + __popc(equal & ((1u << lane) - 1u)) < need;
+      rank_of += __popc(equal);
+      u64 w = weigher(v);
+      if (!in || w < least) w = 0;
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        sum += w4[j];
-        if (pick < 0 && sum > target) pick = i + j;
+      for (int i = 1; i < 32; i <<= 1) {
+        const u64 o = __shfl_up_sync(0xffffffffu, w, i);
+        if (lane >= i) w += o;
       }
+      const unsigned past = __ballot_sync(0xffffffffu, sum + w > target);
+      if (past) {
+        if (lane == 0) a.next[row] = id0 + at + __ffs(past) - 1;
+        break;
+      }
+      sum += __shfl_sync(0xffffffffu, w, 31);
     }
-    a.next[row] = id0 + pick;
   }
-  if (split > 1) cluster_barrier_all();  // nobody leaves while its shared memory is read
+  if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 template <typename T>
