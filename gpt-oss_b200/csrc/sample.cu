@@ -17,7 +17,7 @@
 //      cut into kBins parts first, and where a part still has more (equal logits, or what lies
 //      beyond the last bin) it is searched by the digits of their bits
 //   3. running sums in the order of the ids: threads own consecutive ids, block and cluster
-//      prefix; the thread in whose run the drawn value falls walks its run again
+//      prefix; the warp of the thread in whose run the drawn value falls walks that run again
 // What bounds it: for large batches the weights' arithmetic, 54 instructions a logit, 14 of them
 // fp64 (two CTAs per SM, so that one loads while the other computes; 512 rows of 201088 by
 // temperature 288 us, 1.4 TB/s); with top-p without top-k the weights once more and the shared
@@ -73,7 +73,7 @@ struct SampleShared {
   };
   unsigned count[kBins];           // cluster reads: logits of a bin
   uint32_t list[kList];            // cluster reads: keys that the CTA contributes to a list
-  u64 warp_sum[kSampleWarps];
+  u64 warp_sum[2][kSampleWarps];
   float warp_max[kSampleWarps];
   uint32_t best;                   // cluster reads: key of the CTA's largest logit
   unsigned first;                  // cluster reads: lowest id of the largest logit
@@ -158,7 +158,8 @@ struct Weigher {
   }
 };
 
-// Sum over the block of v; every thread gets the exclusive prefix in *before.
+// Sum over the block of v; every thread gets the exclusive prefix in *before.  Two scans in a row
+// use different scratch, so that one barrier each is enough.
 __device__ u64 block_scan(u64 v, u64 *before, u64 *scratch) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   u64 inc = v;
@@ -169,15 +170,15 @@ __device__ u64 block_scan(u64 v, u64 *before, u64 *scratch) {
   }
   if (lane == 31) scratch[warp] = inc;
   __syncthreads();
-  u64 base = 0, total = 0;
+  const u64 mine = scratch[lane & (kSampleWarps - 1)];
+  u64 sums = mine;
 #pragma unroll
-  for (int w = 0; w < kSampleWarps; w++) {
-    if (w == warp) base = total;
-    total += scratch[w];
+  for (int i = 1; i < kSampleWarps; i <<= 1) {
+    const u64 o = __shfl_up_sync(0xffffffffu, sums, i);
+    if (lane >= i) sums += o;
   }
-  __syncthreads();
-  *before = base + inc - v;
-  return total;
+  *before = __shfl_sync(0xffffffffu, sums - mine, warp) + inc - v;
+  return __shfl_sync(0xffffffffu, sums, kSampleWarps - 1);
 }
 
 // split: CTAs of a row
@@ -189,6 +190,8 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
   const int tid = threadIdx.x, lane = tid & 31;
   const int rank = split > 1 ? static_cast<int>(cluster_cta_rank()) : 0;
   const int row = blockIdx.x / split;
+  int turn = 0;
+  auto scan = [&](u64 v, u64 *before) { return block_scan(v, before, s.warp_sum[turn ^= 1]); };
   auto sync = [&]() {
     if (split > 1)
       cluster_barrier_all();
@@ -386,8 +389,8 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
       }
       sync();
       gather(tid, weights, &my_count, &my_mass);
-      all_count = block_scan(my_count, &count_before, s.warp_sum);
-      all_mass = block_scan(my_mass, &mass_before, s.warp_sum);
+      all_count = scan(my_count, &count_before);
+      all_mass = scan(my_mass, &mass_before);
     };
     // The arrays are cleared for another histogram once everyone has read them.
     auto clear = [&]() {
@@ -494,7 +497,7 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
           w[j] = i < stay ? weigher(key_value(s.merged[i])) : 0;
           sum += w[j];
         }
-        const u64 all = block_scan(sum, &front, s.warp_sum);
+        const u64 all = scan(sum, &front);
         if (share >= 0.0) limit = share * static_cast<double>(all);
         unsigned kept = 0;
         u64 f = acc + front;
@@ -576,8 +579,8 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
         u64 w = 0, c_before, w_before;
         const int digit = 255 - tid;  // largest digit first
         if (tid < 256) gather(digit, weights, &c, &w);
-        const u64 c_all = block_scan(c, &c_before, s.warp_sum);
-        block_scan(w, &w_before, s.warp_sum);
+        const u64 c_all = scan(c, &c_before);
+        scan(w, &w_before);
         bool here = c > 0;
         if (limit < 0.0) {
           here = here && c_before < want && want <= c_before + c;
@@ -615,7 +618,7 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
       if (best > -INFINITY) atomicAdd(&s.count[bin_of(best)], 1u);
       sync();
       gather(tid, false, &my_count, &my_mass);
-      all_count = block_scan(my_count, &count_before, s.warp_sum);
+      all_count = scan(my_count, &count_before);
       const u64 want = top_k;
       if (want <= all_count) {
         if (count_before < want && want <= count_before + my_count) s.bin = tid;
@@ -690,7 +693,7 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
   if (need != kAll) {  // ids equal to the edge in front of the thread's
     u64 eq = 0;
     for (int i = i0; i < i1; i++) eq += slice[i] == edge_value;
-    const u64 all = block_scan(eq, &eq_before, s.warp_sum);
+    const u64 all = scan(eq, &eq_before);
     if (split > 1) {
       if (tid == 0) s.equal = static_cast<unsigned>(all);
       sync();
@@ -737,7 +740,7 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
     weights_at(i, w4, &r);
     mass += (w4[0] + w4[1]) + (w4[2] + w4[3]);
   }
-  const u64 own = block_scan(mass, &before, s.warp_sum);
+  const u64 own = scan(mass, &before);
   u64 total = own;
   if (split > 1) {
     if (tid == 0) s.sum = own;
