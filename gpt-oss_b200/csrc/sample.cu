@@ -18,11 +18,12 @@
 //      beyond the last bin) it is searched by the digits of their bits
 //   3. running sums in the order of the ids: threads own consecutive ids, block and cluster
 //      prefix; the warp of the thread in whose run the drawn value falls walks that run again
-// What bounds it: for large batches the weights' arithmetic, 54 instructions a logit, 14 of them
-// fp64 (two CTAs per SM, so that one loads while the other computes; 512 rows of 201088 by
-// temperature 288 us, 1.4 TB/s); with top-p without top-k the weights once more and the shared
-// atomics of the bins (96 rows of 50257: 64 us); for a few rows the cluster barriers between the
-// steps, 1.3 us each (one row of 201088 with all limits 20 us, 64 rows of mixed settings 99).
+// What bounds it: for large batches the chain of a CTA's steps - load 4 us, maximum 2, weights 5
+// (some fifty instructions a logit, 11 of them fp64), sums 2, pick 1 - of which two CTAs per SM
+// overlap (512 rows of 201088 by temperature 251 us, 1.6 TB/s, issue 55 %); with top-p without
+// top-k the weights once more and the shared atomics of the bins, 13 us (96 rows of 50257: 59
+// us); for a few rows the cluster barriers between the steps, 1.3 us each (one row of 201088
+// with all limits 18 us, 64 rows of mixed settings 88).
 //
 // A weight has to be good to about 2^-44 relative, not to fp32's 2^-24: with 200000 kept tokens
 // a draw lies within 2^-24 of some running sum every few rows, and would then pick the wrong one.
