@@ -19,6 +19,7 @@
 // with a graph launch), with four an SM holds fewer CTAs (256 sequences of 512 keys: 102 instead
 // of 74).  Clusters of 8 take 88 us for the long token.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "attention_rows.cuh"
@@ -330,6 +331,36 @@ token_attention_kernel(const gptoss_attention_args_t a, int group, int span, int
   cluster_barrier_all();  // nobody leaves while its shared memory is read
 }
 
+// Whether the device takes clusters of 16 of this kernel (a part of a GPU may not); asked once
+// per device.
+template <typename T, int D>
+static bool takes_16() {
+  static std::atomic<int> known[64];
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return false;
+  int state = known[device].load(std::memory_order_relaxed);
+  if (state == 0) {
+    typedef TokenShape<D> S;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(16);
+    cfg.blockDim = dim3(kTokenThreads);
+    cfg.dynamicSmemBytes = S::kSmemBytes;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 16;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    const bool yes = cudaOccupancyMaxActiveClusters(&clusters, token_attention_kernel<T, D>, &cfg) == cudaSuccess &&
+                     clusters > 0;
+    if (!yes) cudaGetLastError();
+    state = yes ? 2 : 1;
+    known[device].store(state, std::memory_order_relaxed);
+  }
+  return state == 2;
+}
+
 template <typename T, int D>
 static int token_launch(const gptoss_attention_args_t &a, int sms, cudaStream_t st) {
   typedef TokenShape<D> S;
@@ -344,12 +375,14 @@ static int token_launch(const gptoss_attention_args_t &a, int sms, cudaStream_t 
   const long long blocks = (most + S::kKeys - 1) / S::kKeys;
   int split = 1;
   while (split < kTokenSplit && jobs * split * 2 <= 2 * sms && blocks >= 4 * kTokenWarps * split) split *= 2;
-  const long long grid = slots * a.n_kv_heads * split;
-  if (grid > INT32_MAX) return decode_error(GPTOSS_E_CAPACITY, "prompt_attention: too many rows for one launch");
   auto kernel = token_attention_kernel<T, D>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes);
-  if (e == cudaSuccess && split > 8)
+  if (e == cudaSuccess && split > 8) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && !takes_16<T, D>()) split = 8;
+  }
+  const long long grid = slots * a.n_kv_heads * split;
+  if (grid > INT32_MAX) return decode_error(GPTOSS_E_CAPACITY, "prompt_attention: too many rows for one launch");
   if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
