@@ -411,3 +411,14 @@ def test_starts_that_do_not_ascend(pkg, starts_of, group):
     assert status.item() == (0 if starts_of[0] == 2 else 104)
     assert (whole[:, group * 64:] == 9.0).all()
     assert torch.isfinite(out.float()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [
+    ([1500], [1500], 8, 2, 64, 600, True, "bfloat16", 0),
+    ([700, 3], [2000, 1300], 4, 4, 32, 513, False, "float16", 8),
+    ([900, 300], [900, 2100], 8, 1, 64, 512, True, "bfloat16", 0),
+    ([1100], [1400], 4, 1, 128, 700, True, "float16", 0),
+], ids=str)
+def test_wide_windows(pkg, case):
+    test_against_64_bits(pkg, case)
