@@ -46,6 +46,7 @@ constexpr int kSampleThreads = 512;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleMaxSplit = 8;     // CTAs of a row
 constexpr int kSampleMaxVocab = 1 << 18;
+constexpr int kSamplePart = 25600;     // logits of a CTA that leave room for two CTAs on an SM
 constexpr int kBins = 512;
 constexpr int kList = 1024;
 constexpr unsigned kAll = 0xffffffffu;        // no limit among equal logits; no id
@@ -791,22 +792,28 @@ sample_kernel(const gptoss_sample_args_t a, int per) {
   if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// Shared memory of a CTA that holds `logits` of them (their start is moved by up to 3, see step 1).
+constexpr size_t sample_smem(int logits) { return (static_cast<size_t>(logits) + 4) * sizeof(float); }
+
 template <typename T>
 static int sample_launch(const gptoss_sample_args_t &a, int sms, cudaStream_t st) {
   // CTAs per row: as few as let two CTAs share an SM, more while that leaves SMs without work
   int split = 1;
   auto per_cta = [&](int c) { return ((a.vocab + c - 1) / c + 7) & ~7; };
-  while (split < kSampleMaxSplit && per_cta(split) > 25600) split *= 2;
+  while (split < kSampleMaxSplit && per_cta(split) > kSamplePart) split *= 2;
   while (split < kSampleMaxSplit && static_cast<long long>(a.n_rows) * split * 2 <= sms && per_cta(split) > 4096)
     split *= 2;
   const int per = per_cta(split);
-  const size_t smem = (static_cast<size_t>(per) + 4) * sizeof(float);
+  const size_t smem = sample_smem(per);
   const long long grid = static_cast<long long>(a.n_rows) * split;
   if (grid > INT32_MAX) return decode_error(GPTOSS_E_CAPACITY, "sample: too many rows for one launch");
   void (*kernel)(const gptoss_sample_args_t, int) =
       split == 1 ? sample_kernel<T, 1>
                  : (split == 2 ? sample_kernel<T, 2> : (split == 4 ? sample_kernel<T, 4> : sample_kernel<T, 8>));
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  // The attribute belongs to the kernel and not to this launch, and another thread may be about to
+  // launch it for another vocabulary: always the most that it is ever launched with.
+  const size_t most = sample_smem(split < kSampleMaxSplit ? kSamplePart : kSampleMaxVocab / kSampleMaxSplit);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
   if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
