@@ -831,6 +831,17 @@ static int attention_launch(const gptoss_attention_args_t &a, int sms, cudaStrea
   const int group = a.n_q_heads / a.n_kv_heads, tok = 128 / group;
   const long long slots = a.n_tokens / (2 * tok) + static_cast<long long>(a.n_seqs);
   if (slots > INT32_MAX) return decode_error(GPTOSS_E_CAPACITY, "prompt_attention: too many rows and sequences");
+  // Kernel attributes first: a host thread that has made no CUDA call yet has no context, these
+  // give it the device's, and the encoding of the tensor maps fails without one.
+  auto kernel = prompt_attention_kernel<T, D, KEYS>;
+  // the kernel's warps share out the registers of a launch with 96 each: with fewer they would
+  // wait for more for ever
+  cudaFuncAttributes fa = {};
+  cudaError_t e = cudaFuncGetAttributes(&fa, kernel);
+  if (e == cudaSuccess && fa.numRegs != 96)
+    return decode_error(GPTOSS_E_STATE, "prompt_attention: built with %d registers, not 96", fa.numRegs);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes);
+  if (e != cudaSuccess) return launch_result("prompt_attention", e);
   CUtensorMap map_q, map_k, map_v;
   std::string err;
   const bool fp16 = !std::is_same<T, bf16>::value;
@@ -852,28 +863,18 @@ static int attention_launch(const gptoss_attention_args_t &a, int sms, cudaStrea
   const long long units = slots * a.n_kv_heads;
   const long long grid = units * split;
   if (grid > INT32_MAX) return decode_error(GPTOSS_E_CAPACITY, "prompt_attention: too many rows for one launch");
-  auto kernel = prompt_attention_kernel<T, D, KEYS>;
-  // the kernel's warps share out the registers of a launch with 96 each: with fewer they would
-  // wait for more for ever
-  cudaFuncAttributes fa = {};
-  cudaError_t e = cudaFuncGetAttributes(&fa, kernel);
-  if (e == cudaSuccess && fa.numRegs != 96)
-    return decode_error(GPTOSS_E_STATE, "prompt_attention: built with %d registers, not 96", fa.numRegs);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes);
-  if (e == cudaSuccess) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(grid));
-    cfg.blockDim = dim3(kAttnThreads);
-    cfg.dynamicSmemBytes = S::kSmemBytes;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = split;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = split > 1 ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, kernel, map_q, map_k, map_v, a, group, tok, static_cast<int>(slots), split);
-  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kAttnThreads);
+  cfg.dynamicSmemBytes = S::kSmemBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = split > 1 ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, kernel, map_q, map_k, map_v, a, group, tok, static_cast<int>(slots), split);
   return launch_result("prompt_attention", e);
 }
 

@@ -2,6 +2,7 @@
 import ctypes
 import threading
 
+import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -65,3 +66,45 @@ def test_two_threads_two_vocabularies(pkg):
     torch.cuda.synchronize()
     assert not raised, raised[0]
     assert all(torch.equal(s[1], w) for s, w in zip(sets, want))
+
+
+def test_all_operators_from_threads_of_their_own(pkg):
+    """Each operator with two shapes at once, through the bindings; the results are those of
+    calls one after the other."""
+    import torch
+
+    dev = torch.device("cuda:0")
+    calls = []
+    for hq, hkv, d, q_lens, kv_lens in ((16, 2, 64, [300, 1], [900, 5000]), (4, 4, 32, [1] * 5, [700] * 5)):
+        q = torch.randn(sum(q_lens), hq, d, device=dev).bfloat16()
+        k, v = (torch.randn(sum(kv_lens), hkv, d, device=dev).bfloat16() for _ in range(2))
+        index = (torch.tensor(np.concatenate([[0], np.cumsum(q_lens)]), dtype=torch.int32, device=dev),
+                 torch.tensor(np.cumsum([0] + kv_lens[:-1]), dtype=torch.int64, device=dev),
+                 torch.tensor(kv_lens, dtype=torch.int32, device=dev))
+        calls.append((torch.zeros_like(q), lambda out, st, q=q, k=k, v=v, index=index: pkg.prompt_attention(
+            q, k, v, *index, out, max_kv_len=5000, stream=st)))
+        pos = torch.arange(q.shape[0], dtype=torch.int32, device=dev) + 7
+        inv = torch.from_numpy(pkg.rope_table(d, 10000.0)[0]).to(dev)
+        calls.append((torch.zeros_like(q), lambda out, st, q=q, pos=pos, inv=inv: pkg.rope_append(
+            q, None, None, pos, inv, q_out=out, stream=st)))
+        logits, u = torch.randn(sum(q_lens), 50 * d, device=dev), torch.rand(sum(q_lens), device=dev)
+        calls.append((torch.zeros(sum(q_lens), dtype=torch.int32, device=dev),
+                      lambda out, st, x=logits, u=u: pkg.sample_tokens(x, u, out, stream=st)))
+    torch.cuda.synchronize()
+    want = []
+    for out, call in calls:
+        call(out, torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        want.append(out.clone())
+        out.zero_()
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+
+    def job(out, call, st):
+        for _ in range(100):
+            call(out, st)
+
+    raised = _at_once([lambda c=c, s=s: job(*c, s.cuda_stream) for c, s in zip(calls, streams)])
+    torch.cuda.synchronize()
+    assert not raised, raised[0]
+    assert all(torch.equal(c[0], w) for c, w in zip(calls, want))
