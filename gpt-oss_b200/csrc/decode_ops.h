@@ -53,11 +53,11 @@ class OnDeviceOf {
   bool switched_ = false;
 };
 
-// Launch result -> status code of the entry point.
-inline int launch_result(const char *what, cudaError_t e = cudaSuccess) {
-  const cudaError_t last = cudaGetLastError();
-  if (e == cudaSuccess) e = last;
+// Result of a launch (cudaLaunchKernelEx) or of a call before it -> status code of the entry
+// point.  The thread's last error is not asked: it may be left over from something else.
+inline int launch_result(const char *what, cudaError_t e) {
   if (e == cudaSuccess) return GPTOSS_OK;
+  cudaGetLastError();  // not sticky: the next call starts clean
   return decode_error(GPTOSS_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 

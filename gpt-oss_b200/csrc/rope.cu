@@ -195,7 +195,7 @@ static bool rope_vector_fits(const gptoss_rope_args_t &a, int v, int size) {
 }
 
 template <typename T, int V>
-static void rope_launch(const gptoss_rope_args_t &a, int sms, cudaStream_t st) {
+static int rope_launch(const gptoss_rope_args_t &a, int sms, cudaStream_t st) {
   // rows per CTA: enough CTAs for two waves before a CTA takes more rows
   int rows_per_cta = 1;
   while (rows_per_cta < kRopeRows && a.n_rows / (4 * rows_per_cta) >= sms) rows_per_cta *= 2;
@@ -209,10 +209,13 @@ static void rope_launch(const gptoss_rope_args_t &a, int sms, cudaStream_t st) {
   const int passes = (items + most - 1) / most;
   const int threads = std::max(32, (((items + passes - 1) / passes) + 31) & ~31);
   const size_t smem = static_cast<size_t>(rows_per_cta) * (a.rotary_dim / 2) * sizeof(float2);
-  if (a.interleaved)
-    rope_append_kernel<T, V, true><<<grid, threads, smem, st>>>(a, rows_per_cta);
-  else
-    rope_append_kernel<T, V, false><<<grid, threads, smem, st>>>(a, rows_per_cta);
+  auto kernel = a.interleaved ? rope_append_kernel<T, V, true> : rope_append_kernel<T, V, false>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  return launch_result("rope_append", cudaLaunchKernelEx(&cfg, kernel, a, rows_per_cta));
 }
 
 }  // namespace gptoss
@@ -260,25 +263,14 @@ extern "C" int gptoss_decode_rope_append(const gptoss_rope_args_t *args, void *s
   if (dev.code) return dev.code;
   const int sms = sm_count(dev.device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a.dtype == GPTOSS_DTYPE_FP32) {
-    if (rope_vector_fits(a, 4, 4))
-      rope_launch<float, 4>(a, sms, st);
-    else
-      rope_launch<float, 1>(a, sms, st);
-  } else if (a.dtype == GPTOSS_DTYPE_BF16) {
-    if (rope_vector_fits(a, 8, 2))
-      rope_launch<bf16, 8>(a, sms, st);
-    else if (rope_vector_fits(a, 4, 2))
-      rope_launch<bf16, 4>(a, sms, st);
-    else
-      rope_launch<bf16, 1>(a, sms, st);
-  } else {
-    if (rope_vector_fits(a, 8, 2))
-      rope_launch<__half, 8>(a, sms, st);
-    else if (rope_vector_fits(a, 4, 2))
-      rope_launch<__half, 4>(a, sms, st);
-    else
-      rope_launch<__half, 1>(a, sms, st);
+  if (a.dtype == GPTOSS_DTYPE_FP32)
+    return rope_vector_fits(a, 4, 4) ? rope_launch<float, 4>(a, sms, st) : rope_launch<float, 1>(a, sms, st);
+  if (a.dtype == GPTOSS_DTYPE_BF16) {
+    if (rope_vector_fits(a, 8, 2)) return rope_launch<bf16, 8>(a, sms, st);
+    if (rope_vector_fits(a, 4, 2)) return rope_launch<bf16, 4>(a, sms, st);
+    return rope_launch<bf16, 1>(a, sms, st);
   }
-  return launch_result("rope_append");
+  if (rope_vector_fits(a, 8, 2)) return rope_launch<__half, 8>(a, sms, st);
+  if (rope_vector_fits(a, 4, 2)) return rope_launch<__half, 4>(a, sms, st);
+  return rope_launch<__half, 1>(a, sms, st);
 }

@@ -1,4 +1,5 @@
-"""How the handle-free operators may be called: from several host threads at once."""
+"""How the handle-free operators may be called: from several host threads at once, and after a
+failed call of something else."""
 import ctypes
 import threading
 
@@ -108,3 +109,54 @@ def test_all_operators_from_threads_of_their_own(pkg):
     torch.cuda.synchronize()
     assert not raised, raised[0]
     assert all(torch.equal(c[0], w) for c, w in zip(calls, want))
+
+
+def _small_calls(pkg):
+    """name -> (output, function that fills it on a stream), with fixed inputs."""
+    import torch
+
+    dev = torch.device("cuda:0")
+    gen = torch.Generator(device=dev).manual_seed(5)
+    q = torch.randn(40, 8, 64, generator=gen, device=dev).bfloat16()
+    k, v = (torch.randn(90, 2, 64, generator=gen, device=dev).bfloat16() for _ in range(2))
+    one = torch.tensor([0], dtype=torch.int64, device=dev)
+    length = torch.tensor([90], dtype=torch.int32, device=dev)
+    pos = torch.arange(40, dtype=torch.int32, device=dev)
+    inv = torch.from_numpy(pkg.rope_table(64, 10000.0)[0]).to(dev)
+    logits, u = torch.randn(6, 900, generator=gen, device=dev), torch.rand(6, generator=gen, device=dev)
+
+    def attend(n):
+        start = torch.tensor([0, n], dtype=torch.int32, device=dev)
+        return torch.zeros_like(q[:n]), lambda out, st: pkg.prompt_attention(q[:n], k, v, start, one, length, out,
+                                                                             stream=st)
+
+    return {"prompt": attend(40), "token": attend(1),
+            "rope": (torch.zeros_like(q), lambda out, st: pkg.rope_append(q, None, None, pos, inv, q_out=out, stream=st)),
+            "sample": (torch.zeros(6, dtype=torch.int32, device=dev),
+                       lambda out, st: pkg.sample_tokens(logits, u, out, stream=st))}
+
+
+def _failed_create(pkg):
+    """An engine whose cache no GPU holds: its allocation is refused."""
+    from gpt_oss_b200 import synth
+
+    with pytest.raises(pkg.MoeError) as ei:
+        pkg.DecodeEngine(dict(synth.MINI_MODEL, seq_len=1 << 30), 64)
+    assert ei.value.code == pkg.GPTOSS_E_CUDA and "allocation" in str(ei.value)
+
+
+@pytest.mark.parametrize("which", ["prompt", "token", "rope", "sample"])
+def test_an_earlier_failure_is_not_the_operators(pkg, which):
+    """An error that another call left on the thread does not make a launched operator fail."""
+    import torch
+
+    out, call = _small_calls(pkg)[which]
+    st = torch.cuda.current_stream().cuda_stream
+    call(out, st)
+    torch.cuda.synchronize()
+    want = out.clone()
+    out.zero_()
+    _failed_create(pkg)
+    call(out, st)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
