@@ -490,6 +490,7 @@ static int dfail(gptoss_decode *h, int code, const char *fmt, ...) {
   va_start(ap, fmt);
   vsnprintf(buf, sizeof(buf), fmt, ap);
   va_end(ap);
+  if (code == GPTOSS_E_CUDA) cudaGetLastError();  // it is reported: the next call starts clean
   if (h)
     h->err = buf;
   else
@@ -680,9 +681,8 @@ static int decode_create(const gptoss_model_config_t *cfg, int max_batch, int ma
   h->moe = moe;
   h->have.assign(c.n_layers + 1, 0u);
   auto bail = [&](int code, const std::string &msg) {
-    g_decode_create_err = msg;
     gptoss_decode_destroy(h);
-    return code;
+    return dfail(nullptr, code, "%s", msg.c_str());
   };
   std::string err;
   const size_t V = c.vocab_size, H = c.hidden_dim, L = c.n_layers, D = c.head_dim;

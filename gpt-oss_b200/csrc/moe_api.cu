@@ -21,6 +21,7 @@ static int fail(const gptoss_moe *h, int code, const char *fmt, ...) {
   va_start(ap, fmt);
   vsnprintf(buf, sizeof(buf), fmt, ap);
   va_end(ap);
+  if (code == GPTOSS_E_CUDA) cudaGetLastError();  // it is reported: the next call starts clean
   if (h)
     h->err = buf;
   else

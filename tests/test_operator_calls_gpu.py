@@ -160,3 +160,23 @@ def test_an_earlier_failure_is_not_the_operators(pkg, which):
     call(out, st)
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("kind", ["decode", "moe"])
+def test_an_engine_outlives_the_failed_creation_of_another(pkg, tmp_path, kind):
+    """The creation that fails leaves no error behind for the calls of an engine that is there."""
+    from gpt_oss_b200 import synth
+
+    cfg = dict(synth.MINI_MODEL, vocab_size=300, n_layers=1)
+    synth.write_model_bin(tmp_path / "m.bin", cfg, 1)
+    eng = pkg.DecodeEngine(cfg, 2)
+    eng.load_bin(np.fromfile(tmp_path / "m.bin", dtype=np.uint8))
+    want = eng.step([5, 7], [0, 0])
+    if kind == "decode":
+        _failed_create(pkg)
+    else:
+        with pytest.raises(pkg.MoeError) as ei:
+            pkg.MoeEngine(1 << 16, 128, 8, 4, max_tokens=1 << 24)  # rows of 9 TB
+        assert ei.value.code == pkg.GPTOSS_E_CUDA
+    assert (eng.step([5, 7], [0, 0]) == want).all()
+    eng.close()
