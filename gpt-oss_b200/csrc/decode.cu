@@ -469,6 +469,7 @@ struct gptoss_decode {
   // prompt passes and sampling settings: device copies and their pinned sources
   unsigned char *prompt_dev = nullptr, *prompt_host = nullptr;
   float *samp_dev = nullptr, *samp_host = nullptr;  // u | temperature | top_p | min_p | top_k
+  cudaEvent_t inputs_read = nullptr;  // a call's copies out of pinned memory
   // QKV and output projections on this library's tcgen05 kernel (one "expert" = all rows)
   bool own_gemm = true;
   int num_sms = 0, sched_B = -1, sched_cap = 0;
@@ -619,6 +620,7 @@ int gptoss_decode_destroy(gptoss_decode_t *h) {
   if (h->prompt_host) cudaFreeHost(h->prompt_host);
   if (h->samp_host) cudaFreeHost(h->samp_host);
   if (h->h_pinned) cudaFreeHost(h->h_pinned);
+  if (h->inputs_read) cudaEventDestroy(h->inputs_read);
   delete h;
   return GPTOSS_OK;
 }
@@ -714,6 +716,7 @@ static int decode_create(const gptoss_model_config_t *cfg, int max_batch, int ma
   A(cudaMallocHost(reinterpret_cast<void **>(&h->samp_host), 5 * B * sizeof(float)));
   A(cudaDeviceGetAttribute(&h->num_sms, cudaDevAttrMultiProcessorCount, device));
   A(cudaMallocHost(reinterpret_cast<void **>(&h->h_pinned), 3 * B * sizeof(int)));
+  A(cudaEventCreateWithFlags(&h->inputs_read, cudaEventDisableTiming));
   if (e == cudaSuccess) e = cudaMemset(h->status, 0, sizeof(int));
   if (e == cudaSuccess) e = cudaMemset(h->x, 0, R * H * sizeof(bf16));
   if (e != cudaSuccess) return bail(GPTOSS_E_CUDA, std::string("allocation: ") + cudaGetErrorString(e));
@@ -1110,10 +1113,28 @@ static int run_layers(gptoss_decode *h, int B, const int *tokens, const int *pos
   return GPTOSS_OK;
 }
 
+// The settings of the draws, n of each, into the operator's arguments (their copies are queued).
+static int upload_sampling(gptoss_decode *h, const gptoss_decode_sampling_t *sampling, int n,
+                           gptoss_sample_args_t *draw, cudaStream_t st) {
+  const size_t stride = h->max_batch;
+  auto put = [&](int i, const void *src) -> float * {
+    if (!src) return nullptr;
+    memcpy(h->samp_host + i * stride, src, n * sizeof(float));
+    return h->samp_dev + i * stride;
+  };
+  draw->u = put(0, sampling->u);
+  draw->temperature = put(1, sampling->temperature);
+  draw->top_p = put(2, sampling->top_p);
+  draw->min_p = put(3, sampling->min_p);
+  draw->top_k = reinterpret_cast<const int *>(put(4, sampling->top_k));
+  DCK(h, cudaMemcpyAsync(h->samp_dev, h->samp_host, 5 * stride * sizeof(float), cudaMemcpyHostToDevice, st));
+  return GPTOSS_OK;
+}
+
 // Final norm of B residual rows, logits, and the next tokens into h->d_next: the argmax, or a
-// draw.  pos: inactive rows (NULL: none).
-static int finish_rows(gptoss_decode *h, const bf16 *x, int B, const int *pos,
-                       const gptoss_decode_sampling_t *sampling, cudaStream_t st) {
+// draw with the settings in *draw.  pos: inactive rows (NULL: none).
+static int finish_rows(gptoss_decode *h, const bf16 *x, int B, const int *pos, gptoss_sample_args_t *draw,
+                       cudaStream_t st) {
   const gptoss_model_config_t &c = h->cfg;
   const int H = c.hidden_dim, V = c.vocab_size;
   int rc;
@@ -1126,31 +1147,18 @@ static int finish_rows(gptoss_decode *h, const bf16 *x, int B, const int *pos,
     rc = gemm_xwt(h, h->t, h->unemb, h->logits, B, V, H, st);
   }
   if (rc) return rc;
-  if (!sampling) {
+  if (!draw) {
     argmax_rows_kernel<<<B, 256, 0, st>>>(h->logits, pos, h->d_next, V);
     DCK(h, cudaGetLastError());
     return GPTOSS_OK;
   }
-  const size_t n = B, stride = h->max_batch;
-  gptoss_sample_args_t a = {};
-  auto put = [&](int i, const void *src) -> float * {
-    if (!src) return nullptr;
-    memcpy(h->samp_host + i * stride, src, n * sizeof(float));
-    return h->samp_dev + i * stride;
-  };
-  a.logits = h->logits;
-  a.u = put(0, sampling->u);
-  a.temperature = put(1, sampling->temperature);
-  a.top_p = put(2, sampling->top_p);
-  a.min_p = put(3, sampling->min_p);
-  a.top_k = reinterpret_cast<const int *>(put(4, sampling->top_k));
-  DCK(h, cudaMemcpyAsync(h->samp_dev, h->samp_host, 5 * stride * sizeof(float), cudaMemcpyHostToDevice, st));
-  a.pos = pos;
-  a.next = h->d_next;
-  a.stride = a.vocab = V;
-  a.n_rows = B;
-  a.dtype = GPTOSS_DTYPE_FP32;
-  rc = gptoss_decode_sample(&a, st);
+  draw->logits = h->logits;
+  draw->pos = pos;
+  draw->next = h->d_next;
+  draw->stride = draw->vocab = V;
+  draw->n_rows = B;
+  draw->dtype = GPTOSS_DTYPE_FP32;
+  rc = gptoss_decode_sample(draw, st);
   return rc ? dfail(h, rc, "%s", gptoss_decode_last_error(nullptr)) : GPTOSS_OK;
 }
 
@@ -1171,6 +1179,31 @@ static int check_sampling(gptoss_decode *h, const gptoss_decode_sampling_t *s) {
   return GPTOSS_OK;
 }
 
+// The next call writes the pinned inputs and the engine's buffers again, on any stream.  A call that
+// succeeds waits for its stream, and so does one that fails half-way; under expert parallelism
+// that could be a wait for ranks which failed too, so there it only waits for its copies.
+static int after_failure(gptoss_decode *h, int rc, cudaStream_t st) {
+  if (h->moe->ep_size > 1)
+    cudaEventSynchronize(h->inputs_read);
+  else
+    cudaStreamSynchronize(st);
+  return rc;
+}
+
+static int launch_step(gptoss_decode *h, const int *tokens, const int *pos, int B,
+                       const gptoss_decode_sampling_t *sampling, cudaStream_t st) {
+  int *hp = h->h_pinned, rc;
+  memcpy(hp, tokens, B * sizeof(int));
+  memcpy(hp + h->max_batch, pos, B * sizeof(int));
+  DCK(h, cudaMemcpyAsync(h->d_tokens, hp, B * sizeof(int), cudaMemcpyHostToDevice, st));
+  DCK(h, cudaMemcpyAsync(h->d_pos, hp + h->max_batch, B * sizeof(int), cudaMemcpyHostToDevice, st));
+  gptoss_sample_args_t draw = {};
+  if (sampling && (rc = upload_sampling(h, sampling, B, &draw, st))) return rc;
+  DCK(h, cudaEventRecord(h->inputs_read, st));
+  if ((rc = run_layers(h, B, h->d_tokens, h->d_pos, nullptr, st))) return rc;
+  return finish_rows(h, h->x, B, h->d_pos, sampling ? &draw : nullptr, st);
+}
+
 int gptoss_decode_step(gptoss_decode_t *h, const int *tokens, const int *pos, int B, int *next,
                        void *stream) {
   return gptoss_decode_step_sample(h, tokens, pos, B, nullptr, next, stream);
@@ -1188,16 +1221,68 @@ int gptoss_decode_step_sample(gptoss_decode_t *h, const int *tokens, const int *
     if (pos[i] >= c.seq_len) return dfail(h, GPTOSS_E_CAPACITY, "row %d: position %d >= seq_len %d", i, pos[i], c.seq_len);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   DCK(h, cudaSetDevice(h->device));
-  int *hp = h->h_pinned;
-  memcpy(hp, tokens, B * sizeof(int));
-  memcpy(hp + h->max_batch, pos, B * sizeof(int));
-  DCK(h, cudaMemcpyAsync(h->d_tokens, hp, B * sizeof(int), cudaMemcpyHostToDevice, st));
-  DCK(h, cudaMemcpyAsync(h->d_pos, hp + h->max_batch, B * sizeof(int), cudaMemcpyHostToDevice, st));
-  int rc;
-  if ((rc = run_layers(h, B, h->d_tokens, h->d_pos, nullptr, st)) ||
-      (rc = finish_rows(h, h->x, B, h->d_pos, sampling, st)))
-    return rc;
-  return read_next(h, B, next, st);
+  const int rc = launch_step(h, tokens, pos, B, sampling, st);
+  return rc ? after_failure(h, rc, st) : read_next(h, B, next, st);
+}
+
+// The passes of a prefill whose arguments have been checked, and the next tokens.
+static int launch_prefill(gptoss_decode *h, const int *tokens, const int *rows, const int *pos0, const int *lens,
+                          int n_seqs, const gptoss_decode_sampling_t *sampling, cudaStream_t st) {
+  const gptoss_model_config_t &c = h->cfg;
+  gptoss_sample_args_t draw = {};
+  if (sampling)
+    if (int rc = upload_sampling(h, sampling, n_seqs, &draw, st)) return rc;
+  const PromptLayout at(h->max_rows, h->max_batch);
+  unsigned char *hp = h->prompt_host, *dp = h->prompt_dev;
+  auto host = [&](size_t off) { return reinterpret_cast<int *>(hp + off); };
+  auto dev = [&](size_t off) { return reinterpret_cast<int *>(dp + off); };
+  int seq = 0, done = 0;  // tokens of sequence `seq` that went through so far
+  const int *next_token = tokens;
+  while (seq < n_seqs) {
+    // as many tokens as a pass takes; a prompt that does not fit goes on in the next pass, on
+    // top of what is in the cache by then
+    PromptPass pass = {};
+    int last = 0;
+    while (seq < n_seqs && pass.tokens < h->max_rows) {
+      const int n = std::min(lens[seq] - done, h->max_rows - pass.tokens);
+      const long long base = static_cast<long long>(rows[seq]) * c.seq_len;
+      host(at.q_start)[pass.seqs] = pass.tokens;
+      host(at.kv_len)[pass.seqs] = pos0[seq] + done + n;
+      reinterpret_cast<long long *>(hp + at.kv_start)[pass.seqs] = base;
+      for (int j = 0; j < n; j++) {
+        const int p = pos0[seq] + done + j, r = pass.tokens + j;
+        host(at.tokens)[r] = *next_token++;
+        host(at.pos)[r] = p;
+        reinterpret_cast<long long *>(hp + at.slots)[r] = base + p;
+      }
+      pass.max_kv_len = std::max(pass.max_kv_len, pos0[seq] + done + n);
+      pass.tokens += n;
+      pass.seqs++;
+      done += n;
+      if (done == lens[seq]) {
+        host(at.last_from)[last] = pass.tokens - 1;
+        host(at.last_to)[last++] = seq;
+        seq++;
+        done = 0;
+      }
+    }
+    host(at.q_start)[pass.seqs] = pass.tokens;
+    DCK(h, cudaMemcpyAsync(dp, hp, at.bytes, cudaMemcpyHostToDevice, st));
+    DCK(h, cudaEventRecord(h->inputs_read, st));
+    pass.slots = reinterpret_cast<const long long *>(dp + at.slots);
+    pass.kv_start = reinterpret_cast<const long long *>(dp + at.kv_start);
+    pass.q_start = dev(at.q_start);
+    pass.kv_len = dev(at.kv_len);
+    if (int rc = run_layers(h, pass.tokens, dev(at.tokens), dev(at.pos), &pass, st)) return rc;
+    if (last > 0) {
+      gather_last_rows_kernel<<<(last + 7) / 8, 256, 0, st>>>(h->last_x, h->x, dev(at.last_from),
+                                                              dev(at.last_to), last, c.hidden_dim);
+      DCK(h, cudaGetLastError());
+    }
+    // the pinned image is written again for the next pass
+    if (seq < n_seqs) DCK(h, cudaStreamSynchronize(st));
+  }
+  return finish_rows(h, h->last_x, n_seqs, nullptr, sampling ? &draw : nullptr, st);
 }
 
 int gptoss_decode_prefill(gptoss_decode_t *h, const int *tokens, const int *rows, const int *pos0,
@@ -1235,61 +1320,8 @@ int gptoss_decode_prefill(gptoss_decode_t *h, const int *tokens, const int *rows
   if (n_seqs == 0) return GPTOSS_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   DCK(h, cudaSetDevice(h->device));
-  const PromptLayout at(h->max_rows, h->max_batch);
-  unsigned char *hp = h->prompt_host, *dp = h->prompt_dev;
-  auto host = [&](size_t off) { return reinterpret_cast<int *>(hp + off); };
-  auto dev = [&](size_t off) { return reinterpret_cast<int *>(dp + off); };
-  int seq = 0, done = 0;  // tokens of sequence `seq` that went through so far
-  const int *next_token = tokens;
-  while (seq < n_seqs) {
-    // as many tokens as a pass takes; a prompt that does not fit goes on in the next pass, on
-    // top of what is in the cache by then
-    PromptPass pass = {};
-    int last = 0;
-    while (seq < n_seqs && pass.tokens < h->max_rows) {
-      const int n = std::min(lens[seq] - done, h->max_rows - pass.tokens);
-      const long long base = static_cast<long long>(rows[seq]) * c.seq_len;
-      host(at.q_start)[pass.seqs] = pass.tokens;
-      host(at.kv_len)[pass.seqs] = pos0[seq] + done + n;
-      reinterpret_cast<long long *>(hp + at.kv_start)[pass.seqs] = base;
-      for (int j = 0; j < n; j++) {
-        const int p = pos0[seq] + done + j, r = pass.tokens + j;
-        host(at.tokens)[r] = *next_token++;
-        host(at.pos)[r] = p;
-        reinterpret_cast<long long *>(hp + at.slots)[r] = base + p;
-      }
-      pass.max_kv_len = std::max(pass.max_kv_len, pos0[seq] + done + n);
-      pass.tokens += n;
-      pass.seqs++;
-      done += n;
-      if (done == lens[seq]) {
-        host(at.last_from)[last] = pass.tokens - 1;
-        host(at.last_to)[last++] = seq;
-        seq++;
-        done = 0;
-      }
-    }
-    host(at.q_start)[pass.seqs] = pass.tokens;
-    DCK(h, cudaMemcpyAsync(dp, hp, at.bytes, cudaMemcpyHostToDevice, st));
-    pass.slots = reinterpret_cast<const long long *>(dp + at.slots);
-    pass.kv_start = reinterpret_cast<const long long *>(dp + at.kv_start);
-    pass.q_start = dev(at.q_start);
-    pass.kv_len = dev(at.kv_len);
-    int rc = run_layers(h, pass.tokens, dev(at.tokens), dev(at.pos), &pass, st);
-    if (rc) {
-      cudaStreamSynchronize(st);  // the next call writes the pinned image again
-      return rc;
-    }
-    if (last > 0) {
-      gather_last_rows_kernel<<<(last + 7) / 8, 256, 0, st>>>(h->last_x, h->x, dev(at.last_from),
-                                                              dev(at.last_to), last, c.hidden_dim);
-      DCK(h, cudaGetLastError());
-    }
-    // the pinned image is written again for the next pass
-    if (seq < n_seqs) DCK(h, cudaStreamSynchronize(st));
-  }
-  int rc = finish_rows(h, h->last_x, n_seqs, nullptr, sampling, st);
-  return rc ? rc : read_next(h, n_seqs, next, st);
+  const int rc = launch_prefill(h, tokens, rows, pos0, lens, n_seqs, sampling, st);
+  return rc ? after_failure(h, rc, st) : read_next(h, n_seqs, next, st);
 }
 
 int gptoss_decode_get_logits(gptoss_decode_t *h, int row, float *logits_host) {

@@ -209,3 +209,61 @@ def test_null_handles(pkg):
     lib = pkg.load_library()
     assert lib.gptoss_decode_prefill(None, None, None, None, None, 0, None, None, None) == pkg.GPTOSS_E_INVALID
     assert lib.gptoss_decode_step_sample(None, None, None, 1, None, None, None) == pkg.GPTOSS_E_INVALID
+
+
+UNFINISHED = """
+import ctypes, sys
+sys.path[:0] = [{root!r}]
+ctypes.CDLL({blas!r}, mode=ctypes.RTLD_GLOBAL)  # answers every cublasCreate with an error
+import numpy as np
+import __graft_entry__ as entry
+pkg = entry.load_package()
+from gpt_oss_b200 import synth
+cfg = dict(synth.MINI_MODEL, vocab_size=901, n_layers=1)  # (logits of such rows go to cuBLAS)
+eng = pkg.DecodeEngine(cfg, 2, max_tokens=16)
+eng.load_bin(np.fromfile({model!r}, dtype=np.uint8))
+cuda = ctypes.CDLL("libcuda.so.1")
+big, size = ctypes.c_uint64(), 4 << 30
+assert cuda.cuMemAlloc_v2(ctypes.byref(big), ctypes.c_size_t(size)) == 0
+before = ctypes.c_void_p()
+assert cuda.cuEventCreate(ctypes.byref(before), 0) == 0
+step = {step!r}
+for again in range(2):  # the second call builds no schedule, which would wait for the stream
+    for i in range(40):
+        assert cuda.cuMemsetD8Async(big, ctypes.c_ubyte(i), ctypes.c_size_t(size), None) == 0
+    assert cuda.cuEventRecord(before, None) == 0  # what the call's copies have to wait for
+    try:
+        if step:
+            eng.step([3, 4], [0, 0], sampling=dict(u=[0.5, 0.5]))
+        else:
+            eng.prefill([np.arange(10), np.arange(6)], [0, 1])
+        raise SystemExit("the call did not fail")
+    except pkg.MoeError as e:
+        assert "cublasCreate" in str(e), e
+    pending = cuda.cuEventQuery(before)
+    assert cuda.cuCtxSynchronize() == 0
+print("still to be read" if pending else "inputs read")
+"""
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("step", [False, True])
+def test_a_failed_call_has_read_its_pinned_inputs(pkg, tmp_path, step):
+    """A call that fails after its copies were queued waits for them: the next call writes the
+    same pinned memory.  The failure is cuBLAS refusing to start (a stand-in library)."""
+    import pathlib
+    import subprocess
+    import sys
+
+    from gpt_oss_b200 import synth
+
+    src, lib = tmp_path / "blas.c", tmp_path / "libcublas.so.12"
+    src.write_text("int cublasCreate_v2(void **h) { (void)h; return 1; }\nint cublasDestroy_v2(void *h) { (void)h; return 0; }\n"
+                   "int cublasSetStream_v2(void *h, void *s) { (void)h; (void)s; return 1; }\nint cublasGemmEx(void) { return 1; }\n")
+    subprocess.run(["gcc", "-shared", "-fPIC", "-Wl,-soname,libcublas.so.12", "-o", str(lib), str(src)], check=True)
+    model = tmp_path / "model.bin"
+    synth.write_model_bin(model, dict(synth.MINI_MODEL, vocab_size=901, n_layers=1), 3)
+    code = UNFINISHED.format(root=str(pathlib.Path(__file__).resolve().parents[1]), blas=str(lib),
+                             model=str(model), step=step)
+    res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and "inputs read" in res.stdout, res.stdout + res.stderr
