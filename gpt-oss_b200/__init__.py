@@ -678,8 +678,8 @@ class DecodeEngine:
         "u" and any of "temperature", "top_k", "top_p", "min_p" (one entry per row)."""
         tokens = np.ascontiguousarray(tokens, dtype=np.int32)
         pos = np.ascontiguousarray(pos, dtype=np.int32)
-        if tokens.ndim != 1 or pos.shape != tokens.shape:
-            raise ValueError("tokens and pos must be 1-D of one length")
+        if tokens.size < tokens.shape[0] or pos.size < tokens.shape[0]:
+            raise ValueError(f"tokens and pos must have an entry for each of the {tokens.shape[0]} rows")
         nxt = np.empty(tokens.shape[0], dtype=np.int32)
         if sampling is None:
             self._check(self.lib.gptoss_decode_step(self.handle, _ptr(tokens), _ptr(pos),

@@ -117,3 +117,28 @@ def test_operator_structs_match_header(pkg):
                  for w in line.split(",")]
         assert order == [f[0] for f in mirror._fields_]
         assert ctypes.sizeof(mirror) == struct.calcsize(pack)
+
+
+def test_step_takes_rows_as_lists_columns_and_longer_positions(pkg):
+    """What the binding hands to a step: an entry for each of the rows of `tokens`, whatever more
+    `pos` holds (a buffer for the whole batch) and whether the ids come as a column; fewer
+    positions than tokens are refused."""
+    import numpy as np
+
+    class Library:
+        def gptoss_decode_step(self, handle, tokens, pos, batch, nxt, stream):
+            ints = [np.ctypeslib.as_array(ctypes.cast(p, ctypes.POINTER(ctypes.c_int)), (batch,))
+                    for p in (tokens, pos, nxt)]
+            self.seen = ints[0].tolist(), ints[1].tolist()
+            ints[2][:] = ints[0] + 1
+            return 0
+
+    eng = object.__new__(pkg.DecodeEngine)
+    eng.lib, eng.handle = Library(), None
+    for tokens, pos in (([5, 6, 7], [1, 2, 3]), ([5, 6, 7], [1, 2, 3, -1, -1]),
+                        (np.array([[5], [6], [7]]), [1, 2, 3]), (np.array([5, 6, 7]), np.array([[1], [2], [3]]))):
+        assert eng.step(tokens, pos).tolist() == [6, 7, 8]
+        assert eng.lib.seen == ([5, 6, 7], [1, 2, 3])
+    assert eng.step(5, 1).tolist() == [6]
+    with pytest.raises(ValueError, match="pos"):
+        eng.step([5, 6, 7], [1, 2])
