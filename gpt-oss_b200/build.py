@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import os
 import pathlib
+import re
 import shutil
 import subprocess
 
@@ -59,6 +60,21 @@ def build_library(force: bool = False, verbose: bool = False) -> pathlib.Path:
     if verbose:
         print(res.stdout + res.stderr)
     return LIB
+
+
+def kernel_resources(source: pathlib.Path) -> dict:
+    """Compiles one CUDA source by itself and returns what the assembler reports of its kernels:
+    mangled name -> (registers of a thread, bytes of spill stores, bytes of spill loads)."""
+    flags = [f for f in NVCC_FLAGS if f != "-shared"]
+    cmd = [_nvcc(), *flags, "-Xptxas=-v", "-cubin", "-o", os.devnull, str(source)]
+    if os.path.exists("/usr/bin/g++"):
+        cmd[1:1] = ["-ccbin", "/usr/bin/g++"]
+    res = subprocess.run(cmd, cwd=str(CSRC), capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
+    found = re.findall(r"Compiling entry function '(\w+)'.*?(\d+) bytes spill stores, (\d+) bytes spill loads"
+                       r".*?Used (\d+) registers", res.stdout + res.stderr, re.S)
+    return {name: (int(regs), int(stores), int(loads)) for name, stores, loads, regs in found}
 
 
 HOST_LIB = PKG_DIR / "libgptoss_getp_b200.so"

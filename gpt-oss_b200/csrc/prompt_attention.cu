@@ -52,7 +52,14 @@
 namespace gptoss {
 
 constexpr int kAttnThreads = 640;
+// Registers of a thread at launch: the bound on the threads leaves 65536 / 640, in steps of 8, and
+// a kernel that moves registers between its warps is given all of them.  Those warps' shares.
+constexpr int kAttnRegs = 65536 / kAttnThreads / 8 * 8;
+constexpr int kAttnRegsSoftmax = 104, kAttnRegsOther = 64;
 constexpr int kAttnSoftmaxWarps = 16;
+static_assert(32 * kAttnSoftmaxWarps * kAttnRegsSoftmax + (kAttnThreads - 32 * kAttnSoftmaxWarps) * kAttnRegsOther <=
+                  kAttnThreads * kAttnRegs,
+              "the warps would wait for ever for registers that the launch did not bring");
 constexpr int kAttnTmemCols = 512;
 constexpr int kAttnMaxSplit = 8;      // CTAs of a cluster that share a pair of tiles
 constexpr int kAttnNarrow = 512;      // widest window that takes units of 64 keys at head_dim <= 64
@@ -360,7 +367,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
   // Registers: 640 threads were launched with 96 each (61440); the four warps that hold no
   // tiles keep 64 and the sixteen that do take 104 (128 * 64 + 512 * 104 = 61440).
   if (warp >= kAttnSoftmaxWarps) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kAttnRegsOther));
     if (warp == 16) {
       // -------------------------------------------------------------- jobs and loads
       // The grid has a CTA (with a split: a cluster) per pair of tiles; this CTA does its own
@@ -539,7 +546,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q,
     }
   } else {
     // ---------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kAttnRegsSoftmax));
     code = kStatusWaitTimeoutEpilogue;
     // two warps per 32 rows: a thread has a row and half of a unit's keys
     constexpr int kMine = KEYS / 2, kParts = kMine / 32;
@@ -834,12 +841,11 @@ static int attention_launch(const gptoss_attention_args_t &a, int sms, cudaStrea
   // Kernel attributes first: a host thread that has made no CUDA call yet has no context, these
   // give it the device's, and the encoding of the tensor maps fails without one.
   auto kernel = prompt_attention_kernel<T, D, KEYS>;
-  // the kernel's warps share out the registers of a launch with 96 each: with fewer they would
-  // wait for more for ever
+  // with fewer registers than its warps share out they would wait for more for ever
   cudaFuncAttributes fa = {};
   cudaError_t e = cudaFuncGetAttributes(&fa, kernel);
-  if (e == cudaSuccess && fa.numRegs != 96)
-    return decode_error(GPTOSS_E_STATE, "prompt_attention: built with %d registers, not 96", fa.numRegs);
+  if (e == cudaSuccess && fa.numRegs != kAttnRegs)
+    return decode_error(GPTOSS_E_STATE, "prompt_attention: built with %d registers, not %d", fa.numRegs, kAttnRegs);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes);
   if (e != cudaSuccess) return launch_result("prompt_attention", e);
   CUtensorMap map_q, map_k, map_v;
