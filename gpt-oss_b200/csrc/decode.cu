@@ -975,7 +975,9 @@ static int read_status(gptoss_decode *h) {
   DCK(h, cudaMemcpy(&dev_status, h->status, sizeof(int), cudaMemcpyDeviceToHost));
   if (dev_status) {
     cudaMemset(h->status, 0, sizeof(int));
-    return dfail(h, GPTOSS_E_DEVICE, "a decode kernel reported status %d (token id out of range?)", dev_status);
+    return dfail(h, GPTOSS_E_DEVICE,
+                 "a decode kernel reported status %d (101-103: a pipeline wait ran out, 104: a token id, or the "
+                 "rows or keys of a prompt, out of range)", dev_status);
   }
   // the MoE engine keeps its own status word: pipeline and peer-flag waits that ran out
   if (gptoss_moe_take_status(h->moe) != GPTOSS_OK)

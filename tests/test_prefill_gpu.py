@@ -267,3 +267,20 @@ def test_a_failed_call_has_read_its_pinned_inputs(pkg, tmp_path, step):
                              model=str(model), step=step)
     res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert res.returncode == 0 and "inputs read" in res.stdout, res.stdout + res.stderr
+
+
+@pytest.mark.gpu
+def test_a_reported_status_is_not_taken_for_a_token_id_alone(pkg, tmp_path):
+    """The engine's kernels share a status word; the error's text names what its values mean."""
+    from gpt_oss_b200 import synth
+
+    cfg = dict(synth.MINI_MODEL, vocab_size=300, n_layers=1)
+    eng = _engine(pkg, cfg, 2, tmp_path, 2, 16)
+    want = eng.prefill([[5, 6]], [1])
+    with pytest.raises(pkg.MoeError) as ei:
+        eng.step([300, 5], [0, 0])
+    text = str(ei.value)
+    assert ei.value.code == pkg.GPTOSS_E_DEVICE and "status 104" in text
+    assert "101-103" in text and "wait" in text and "token id" in text and "keys of a prompt" in text
+    assert (eng.prefill([[5, 6]], [1]) == want).all()  # reported once
+    eng.close()
