@@ -152,11 +152,13 @@ int gptoss_decode_create_prefill(const gptoss_model_config_t *cfg, int max_batch
  * (packed, host) and goes to cache row rows[i], positions pos0[i] .. pos0[i] + lens[i] - 1;
  * pos0[i] > 0 continues what that row holds.  The rows of one call are different.  next[i]
  * receives the token after the last one of sequence i: the argmax, or drawn as `sampling` says.
- * Same arithmetic as the step except for the order of sums in the attention and its
- * probabilities, which are rounded to bf16 there too; the cache it leaves is what the steps
- * leave.  Prompts longer than max_tokens, and as many of them as do not fit, go through in
- * several passes.  All tokens and positions are checked first; a call that is refused has
- * changed nothing.  Synchronises the stream.  Not under expert parallelism (GPTOSS_E_STATE).
+ * Same arithmetic as the step except in the attention: the order of its sums, its exponentials
+ * (see gptoss_decode_prompt_attention), and q, which the step multiplies by 1 / sqrt(head_dim)
+ * before it rounds it to bf16 and the prefill rounds unscaled (the same bits where head_dim is
+ * 64).  The cache it leaves is what the steps leave, but for roundings that fall the other way.
+ * Prompts longer than max_tokens, and as many of them as do not fit, go through in several
+ * passes.  All tokens and positions are checked first; a call that is refused has changed
+ * nothing.  Synchronises the stream.  Not under expert parallelism (GPTOSS_E_STATE).
  */
 int gptoss_decode_prefill(gptoss_decode_t *h, const int *tokens, const int *rows, const int *pos0,
                           const int *lens, int n_seqs, const gptoss_decode_sampling_t *sampling,
@@ -201,7 +203,7 @@ int gptoss_decode_rope_table(int rotary_dim, float theta, float scaling_factor,
  * i; NULL: row i (n_slots >= n_rows then).  A row whose slot is outside [0, n_slots) is not
  * stored.  Two rows with one slot leave one of them there, element by element undefined.
  * q (with q_out), k (with k_cache) and v (with v_cache) may each be NULL.  k_cache may be k
- * itself when slots is NULL; other overlaps of inputs and outputs are not allowed.
+ * itself (and v_cache v) when slots is NULL; other overlaps of inputs and outputs are not allowed.
  * angle_f32 = 0: the angle is formed in fp64 (exact for every position); 1: pos * inv_freq
  * is rounded to fp32 first, as the reference and gptoss_decode_step do.
  */
@@ -230,8 +232,10 @@ int gptoss_decode_rope_append(const gptoss_rope_args_t *args, void *stream);
  *   k, v    [n_kv_rows, n_kv_heads, head_dim]; its keys are rows kv_start[i] .. + kv_len[i]
  * The last query of a sequence stands at its last key: query j of L sees key t when
  * t <= p and (window == 0 or t > p - window), p = kv_len[i] - L + j.  A query that sees no
- * key (kv_len[i] < L leaves p < 0) gets zeros.  bf16 or fp16, softmax in fp32; the
- * probabilities are rounded to the type before they multiply v, the result once at the end.
+ * key (kv_len[i] < L leaves p < 0) gets zeros.  bf16 or fp16, maxima and sums in fp32; the
+ * exponentials are good to 2^-22 relative, with many query rows per sequence some of them to
+ * 7.5e-5 in bf16 and 2.6e-6 in fp16; the probabilities are rounded to the type before they
+ * multiply v, the result once at the end.  Scores scale * q.k are below 2^26 in magnitude.
  * K and V rows outside every sequence, or that no query of a sequence sees, may hold
  * anything (NaN included); those that some query sees must be finite.
  * Heads are contiguous, rows are `*_stride` elements apart; addresses and strides in bytes
@@ -239,10 +243,15 @@ int gptoss_decode_rope_append(const gptoss_rope_args_t *args, void *stream);
  * 128 times it; out does not overlap the inputs.  q_start is ascending from 0; its last entry
  * may be below n_tokens.  A sequence whose keys leave [0, n_kv_rows) or whose kv_len is negative
  * is left unwritten and reported as status 104; so are entries of q_start that do not ascend or
- * pass n_tokens, and then it is open which rows of out are written.  Rows that belong to no
- * sequence are left unwritten.  Sinks are finite or -infinity (no sink).
+ * pass n_tokens, and then it is open which rows of out are written.  kv_start and kv_len of a
+ * sequence without query rows are not looked at.  Rows that belong to no sequence are left
+ * unwritten.  Sinks are finite or -infinity (no sink); scale is positive and finite.
  * max_kv_len: an upper bound on kv_len that the host knows (0 = not known); it only chooses
  * how the work is split.
+ * One of two kernels takes the whole call: one for single tokens where the sequences, empty ones
+ * included, have on average no more query rows than 16 / (n_q_heads / n_kv_heads), else one for
+ * prompts.  A long prompt with many single tokens beside it is right either way, but faster as
+ * two calls.
  */
 typedef struct {
   const void *q, *k, *v;

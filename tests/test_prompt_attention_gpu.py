@@ -422,3 +422,49 @@ def test_starts_that_do_not_ascend(pkg, starts_of, group):
 ], ids=str)
 def test_wide_windows(pkg, case):
     test_against_64_bits(pkg, case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv", [(8, 1), (2, 2)])
+def test_entries_of_a_sequence_without_queries_do_not_count(pkg, hq, hkv):
+    """Places that a batch of fixed size leaves empty may hold any kv_start and kv_len."""
+    import torch
+
+    dev = torch.device("cuda:0")
+    q_lens, kv_lens = [0, 5, 0, 7, 0], [30, 50, 30, 60, 30]
+    q, k, v, sinks, out, whole, starts = _make(torch, dev, 21, q_lens, kv_lens, hq, hkv, 64, "bfloat16")
+    q_start, kv_start, kv_len = _index(torch, dev, q_lens, starts, kv_lens)
+    want, mag, keys = _reference(q, k, v, q_lens, starts, kv_lens, sinks, 0.125, 0)
+    kv_start[0], kv_len[2], kv_start[4], kv_len[4] = 1 << 40, -9, -1, 1 << 30
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    pkg.prompt_attention(q, k, v, q_start, kv_start, kv_len, out, sinks=sinks, status=status,
+                         stream=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert status.item() == 0
+    _check(out, want, mag, keys, "bfloat16", 10.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d,window", [("bfloat16", 64, 0), ("float16", 64, 0), ("float16", 64, 100),
+                                            ("bfloat16", 128, 0), ("float16", 128, 0), ("bfloat16", 32, 0)])
+@pytest.mark.parametrize("tokens", [1, 150])
+def test_scores_near_the_documented_limit(pkg, dtype, d, window, tokens):
+    """Scores of up to 2^25.5.  Queries and keys are signs times a power of two, so every score is
+    exact: equal patterns tie, others are millions apart, and the result is a mean of values (or
+    nothing, where the sink is above them)."""
+    import torch
+
+    dev = torch.device("cuda:0")
+    q_lens, kv_lens = [tokens, tokens], [700, tokens]
+    q, k, v, sinks, out, whole, starts = _make(torch, dev, 22, q_lens, kv_lens, 8, 2, d, dtype)
+    gen = torch.Generator(device=dev).manual_seed(23)
+    signs = torch.randint(0, 2, (6, d), generator=gen, device=dev).to(q.dtype) * 2 - 1
+    q.copy_(signs[torch.randint(0, 6, q.shape[:2], generator=gen, device=dev)] * 2.0 ** 11)
+    k.copy_(signs[torch.randint(0, 6, k.shape[:2], generator=gen, device=dev)] * 2.0 ** 11)
+    q_start, kv_start, kv_len = _index(torch, dev, q_lens, starts, kv_lens)
+    want, mag, keys = _reference(q, k, v, q_lens, starts, kv_lens, sinks, d ** -0.5, window)
+    for bound in (0, 700):
+        pkg.prompt_attention(q, k, v, q_start, kv_start, kv_len, out, sinks=sinks, window=window,
+                             max_kv_len=bound, stream=torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        _check(out, want, mag, keys, dtype, 10.0)
