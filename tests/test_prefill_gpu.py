@@ -284,3 +284,57 @@ def test_a_reported_status_is_not_taken_for_a_token_id_alone(pkg, tmp_path):
     assert "101-103" in text and "wait" in text and "token id" in text and "keys of a prompt" in text
     assert (eng.prefill([[5, 6]], [1]) == want).all()  # reported once
     eng.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,max_tokens", [((600, 257, 1), 1000), ((600, 257, 1), 512), ((600, 257, 1), 300),
+                                             ((256,), 513), ((257,), 513), ((513,), 513)], ids=str)
+def test_passes_of_more_rows_than_a_tile(pkg, tmp_path, lens, max_tokens):
+    """Passes of one to four row tiles in the projections, the schedule rebuilt between them and
+    for the few rows of the logits, against the same prompts fed token by token."""
+    import torch
+
+    from gpt_oss_b200 import synth
+
+    cfg = dict(synth.MINI_MODEL, vocab_size=900, sliding_window=200, n_layers=2, seq_len=700, n_attn_heads=6,
+               n_kv_heads=2, n_experts=4, experts_per_token=4)
+    rng = np.random.default_rng(17)
+    prompts = [rng.integers(0, 900, n, dtype=np.int32) for n in lens]
+    steps = _engine(pkg, cfg, 6, tmp_path, 4)
+    logits = {}
+    for p in range(max(lens)):  # all sequences side by side, sequence i in row i + 1
+        tok, pos = np.full(4, -1, np.int32), np.full(4, -1, np.int32)
+        for i, prompt in enumerate(prompts):
+            if p < len(prompt):
+                tok[i + 1], pos[i + 1] = prompt[p], p
+        steps.step(tok, pos)
+        for i, prompt in enumerate(prompts):
+            if p == len(prompt) - 1:
+                logits[i] = steps.logits(i + 1)
+    eng = _engine(pkg, cfg, 6, tmp_path, 4, max_tokens)
+    rows = list(range(1, len(lens) + 1))
+    for _ in range(2):  # the second call meets the schedule that the first one left
+        nxt = eng.prefill(prompts, rows)
+        for i, want in logits.items():
+            _close(eng.logits(i), want)
+            assert want.max() - want[nxt[i]] <= 4 * LOGIT_MAX_ABS
+    # Caches.  The two sides' projections may round the other way: a step of bf16, 2^-7 of the
+    # element (1e-5 for sums near zero: 128 products of rows of norm 1 and weights of 0.02, at
+    # 2^-24 each).  Rotation takes two of them to at most 2^-7 of the pair's length (Cauchy), and
+    # both sides round once more, 2^-8 of the element each.
+    dev, d, dkv = torch.device("cuda:0"), cfg["head_dim"], cfg["n_kv_heads"] * cfg["head_dim"]
+    for layer in range(2):
+        for row, n in zip(rows, lens):
+            a = [torch.zeros(1, n, dkv, dtype=torch.bfloat16, device=dev) for _ in range(4)]
+            steps.get_kv(layer, row, 0, a[0], a[1])
+            eng.get_kv(layer, row, 0, a[2], a[3])
+            k0, v0, k1, v1 = (x[0].float().reshape(n, -1, 2, d // 2) for x in a)
+            if layer == 0:
+                length = k0.pow(2).sum(2, keepdim=True).sqrt()
+                assert ((k0 - k1).abs() <= length * 2.0 ** -6 + 2e-5).all()
+                assert ((v0 - v1).abs() <= v0.abs() * 2.0 ** -7 + 1e-5).all()
+            else:
+                assert (k0 - k1).abs().max() <= 0.05 * k0.abs().max()
+                assert (v0 - v1).abs().max() <= 0.05 * v0.abs().max()
+    steps.close()
+    eng.close()
