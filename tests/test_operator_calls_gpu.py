@@ -1,12 +1,16 @@
-"""How the handle-free operators may be called: from several host threads at once, and after a
-failed call of something else."""
+"""How the handle-free operators may be called: from several host threads at once, after a
+failed call of something else, and captured before they have ever run."""
 import ctypes
+import pathlib
+import subprocess
+import sys
 import threading
 
 import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
+ROOT = pathlib.Path(__file__).resolve().parents[1]
 
 
 def _at_once(jobs):
@@ -180,3 +184,33 @@ def test_an_engine_outlives_the_failed_creation_of_another(pkg, tmp_path, kind):
         assert ei.value.code == pkg.GPTOSS_E_CUDA
     assert (eng.step([5, 7], [0, 0]) == want).all()
     eng.close()
+
+
+FIRST_CALL = """
+import sys
+sys.path[:0] = [{root!r}, {tests!r}]
+import torch
+import __graft_entry__ as entry
+import test_operator_calls_gpu as calls
+out, call = calls._small_calls(entry.load_package())[{which!r}]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    call(out, torch.cuda.current_stream().cuda_stream)
+graph.replay()
+torch.cuda.synchronize()
+got = out.clone()
+out.zero_()
+call(out, torch.cuda.current_stream().cuda_stream)
+torch.cuda.synchronize()
+assert out.any() and torch.equal(got, out)
+print("captured")
+"""
+
+
+@pytest.mark.parametrize("which", ["prompt", "token", "rope", "sample"])
+def test_the_first_call_may_be_a_captured_one(which):
+    """In a process of its own, so that nothing of the operator has been loaded before."""
+    code = FIRST_CALL.format(root=str(ROOT), tests=str(ROOT / "tests"), which=which)
+    res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and "captured" in res.stdout, res.stdout + res.stderr
