@@ -468,3 +468,18 @@ def test_scores_near_the_documented_limit(pkg, dtype, d, window, tokens):
                              max_kv_len=bound, stream=torch.cuda.current_stream().cuda_stream)
         torch.cuda.synchronize()
         _check(out, want, mag, keys, dtype, 10.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [
+    ([300] + [0] * 200, [2000] + [0] * 200, 16, 2, 64, 100, True, "bfloat16", 0),
+    ([0] * 200 + [300], [5] * 200 + [2000], 16, 2, 64, 0, False, "float16", 8),
+    ([40, 3, 0, 0], [3000, 700, 9, 0], 4, 4, 64, 0, True, "bfloat16", 0),
+    ([40, 3, 0, 0], [3000, 700, 9, 0], 4, 4, 32, 500, True, "float16", 0),
+    ([10, 0, 2], [5000, 10, 300], 3, 1, 128, 0, False, "bfloat16", 0),
+    ([0, 10, 2], [10, 5000, 300], 3, 1, 128, 77, True, "float16", 0),
+    ([3, 0, 0], [900, 0, 0], 16, 1, 64, 0, True, "bfloat16", 0),
+], ids=str)
+def test_batches_padded_with_empty_sequences(pkg, case):
+    """Few rows on average, many in one sequence: several jobs of the kernel for single tokens."""
+    test_against_64_bits(pkg, case)
