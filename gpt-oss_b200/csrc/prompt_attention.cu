@@ -9,8 +9,8 @@
 // over the same stream of units of KEYS keys.  One CTA per SM:
 //   warps 0-15   softmax, eight per tile: two warps share 32 rows, a thread has a row (a TMEM
 //                lane) and half of a unit's keys
-//   warp 16      the jobs (a CTA takes over the work of CTAs that have not started, longest
-//                jobs first), TMA: Q of both tiles, then K and V units into two rings
+//   warp 16      the jobs (a CTA takes over the work of CTAs that have not started), TMA: Q of
+//                both tiles, then K and V units into two rings
 //   warps 17, 18 the MMAs of either tile, S = Q K^T a unit ahead of O += P V
 // S comes from TMEM into registers whole, so the row maximum costs no second read, and S is
 // free for the next unit's scores while P is being made; P goes back to TMEM as the MMA's
@@ -20,24 +20,30 @@
 //
 // What bounds it: an exponential per (row, key), 16 per cycle and SM.  64 keys of both tiles
 // are 1024 cycles of exponentials against 256 of MMAs at head_dim 64 and 512 at 128; masking,
-// maximum, scaling, sum and packing are issued beside them.  With units of 128 keys one in five
-// pairs of exponentials is therefore computed on the FMA pipes (one prompt of 8192 tokens, 64/8
-// heads of 64: 656 us, 73 % of the exponentials' rate; 740 with none, 680 with one in four); with
-// units of 64 keys that gains nothing (one prompt of 4096 tokens, 32/4 heads of 128: 137 us, 1.0
-// PFLOP/s; 143 with one in eight).  Handing S over earlier is slower (784 us): the late arrival
-// keeps the two tiles out of phase.
+// maximum, scaling, sum and packing are issued beside them.  No pipe is full: one prompt of 8192
+// tokens, 64/8 heads of 64, takes 690 to 725 us call after call, under the power limit (650 in a
+// burst), which is 69 to 66 % (73) of the exponentials' rate; in a prompt of 4096 tokens the
+// tensor pipe is at 36 % and the issue slots are at 61 %.  With units of 128 keys three of 16
+// pairs of exponentials are computed on the FMA pipes.  That share is what measured best in this
+// schedule: none takes 700 us (688 in a burst), four of 16 706 (666).  With units of 64 keys it
+// gains nothing (one prompt of 4096 tokens, 32/4 heads of 128: 139 us, 0.99 PFLOP/s; 142 with two
+// of 16).
 //
 // KEYS: 128 where TMEM holds S, P and O of both tiles (head_dim <= 64), 64 at 128.  A narrow
 // window leaves most of a unit of 128 masked, so 64 are taken there too.  Time with 64 and 128
-// keys of 10 packed prompts (13626 tokens), 64/8 heads of 64, by window: 32 tokens 117 and 125
-// us, 128 133 and 156, 256 170 and 182, 512 231 and 231, 1024 332 and 303, 2048 471 and 418.
+// keys of 10 packed prompts (13626 tokens), 64/8 heads of 64, by window: 32 tokens 112 and 119
+// us, 128 127 and 147, 256 162 and 172, 512 222 and 220, 1024 321 and 309, 2048 460 and 436.
 //
 // Few tiles and long contexts: a cluster of up to 8 CTAs shares one pair of tiles, each taking
 // an equal run of units; the partial (m, l, O) are joined through distributed shared memory, in
 // rank order, so the result does not depend on timing and no workspace is needed.  Only as far
 // as SMs would be idle otherwise: a cluster waits until that many SMs are free at once, and
 // four packed pieces of prompts (3690 tokens, 32/4 heads of 128, contexts up to 16130) took 264
-// us with whole jobs (250 now), 309 with every job in two parts and 471 in four.
+// us with whole jobs, 309 with every job in two parts and 471 in four.
+//
+// Jobs start in the order of their slots, the last one first.  Within a sequence that is the
+// longest first, across sequences it is not: those four pieces take 259 us, and 336 with the one
+// on 16130 keys at the front of the batch, which then starts last.
 //
 // Probabilities are rounded to the 16-bit type for the second product (tensor cores take both
 // operands in one type); their sum is taken in fp32 before that rounding.
@@ -79,7 +85,7 @@ struct AttnShape {
   static constexpr int kColP = 2 * KEYS;
   static constexpr int kColO = D == 128 ? 256 : 384;
   static_assert(3 * KEYS <= kColO && kColO + 2 * D <= kAttnTmemCols, "TMEM");
-  // every kPolyStep-th of 16 pairs of exponentials is computed on the FMA pipes
+  // every kPolyStep-th of 16 pairs of exponentials is computed on the FMA pipes (17: none)
   static constexpr int kPolyStep = KEYS == 64 ? 17 : 5;
   static constexpr int kOperandBytes = 2 * kQBytes + 2 * kRingBytes;
   // fp32 partial outputs of both tiles take the operands' place in a split launch
@@ -886,8 +892,11 @@ static int attention_launch(const gptoss_attention_args_t &a, int sms, cudaStrea
 
 // Few query rows per sequence go to the kernel of token_attention.cu: when a sequence has on
 // average at most the tokens that fill 16 rows, one job there.  (64/8 heads of 64: one token each
-// of 64 sequences with up to 7747 keys 160 us here and 100 there, one of 131071 keys 150 and 59.
-// With more tokens a sequence that kernel reads its K and V once for every 16 rows.)
+// of 64 sequences with up to 7747 keys 152 us here and 98 there, one of 131071 keys 143 and 59.
+// With more tokens a sequence that kernel reads its K and V once for every 16 rows.)  The choice
+// holds for the whole call, so one kind pays where a call mixes them: a prompt of 4000 tokens and
+// 63 single tokens on 8000 keys take 440 us here, 1070 there and 363 as two calls; with 4000
+// single tokens on 512 keys beside it 1350 here, 1980 there and 1200 as two calls.
 static bool rows_are_few(const gptoss_attention_args_t &a) {
   const int group = a.n_q_heads / a.n_kv_heads;
   return group <= 16 && a.n_tokens <= static_cast<long long>(a.n_seqs) * (16 / group);

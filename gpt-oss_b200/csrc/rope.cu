@@ -44,10 +44,11 @@ constexpr int kRopeRows = 8;  // rows of a CTA, at most
 // accesses of v.  A thread takes the same item of every row of the CTA, so that what an item is
 // - two divisions - is found once.  What bounds the kernel is the bytes in flight: interleaved,
 // a thread has four rows' loads on their way (30011 rows of 32 + 2 x 4 heads of 128, half of
-// each rotated: 154 us with one, 103 us with four, a copy of as many bytes 95 us); half-split,
-// one row's two loads and twice as many threads per SM are the better way to have them (8191
-// rows of 64 + 2 x 8 heads of 64: 34 us, against 43 us with four rows or with the halves brought
-// together by shuffles, which read the angles twice as often).
+// each rotated: 134 us with one, 106 us with four, 94 us at a copy's rate); half-split, one row's
+// two loads and twice as many threads per SM are the better way to have them (8191 rows of 64 + 2
+// x 8 heads of 64: 33 us, against 39 us with four rows and half as many threads; 26 us at a copy's
+// rate).  Eight CTAs of 256 threads leave 32 registers, of which the 16-byte accesses spill some
+// (100 bytes stored, 40 loaded).
 template <typename T, int V, bool IL>
 __global__ void __launch_bounds__(IL ? 384 : 256, IL ? 3 : 8)
 rope_append_kernel(const gptoss_rope_args_t a, int rows_per_cta) {

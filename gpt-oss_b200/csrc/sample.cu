@@ -23,10 +23,13 @@
 // overlap (512 rows of 201088 by temperature 251 us, 1.6 TB/s, issue 55 %); with top-p without
 // top-k the weights once more and the shared atomics of the bins, 13 us (96 rows of 50257: 59
 // us); for a few rows the cluster barriers between the steps, 1.3 us each (one row of 201088
-// with all limits 18 us, 64 rows of mixed settings 88).
+// with all limits 16 us in a graph, 64 rows of mixed settings 89).  64 rows of 201088 by top-k
+// alone: 46 us for the first 50, 63 for 512, the most that the sorted list takes, 64 for 513, 96
+// for 20000.
 //
-// A weight has to be good to about 2^-44 relative, not to fp32's 2^-24: with 200000 kept tokens
-// a draw lies within 2^-24 of some running sum every few rows, and would then pick the wrong one.
+// A weight is within half a unit of 2^-44 of the likeliest token's (what is lighter has fewer
+// bits); fp32's 2^-24 would not do: with 200000 kept tokens a draw lies within 2^-24 of some
+// running sum every few rows, and would then pick the wrong one.
 #include <cuda_fp16.h>
 #include <float.h>
 #include <math.h>

@@ -13,11 +13,11 @@
 // block of keys; on 8 rows its warps wait for each other most of the time.
 //
 // What bounds it: the read of K and V.  One token each of 64 sequences with 1 to 7747 keys, 64/8
-// heads of 64: 100 us, 77 % of a copy's rate (the last jobs run alone); one token of 131071
-// keys: 59 us, 69 % (its 8 clusters of 16 CTAs are 128 CTAs, two to an SM, and leave SMs idle).
-// Three blocks are in flight per warp: with two the long token takes 86 us instead of 74 (both
-// with a graph launch), with four an SM holds fewer CTAs (256 sequences of 512 keys: 102 instead
-// of 74).  Clusters of 8 take 88 us for the long token.
+// heads of 64: 98 to 102 us with the same inputs, 105 with new ones for every call, 79 to 74 % of a
+// copy's rate (the last jobs run alone); one token of 131071 keys: 59 us, 69 % (its 8 clusters of
+// 16 CTAs are 128 CTAs, two to an SM, and leave SMs idle).  A ring of three blocks per warp, by
+// those two and 256 sequences of 512 keys: 98, 59 and 66 us; of two 97, 72 and 58; of four, where
+// an SM holds fewer CTAs, 93, 82 and 103.  Clusters of 8 take 75 us for the long token.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
