@@ -247,7 +247,8 @@ int gptoss_decode_rope_append(const gptoss_rope_args_t *args, void *stream);
  * sequence without query rows are not looked at.  Rows that belong to no sequence are left
  * unwritten.  Sinks are finite or -infinity (no sink); scale is positive and finite.
  * max_kv_len: an upper bound on kv_len that the host knows (0 = not known); it only chooses
- * how the work is split.
+ * how the work is split.  (Query rows on more than 10^8 keys may outlast the kernel's waits of
+ * 2 s: status 101 to 103, rows unwritten.)
  * One of two kernels takes the whole call: one for single tokens where the sequences, empty ones
  * included, have on average no more query rows than 16 / (n_q_heads / n_kv_heads), else one for
  * prompts.  A long prompt with many single tokens beside it is right either way, but faster as
