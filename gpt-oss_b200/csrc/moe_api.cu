@@ -75,6 +75,10 @@ int gptoss_moe_create(const gptoss_moe_config_t *cfg, gptoss_moe_t **out) {
   const int ep_rank = ep_size > 1 ? cfg->ep_rank : 0;
   if (ep_rank < 0 || ep_rank >= ep_size || E % ep_size)
     return fail(nullptr, GPTOSS_E_INVALID, "ep_rank/ep_size do not partition n_experts");
+  // row, assignment and tile indices are 32-bit, rounded up to tiles of at most 256
+  if (static_cast<long long>(cfg->max_tokens) * ep_size * K > INT32_MAX - 256)
+    return fail(nullptr, GPTOSS_E_CAPACITY, "max_tokens %d times ranks times experts per token is above 2^31 - 257",
+                cfg->max_tokens);
   if (cfg->weight_format != GPTOSS_WEIGHTS_BF16 && cfg->weight_format != GPTOSS_WEIGHTS_MXFP4)
     return fail(nullptr, GPTOSS_E_INVALID, "unknown weight_format");
   if (cfg->weight_format == GPTOSS_WEIGHTS_MXFP4 && (H % 32 || IM % 32))

@@ -142,3 +142,17 @@ def test_step_takes_rows_as_lists_columns_and_longer_positions(pkg):
     assert eng.step(5, 1).tolist() == [6]
     with pytest.raises(ValueError, match="pos"):
         eng.step([5, 6, 7], [1, 2])
+
+
+def test_batches_whose_assignments_pass_32_bits_are_refused(pkg):
+    """Rows times experts per token index the engine's buffers in 32 bits; refused before the
+    GPU is looked for, for an engine of prompts as well."""
+    from gpt_oss_b200 import synth
+
+    for tokens, k in ((1 << 29, 8), (1 << 28, 8), (2147483647, 1)):
+        with pytest.raises(pkg.MoeError) as ei:
+            pkg.MoeEngine(128, 128, 8, k, max_tokens=tokens)
+        assert ei.value.code == pkg.GPTOSS_E_CAPACITY
+        with pytest.raises(pkg.MoeError) as ei:
+            pkg.DecodeEngine(dict(synth.MINI_MODEL, experts_per_token=k), 1, max_tokens=tokens)
+        assert ei.value.code == pkg.GPTOSS_E_CAPACITY
