@@ -469,7 +469,7 @@ struct gptoss_decode {
   // prompt passes and sampling settings: device copies and their pinned sources
   unsigned char *prompt_dev = nullptr, *prompt_host = nullptr;
   float *samp_dev = nullptr, *samp_host = nullptr;  // u | temperature | top_p | min_p | top_k
-  cudaEvent_t inputs_read = nullptr;  // a call's copies out of pinned memory
+  cudaEvent_t inputs_read = nullptr;  // expert parallelism: a step's copies out of pinned memory
   // QKV and output projections on this library's tcgen05 kernel (one "expert" = all rows)
   bool own_gemm = true;
   int num_sms = 0, sched_B = -1, sched_cap = 0;
@@ -1201,7 +1201,7 @@ static int launch_step(gptoss_decode *h, const int *tokens, const int *pos, int 
   DCK(h, cudaMemcpyAsync(h->d_pos, hp + h->max_batch, B * sizeof(int), cudaMemcpyHostToDevice, st));
   gptoss_sample_args_t draw = {};
   if (sampling && (rc = upload_sampling(h, sampling, B, &draw, st))) return rc;
-  DCK(h, cudaEventRecord(h->inputs_read, st));
+  if (h->moe->ep_size > 1) DCK(h, cudaEventRecord(h->inputs_read, st));  // see after_failure
   if ((rc = run_layers(h, B, h->d_tokens, h->d_pos, nullptr, st))) return rc;
   return finish_rows(h, h->x, B, h->d_pos, sampling ? &draw : nullptr, st);
 }
@@ -1270,7 +1270,6 @@ static int launch_prefill(gptoss_decode *h, const int *tokens, const int *rows, 
     }
     host(at.q_start)[pass.seqs] = pass.tokens;
     DCK(h, cudaMemcpyAsync(dp, hp, at.bytes, cudaMemcpyHostToDevice, st));
-    DCK(h, cudaEventRecord(h->inputs_read, st));
     pass.slots = reinterpret_cast<const long long *>(dp + at.slots);
     pass.kv_start = reinterpret_cast<const long long *>(dp + at.kv_start);
     pass.q_start = dev(at.q_start);
